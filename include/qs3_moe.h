@@ -99,7 +99,12 @@ typedef enum { /* upstream qs_tensor.h:15-29 */
 QS3_DECLARE_TENSOR(1);
 QS3_DECLARE_TENSOR(2);
 QS3_DECLARE_TENSOR(3);
+QS3_DECLARE_TENSOR(4); /* additive: the pools of a paged KV cache */
 #undef QS3_DECLARE_TENSOR
+
+/* Additive element types of index and table tensors (qsfi_dtype values upstream does not use). */
+#define QS3_DTYPE_I64 100
+#define QS3_DTYPE_F64 101
 
 /* --------------------------------------------------------------- context -- */
 
@@ -929,6 +934,101 @@ qsfi_status qs3_checkpoint_load_moe_layer(
     qsfi_context* ctx, const qs3_checkpoint* checkpoint, const qs3_moe_layer_load_desc* desc,
     void* weights, size_t weight_bytes, void* scratch, size_t scratch_bytes, qs3_moe_layer_weights* out
 );
+
+/* ---- gated attention between its projections and its output: rotary positions, the paged KV cache as it is written
+ * and read back, attention of new tokens over it (upstream: FlashInfer calls, qsfi_attn.cu and qsfi_norm_rope.cu; the
+ * page table is upstream's CSR one, src/runtime.rs:99-181). Tensors have a contiguous innermost dimension, 16-byte
+ * aligned rows and any other strides. head_dim is a multiple of 8 up to 256. ---- */
+
+/* Rotary positions. Element pairs of the first r = 2 * inv_freq.shape[0] elements of every head are turned by the angle
+ * positions[t] * inv_freq[j]:
+ *   (x, y) -> scale * (x cos - y sin, y cos + x sin),
+ * with pairs (j, j + r/2), or (2j, 2j + 1) when `interleaved`; the rest of the head is passed through. Angles are reduced
+ * in 64 bits, sine, cosine and products are in 32, rounded once. */
+typedef struct {
+    qsfi_tensor3 q;         /* bf16 or f32 [tokens, heads, head_dim] */
+    qsfi_tensor3 k;         /* optional, same type [tokens, kv_heads, head_dim] */
+    qsfi_tensor3 q_out;     /* same shape; absent: q is turned in place. May be q; may not overlap it otherwise */
+    qsfi_tensor3 k_out;     /* likewise for k */
+    qsfi_tensor1 positions; /* i32 or i64 [tokens] */
+    qsfi_tensor1 inv_freq;  /* f64 [r / 2], radians per position */
+    float scale;            /* factor on sine and cosine; 0 means 1 */
+    uint32_t interleaved;
+} qs3_rope_desc;
+qsfi_status qs3_rope(qsfi_context* ctx, const qs3_rope_desc* desc);
+
+/* A pool of pages. bf16, or e4m3 codes with one f32 scale per token and KV head:
+ *   scale = max(amax / 448, 1e-30),  code = e4m3_rn_sat(x * (1 / scale)).
+ * A row with an infinity or a NaN reads back as NaNs. Codes 0x7f and 0xff, which no append writes beside a finite scale, count
+ * as +-480 in attention. */
+typedef struct {
+    qsfi_tensor4 k, v;             /* bf16 or e4m3 [pages, kv_heads, page_size, head_dim] */
+    qsfi_tensor3 k_scale, v_scale; /* e4m3: f32 [pages, kv_heads, page_size] */
+} qs3_paged_kv_cache;
+
+/* Token p of sequence b lies in slot p % page_size of page kv_indices[kv_indptr[b] + p / page_size]. At most 4096 sequences.
+ * The tables are read on the device. A page id outside the pool and a length beyond a sequence's pages are not followed:
+ * such tokens count as zeros, or as absent, and qs3_moe_check_device_error reports 0x5b000001. */
+typedef struct {
+    qsfi_tensor1 kv_indptr;  /* i32 [batch + 1], ascending */
+    qsfi_tensor1 kv_indices; /* i32 */
+    qsfi_tensor1 kv_len;     /* i32 [batch]: tokens of each sequence, those of the present step included */
+} qs3_page_table;
+
+/* Writes k and v of the new tokens into the cache. Rows q_indptr[b] .. q_indptr[b + 1] belong to sequence b (absent: row b
+ * does), the i-th of n of them is token kv_len[b] - n + i; a row without one (n > kv_len[b], or behind the last sequence)
+ * is left out. With inv_freq, k is turned on the way (before it is quantised) and, where given, q as well. */
+typedef struct {
+    qs3_paged_kv_cache cache;
+    qs3_page_table table;
+    qsfi_tensor1 q_indptr;  /* optional i32 [batch + 1], ascending from 0 */
+    qsfi_tensor3 k, v;      /* bf16 [rows, kv_heads, head_dim] */
+    qsfi_tensor3 q, q_out;  /* optional, with inv_freq: as in qs3_rope_desc; rows left out are not written */
+    qsfi_tensor1 positions; /* optional i32 or i64 [rows]: angles go by these and not by the place in the cache */
+    qsfi_tensor1 inv_freq;  /* optional f64 [r / 2] */
+    float rope_scale;       /* 0 means 1 */
+    uint32_t interleaved;
+} qs3_kv_append_desc;
+qsfi_status qs3_kv_append(qsfi_context* ctx, const qs3_kv_append_desc* desc);
+
+/* Reads the cache back: row out_indptr[b] + i of k_out and v_out becomes token kv_start[b] + i of sequence b, up to
+ * out_indptr[b + 1] and kv_len[b]; other rows are left as they are. */
+typedef struct {
+    qs3_paged_kv_cache cache;
+    qs3_page_table table;
+    qsfi_tensor1 kv_start;     /* optional i32 [batch], zeros when absent */
+    qsfi_tensor1 out_indptr;   /* i32 [batch + 1], ascending from 0 */
+    qsfi_tensor3 k_out, v_out; /* bf16 [rows, kv_heads, head_dim] */
+} qs3_kv_gather_desc;
+qsfi_status qs3_kv_gather(qsfi_context* ctx, const qs3_kv_gather_desc* desc);
+
+/* Attention of new tokens over the cache, which holds them already:
+ *   s_j = sm_scale * q . k_j,  out = sum_j softmax(s)_j v_j,  lse = log sum_j exp(s_j)
+ * over the tokens j that row i of n of sequence b sees: with p = kv_len[b] - n + i all j <= p (causal; else all
+ * j < kv_len[b]), and j > p - window where there is one. A row that sees none gets 0 and -infinity. Query heads
+ * h * group .. h * group + group - 1 share KV head h. Head sizes 64, 128 and 256. Sums, maxima and the exponents are in
+ * 32 bits; the weights exp(s_j - max) are rounded to bf16 for the product with v. Values of v at tokens that only some rows
+ * of a tile see have to be finite, as 0 * inf is NaN; what lies in the pages behind a sequence's end does not matter. */
+typedef struct {
+    qsfi_tensor3 q; /* bf16 [rows, heads, head_dim], heads a multiple of kv_heads */
+    qs3_paged_kv_cache cache;
+    qs3_page_table table;
+    qsfi_tensor1 q_indptr;  /* optional i32 [batch + 1], ascending from 0; absent: row b belongs to sequence b */
+    qsfi_tensor3 out;       /* bf16 [rows, heads, head_dim]; rows behind the last sequence are left as they are */
+    qsfi_tensor2 lse;       /* optional f32 [rows, heads] */
+    qsfi_tensor1 workspace; /* u8, qs3_paged_attention_workspace_size bytes, 256-byte aligned; calls that may overlap on
+                               the device need one each */
+    float sm_scale;         /* 0 means 1 / sqrt(head_dim) */
+    uint32_t causal;
+    uint32_t window;        /* 0: none; needs causal */
+    uint32_t max_q_len;     /* most new tokens of one sequence; 0: unknown. A larger number costs time, a smaller one too:
+                               results do not depend on it */
+    uint32_t max_kv_len;    /* likewise for kv_len */
+} qs3_paged_attention_desc;
+qsfi_status qs3_paged_attention_workspace_size(
+    qsfi_context* ctx, uint32_t rows, uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, size_t* bytes
+);
+qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_desc* desc);
 
 #ifdef __cplusplus
 }

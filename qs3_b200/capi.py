@@ -39,6 +39,8 @@ DTYPE_I32 = 9
 DTYPE_U32 = 10
 DTYPE_I8 = 11
 DTYPE_U8 = 12
+DTYPE_I64 = 100  # QS3_DTYPE_I64
+DTYPE_F64 = 101  # QS3_DTYPE_F64
 
 MOE_BACKEND_STAGED_BF16 = 1
 MOE_BACKEND_FUSED_BF16 = 2
@@ -66,6 +68,7 @@ def _tensor(rank):
 Tensor1 = _tensor(1)
 Tensor2 = _tensor(2)
 Tensor3 = _tensor(3)
+Tensor4 = _tensor(4)
 
 
 class ContextDesc(C.Structure):
@@ -209,6 +212,36 @@ class RouteSortStaticDesc(C.Structure):
                 ("local_expert_offset", C.c_uint32), ("local_num_experts", C.c_uint32)]
 
 
+class RopeDesc(C.Structure):
+    _fields_ = [("q", Tensor3), ("k", Tensor3), ("q_out", Tensor3), ("k_out", Tensor3), ("positions", Tensor1),
+                ("inv_freq", Tensor1), ("scale", C.c_float), ("interleaved", C.c_uint32)]
+
+
+class PagedKvCache(C.Structure):
+    _fields_ = [("k", Tensor4), ("v", Tensor4), ("k_scale", Tensor3), ("v_scale", Tensor3)]
+
+
+class PageTable(C.Structure):
+    _fields_ = [("kv_indptr", Tensor1), ("kv_indices", Tensor1), ("kv_len", Tensor1)]
+
+
+class KvAppendDesc(C.Structure):
+    _fields_ = [("cache", PagedKvCache), ("table", PageTable), ("q_indptr", Tensor1), ("k", Tensor3), ("v", Tensor3),
+                ("q", Tensor3), ("q_out", Tensor3), ("positions", Tensor1), ("inv_freq", Tensor1),
+                ("rope_scale", C.c_float), ("interleaved", C.c_uint32)]
+
+
+class KvGatherDesc(C.Structure):
+    _fields_ = [("cache", PagedKvCache), ("table", PageTable), ("kv_start", Tensor1), ("out_indptr", Tensor1),
+                ("k_out", Tensor3), ("v_out", Tensor3)]
+
+
+class PagedAttentionDesc(C.Structure):
+    _fields_ = [("q", Tensor3), ("cache", PagedKvCache), ("table", PageTable), ("q_indptr", Tensor1), ("out", Tensor3),
+                ("lse", Tensor2), ("workspace", Tensor1), ("sm_scale", C.c_float), ("causal", C.c_uint32),
+                ("window", C.c_uint32), ("max_q_len", C.c_uint32), ("max_kv_len", C.c_uint32)]
+
+
 # Every symbol include/qs3_moe.h declares: (restype, argtypes)
 _P = C.POINTER
 class Fp8QuantizeWeightDesc(C.Structure):
@@ -339,6 +372,11 @@ _SIGNATURES = {
     "qsfi_rmsnorm": (C.c_int, [C.c_void_p, _P(RmsnormDesc)]),
     "qsfi_fused_add_rmsnorm": (C.c_int, [C.c_void_p, _P(FusedAddRmsnormDesc)]),
     "qs3_fused_add_rmsnorm_nvfp4": (C.c_int, [C.c_void_p, _P(FusedAddRmsnormNvfp4Desc)]),
+    "qs3_rope": (C.c_int, [C.c_void_p, _P(RopeDesc)]),
+    "qs3_kv_append": (C.c_int, [C.c_void_p, _P(KvAppendDesc)]),
+    "qs3_kv_gather": (C.c_int, [C.c_void_p, _P(KvGatherDesc)]),
+    "qs3_paged_attention_workspace_size": (C.c_int, [C.c_void_p] + [C.c_uint32] * 5 + [_P(C.c_size_t)]),
+    "qs3_paged_attention": (C.c_int, [C.c_void_p, _P(PagedAttentionDesc)]),
     "qs3_moe_ep_pull_routed": (C.c_int, [C.c_void_p, _P(MoeEpPullRoutedDesc)]),
     "qs3_moe_ep_barrier": (C.c_int, [C.c_void_p, _P(MoeEpBarrierDesc)]),
     "qs3_moe_read_device_error": (C.c_int, [C.c_void_p, _P(C.c_uint32)]),

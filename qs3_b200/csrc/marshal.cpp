@@ -30,6 +30,8 @@ int32_t dtype_code(at::ScalarType t)
     case at::kChar: return QSFI_DTYPE_I8;
     case at::kByte: return QSFI_DTYPE_U8;
     case at::kFloat8_e4m3fn: return QSFI_DTYPE_FP8_E4M3;
+    case at::kLong: return QS3_DTYPE_I64;
+    case at::kDouble: return QS3_DTYPE_F64;
     default: return 0;
     }
 }
@@ -91,8 +93,10 @@ PyObject* fill_checked(PyObject* const* args, Py_ssize_t nargs)
             put<qsfi_tensor1, 1>(at_, t, dtype);
         } else if (rank == 2) {
             put<qsfi_tensor2, 2>(at_, t, dtype);
-        } else {
+        } else if (rank == 3) {
             put<qsfi_tensor3, 3>(at_, t, dtype);
+        } else {
+            put<qsfi_tensor4, 4>(at_, t, dtype);
         }
     }
     return PyLong_FromLong(-1);

@@ -1,0 +1,98 @@
+// Views of a paged KV cache and its page table, shared by the kernels that write it, read it back and attend over it.
+#pragma once
+
+#include "common.cuh"
+#include "paged_schedule.h"
+
+namespace qs3 {
+
+// Codes in the device error word: a page id outside the pool, or a sequence longer than its pages.
+enum : uint32_t { ERR_PAGE_TABLE = 0x5b000001u };
+
+constexpr uint32_t kMaxHeadDim = 256;
+constexpr uint32_t kMaxBatch = 4096;
+
+// Pages of [kv_heads, page_size, head_dim] elements; strides in bytes, scales in elements.
+struct PagedPool {
+    uint8_t* data;
+    int64_t page_stride, head_stride, slot_stride;
+    float* scale;
+    int64_t scale_page_stride, scale_head_stride, scale_slot_stride;
+};
+
+struct PagedView {
+    PagedPool k, v;
+    uint32_t pages, kv_heads, page_size, head_dim;
+    FastDiv page_div;
+    const int32_t* indptr;  // [batch + 1]
+    const int32_t* indices; // [num_indices]
+    const int32_t* length;  // [batch]
+    uint32_t batch, num_indices;
+    uint32_t* err;
+};
+
+#ifdef __CUDACC__
+
+// Cached tokens of a sequence and where its page ids begin. Whatever the tables hold, the ids read for positions below the
+// returned length lie inside `indices`.
+struct SeqPages {
+    uint32_t first;  // index of the first page id
+    uint32_t length; // tokens
+};
+
+__device__ __forceinline__ SeqPages seq_pages(const PagedView& p, uint32_t seq)
+{
+    const int32_t a = p.indptr[seq], b = p.indptr[seq + 1], n = p.length[seq];
+    SeqPages s { 0, 0 };
+    if (n <= 0)
+        return s;
+    if (a >= 0 && b > a && static_cast<uint32_t>(a) < p.num_indices) {
+        const uint32_t end = min(static_cast<uint32_t>(b), p.num_indices);
+        const uint64_t room = static_cast<uint64_t>(end - a) * p.page_size;
+        s.first = static_cast<uint32_t>(a);
+        s.length = static_cast<uint32_t>(min(room, static_cast<uint64_t>(n)));
+    }
+    if (s.length != static_cast<uint32_t>(n))
+        atomicCAS(p.err, 0u, ERR_PAGE_TABLE);
+    return s;
+}
+
+// Page of position `pos` < length, and the slot in it; -1: the table names a page that is not there.
+__device__ __forceinline__ int32_t page_of(const PagedView& p, const SeqPages& s, uint32_t pos, uint32_t* slot)
+{
+    const uint32_t i = p.page_div.div(pos);
+    *slot = pos - i * p.page_size;
+    const int32_t page = __ldg(p.indices + s.first + i);
+    if (static_cast<uint32_t>(page) < p.pages)
+        return page;
+    atomicCAS(p.err, 0u, ERR_PAGE_TABLE);
+    return -1;
+}
+
+// Largest i in [0, n) with table[i] <= x, for ascending table[0 .. n] with table[0] <= x; the whole warp searches, 32 places
+// at a time. Any table gives an i in range.
+__device__ __forceinline__ uint32_t warp_upper(const int32_t* table, uint32_t n, int32_t x)
+{
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t lo = 0, len = n; // the answer is in [lo, lo + len)
+    while (len > 1) {
+        const uint32_t step = (len + 31) / 32;
+        const uint32_t at = lo + lane * step;
+        const bool le = lane * step < len && (lane == 0 || table[at] <= x);
+        const uint32_t last = 31 - __clz(__ballot_sync(0xffffffffu, le));
+        lo += last * step;
+        len = min(step, len - last * step);
+    }
+    return lo;
+}
+
+#endif
+
+// Host side: checks and views of the descriptors (kv_cache.cu).
+bool rows_apart(const qsfi_tensor3& t);
+qsfi_status check_rows(qsfi_context* ctx, const qsfi_tensor3& t, const char* op, const char* name, qsfi_dtype dtype);
+qsfi_status check_index(qsfi_context* ctx, const qsfi_tensor1& t, const char* op, const char* name, int64_t length);
+qsfi_status paged_view(qsfi_context* ctx, const qs3_paged_kv_cache& cache, const qs3_page_table& table, const char* op,
+                       PagedView* out, bool* fp8);
+
+} // namespace qs3

@@ -1,0 +1,101 @@
+// Division of attention over a paged cache into pieces of equal work. Arithmetic only, for the kernels and for the host.
+//
+// An item is a tile of query rows of one sequence and KV head: the rows of a sequence and KV head are its new tokens times the
+// query heads that share the KV head, row = token * group + head, cut into tiles of `tile_rows`. Its cost is the number of key
+// tiles that hold a key some row of it sees, at least one (an item without keys still writes its output). Items follow each
+// other by sequence, KV head, tile; their key tiles, laid end to end, are cut into equal ranges, one per block of the launch.
+// A range ends where it ends, inside an item as well, so that lengths which differ leave no block idle and a single long
+// context is spread over all SMs; an item cut this way leaves partial results that a second launch joins.
+#pragma once
+
+#include <cstdint>
+
+#ifdef __CUDACC__
+#define QS3_HD __host__ __device__ __forceinline__
+#else
+#define QS3_HD inline
+#endif
+
+namespace qs3 {
+
+// n / d for n < 2^31 by a multiplication: with s = ceil(log2 d), m = ceil(2^(31+s) / d) has an error below d / 2^(31+s), which
+// times n stays below 1/d.
+struct FastDiv {
+    uint32_t d, mul, shift;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t divisor) : d(divisor)
+    {
+        uint32_t s = 0;
+        while ((1ull << s) < divisor)
+            ++s;
+        mul = static_cast<uint32_t>(((1ull << (31 + s)) + divisor - 1) / divisor);
+        shift = s;
+    }
+    QS3_HD uint32_t div(uint32_t n) const
+    {
+        return static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> (31 + shift));
+    }
+};
+
+struct AttnTiling {
+    uint32_t group;     // query heads per KV head
+    uint32_t tile_rows; // rows of an item
+    uint32_t key_tile;  // keys of a key tile
+    uint32_t kv_heads;
+    uint32_t window;    // 0: none
+    uint32_t causal;
+};
+
+struct KeyTiles {
+    uint32_t first, end; // end > first
+};
+
+// Row tiles of a sequence with `fresh` new tokens.
+QS3_HD uint32_t row_tiles(const AttnTiling& a, uint32_t fresh)
+{
+    return static_cast<uint32_t>((static_cast<uint64_t>(fresh) * a.group + a.tile_rows - 1) / a.tile_rows);
+}
+
+// Keys [lo, hi) that new token `i` of `fresh` sees in a cache of `length` tokens (its own position: length - fresh + i).
+QS3_HD void visible_keys(const AttnTiling& a, uint32_t fresh, uint32_t length, uint32_t i, uint32_t* lo, uint32_t* hi)
+{
+    const int64_t pos = static_cast<int64_t>(length) - fresh + i;
+    const int64_t h = a.causal ? pos + 1 : static_cast<int64_t>(length);
+    *hi = h > 0 ? static_cast<uint32_t>(h) : 0;
+    const int64_t l = a.window != 0 ? pos - a.window + 1 : 0;
+    *lo = l <= 0 ? 0 : l < h ? static_cast<uint32_t>(l) : *hi;
+}
+
+QS3_HD KeyTiles key_tiles(const AttnTiling& a, uint32_t fresh, uint32_t length, uint32_t tile)
+{
+    const uint64_t rows = static_cast<uint64_t>(fresh) * a.group;
+    const uint64_t r0 = static_cast<uint64_t>(tile) * a.tile_rows;
+    const uint64_t r1 = (r0 + a.tile_rows < rows ? r0 + a.tile_rows : rows) - 1;
+    uint32_t lo, hi, unused;
+    visible_keys(a, fresh, length, static_cast<uint32_t>(r0 / a.group), &lo, &unused);
+    visible_keys(a, fresh, length, static_cast<uint32_t>(r1 / a.group), &unused, &hi);
+    KeyTiles k;
+    k.first = lo / a.key_tile;
+    k.end = (hi + a.key_tile - 1) / a.key_tile;
+    if (k.end <= k.first)
+        k.end = k.first + 1;
+    return k;
+}
+
+// Blocks that get work: every one at least `least` key tiles, as far as there are any.
+QS3_HD uint32_t active_blocks(uint64_t total, uint32_t blocks, uint32_t least)
+{
+    const uint64_t n = (total + least - 1) / least;
+    return n < blocks ? static_cast<uint32_t>(n) : blocks;
+}
+
+// First key tile of block `c` of `blocks`. (c * total stays below 2^63: total <= 2^52 and blocks < 2^11 by the limits of the entry point.)
+QS3_HD uint64_t block_begin(uint64_t total, uint32_t blocks, uint32_t c) { return total * c / blocks; }
+
+// Where a position in the row of all key tiles lies.
+struct AttnPlace {
+    uint32_t seq, head, tile;
+    uint32_t offset; // key tiles of the item before the position
+};
+
+} // namespace qs3

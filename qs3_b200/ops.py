@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
 import struct
 from dataclasses import dataclass
 
@@ -104,6 +105,26 @@ _QSCB_GEMM_DESC = _layout(capi.QscbGemmDesc, "x", "weight", "out")
 _RMSNORM_DESC = _layout(capi.RmsnormDesc, "x", "weight", "out")
 _FUSED_ADD_RMSNORM_DESC = _layout(capi.FusedAddRmsnormDesc, "x", "residual_inout", "weight", "out")
 _FUSED_ADD_RMSNORM_NVFP4_DESC = _layout(capi.FusedAddRmsnormNvfp4Desc, "packed", "scale_tiled")
+_ROPE_DESC = _layout(capi.RopeDesc, "q", "k", "q_out", "k_out", "positions", "inv_freq")
+
+
+def _paged_layout(cls, *fields):
+    """Layout of the cache and page table at the head of a descriptor (16-bit or 8-bit pools), then `fields`."""
+    def part(struct_cls, base, *names):
+        packed, ranks = _layout(struct_cls, *names)
+        moved = b"".join(struct.pack("3i", off + base, r, d) for off, r, d in struct.iter_unpack("3i", packed))
+        return moved, ranks
+    def whole(fp8):
+        pool = lambda n: (n, capi.DTYPE_FP8_E4M3 if fp8 else None)
+        parts = (part(capi.PagedKvCache, cls.cache.offset, pool("k"), pool("v"), "k_scale", "v_scale"),
+                 part(capi.PageTable, cls.table.offset, "kv_indptr", "kv_indices", "kv_len"), part(cls, 0, *fields))
+        return b"".join(p for p, _ in parts), sum((r for _, r in parts), [])
+    return whole(False), whole(True)
+
+
+_KV_APPEND_DESC = _paged_layout(capi.KvAppendDesc, "q_indptr", "k", "v", "q", "q_out", "positions", "inv_freq")
+_KV_GATHER_DESC = _paged_layout(capi.KvGatherDesc, "kv_start", "out_indptr", "k_out", "v_out")
+_PAGED_ATTENTION_DESC = _paged_layout(capi.PagedAttentionDesc, "q", "q_indptr", "out", "lse", "workspace")
 _ROUTE_SORT_STATIC_DESC = _layout(capi.RouteSortStaticDesc, "topk_ids", "topk_weights")
 
 
@@ -643,3 +664,145 @@ def fused_add_rmsnorm_nvfp4(ctx: Context, x, residual, weight, eps: float = 1e-6
     d.global_scale = global_scale
     ctx.check(ctx._lib.qs3_fused_add_rmsnorm_nvfp4(ctx.handle, C.byref(d)))
     return packed, tiled
+
+
+# ------------------------------------- rotary positions, paged KV cache, attention ---
+
+@dataclass
+class RotaryFrequencies:
+    """Rotary frequencies of a model: f64 ``inv_freq`` [rotary_dim / 2] in radians per position, and the
+    factor on sine and cosine that some long-context scalings come with."""
+    inv_freq: torch.Tensor
+    scale: float = 1.0
+
+
+def rope_frequencies(rotary_dim: int, theta: float = 10000.0, *, scaling: str = "none", factor: float = 1.0,
+                     original_length: int = 8192, low: float = 1.0, high: float = 4.0, beta_fast: float = 32.0,
+                     beta_slow: float = 1.0, scale: float | None = None, device=None) -> RotaryFrequencies:
+    """``theta ** (-2 j / rotary_dim)``, stretched for contexts ``factor`` times as long as the trained one:
+
+    ``linear``  every frequency divided by ``factor``;
+    ``ntk``     the base raised so that the lowest frequency is divided by ``factor`` and the highest stays;
+    ``yarn``    frequencies that make more than ``beta_fast`` turns in ``original_length`` positions stay, those that make
+                fewer than ``beta_slow`` are divided, those between are blended by their index; sine and cosine
+                are multiplied by ``scale`` (default ``0.1 ln(factor) + 1``);
+    ``llama3``  the same with the number of turns as the measure of the blend, from ``low`` to ``high`` of them.
+    """
+    if rotary_dim <= 0 or rotary_dim % 2 or not theta > 0 or not factor > 0:
+        raise Qs3Error(capi.STATUS_INVALID_ARGUMENT, "rotary_dim must be even and positive, theta and factor positive")
+    j = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    if scaling == "ntk":
+        if rotary_dim < 4:
+            raise Qs3Error(capi.STATUS_INVALID_ARGUMENT, "ntk scaling needs at least two frequencies")
+        theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+    freq = theta ** (-2.0 * j / rotary_dim)
+    turns = original_length * freq / (2 * math.pi)
+    factor_on_both = 1.0
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "yarn":
+        index_of = lambda n: rotary_dim * math.log(original_length / (n * 2 * math.pi)) / (2 * math.log(theta))
+        first, last = max(math.floor(index_of(beta_fast)), 0), min(math.ceil(index_of(beta_slow)), rotary_dim - 1)
+        ramp = ((j - first) / max(last - first, 0.001)).clamp(0, 1)
+        freq = freq / factor * ramp + freq * (1 - ramp)
+        factor_on_both = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    elif scaling == "llama3":
+        kept = ((turns - low) / (high - low)).clamp(0, 1)
+        freq = freq * kept + freq / factor * (1 - kept)
+    elif scaling not in ("none", "ntk"):
+        raise Qs3Error(capi.STATUS_UNSUPPORTED, f"unknown rope scaling {scaling!r}")
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+    return RotaryFrequencies(freq.to(device), factor_on_both if scale is None else scale)
+
+
+def rope(ctx: Context, positions, inv_freq, q, k=None, *, q_out=None, k_out=None, scale: float = 1.0,
+         interleaved: bool = False):
+    """``qs3_rope``: rotary positions (i32 or i64 [tokens]) on q and k (bf16 or f32 [tokens, heads, head_dim]); without
+    ``q_out`` / ``k_out`` in place. Pairs are ``(j, j + r/2)``, or ``(2 j, 2 j + 1)`` with ``interleaved``, of the first
+    ``r = 2 * len(inv_freq)`` elements; the others are passed through."""
+    d = capi.RopeDesc()
+    _fill(d, _ROPE_DESC, q, k, q_out, k_out, positions, inv_freq)
+    d.scale, d.interleaved = scale, 1 if interleaved else 0
+    ctx.check(ctx._lib.qs3_rope(ctx.handle, C.byref(d)))
+
+
+@dataclass
+class PagedKvCache:
+    """A pool of pages ``[pages, kv_heads, page_size, head_dim]``: bf16, or e4m3 codes (``float8_e4m3fn`` or u8) with f32
+    scales ``[pages, kv_heads, page_size]``. A pool laid out ``[pages, page_size, kv_heads, head_dim]`` is passed as its
+    ``transpose(1, 2)``."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor | None = None
+    v_scale: torch.Tensor | None = None
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, *, fp8: bool = False, device=None):
+        """A pool of that shape, its contents undefined."""
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+        new = lambda *shape, dtype: torch.empty(shape, dtype=dtype, device=device)
+        shape, dtype = (pages, kv_heads, page_size, head_dim), torch.float8_e4m3fn if fp8 else torch.bfloat16
+        scales = [new(*shape[:3], dtype=torch.float32) for _ in range(2)] if fp8 else (None, None)
+        return cls(new(*shape, dtype=dtype), new(*shape, dtype=dtype), *scales)
+
+    @property
+    def fp8(self) -> bool:
+        return self.k_scale is not None
+
+
+@dataclass
+class PageTable:
+    """CSR page table of a batch (i32): token p of sequence b lies in slot ``p % page_size`` of page
+    ``kv_indices[kv_indptr[b] + p // page_size]``; ``kv_len[b]`` counts its tokens, those of the present step included."""
+    kv_indptr: torch.Tensor
+    kv_indices: torch.Tensor
+    kv_len: torch.Tensor
+
+
+def _fill_paged(d, layouts, cache: PagedKvCache, table: PageTable, *tensors):
+    if cache.fp8 and not (cache.k.element_size() == cache.v.element_size() == 1):
+        raise Qs3Error(capi.STATUS_INVALID_ARGUMENT, "a cache with scales holds 8-bit codes")
+    _fill(d, layouts[1 if cache.fp8 else 0], cache.k, cache.v, cache.k_scale, cache.v_scale, table.kv_indptr,
+          table.kv_indices, table.kv_len, *tensors)
+
+
+def kv_append(ctx: Context, cache: PagedKvCache, table: PageTable, k, v, *, q_indptr=None, q=None, q_out=None,
+              positions=None, inv_freq=None, rope_scale: float = 1.0, interleaved: bool = False):
+    """``qs3_kv_append``: k and v (bf16 [rows, kv_heads, head_dim]) of the new tokens into the cache. Rows
+    ``q_indptr[b] .. q_indptr[b + 1]`` are the last tokens of sequence b (without ``q_indptr`` row b is). With ``inv_freq``
+    k is rotated on the way, and q as well (in place without ``q_out``), by the tokens' places in the cache or by
+    ``positions``."""
+    d = capi.KvAppendDesc()
+    _fill_paged(d, _KV_APPEND_DESC, cache, table, q_indptr, k, v, q, q_out, positions, inv_freq)
+    d.rope_scale, d.interleaved = rope_scale, 1 if interleaved else 0
+    ctx.check(ctx._lib.qs3_kv_append(ctx.handle, C.byref(d)))
+
+
+def kv_gather(ctx: Context, cache: PagedKvCache, table: PageTable, out_indptr, k_out, v_out, *, kv_start=None):
+    """``qs3_kv_gather``: rows ``out_indptr[b] .. out_indptr[b + 1]`` of k_out and v_out (bf16 [rows, kv_heads, head_dim])
+    become the tokens of sequence b from ``kv_start[b]`` (default 0) on; rows without one are left as they are."""
+    d = capi.KvGatherDesc()
+    _fill_paged(d, _KV_GATHER_DESC, cache, table, kv_start, out_indptr, k_out, v_out)
+    ctx.check(ctx._lib.qs3_kv_gather(ctx.handle, C.byref(d)))
+
+
+def paged_attention_workspace_size(ctx: Context, q, cache: PagedKvCache, *, batch: int) -> int:
+    """Bytes of workspace that :func:`paged_attention` needs for q (or any with fewer rows) and a batch."""
+    n = C.c_size_t(0)
+    ctx.check(ctx._lib.qs3_paged_attention_workspace_size(ctx.handle, q.shape[0], batch, q.shape[1], cache.k.shape[1],
+                                                          q.shape[2], C.byref(n)))
+    return n.value
+
+
+def paged_attention(ctx: Context, q, cache: PagedKvCache, table: PageTable, out, workspace, *, q_indptr=None,
+                    sm_scale: float | None = None, causal: bool = True, window: int = 0, max_q_len: int = 0,
+                    max_kv_len: int = 0, lse=None):
+    """``qs3_paged_attention``: attention of new tokens over the cache, which holds them already. q and out are bf16
+    [rows, heads, head_dim]; rows ``q_indptr[b] .. q_indptr[b + 1]`` are the last tokens of sequence b (without
+    ``q_indptr`` row b is). ``lse`` (f32 [rows, heads]) takes the log-sum-exp of each row. ``max_q_len`` and
+    ``max_kv_len``, where the host knows them, choose the kernels; results do not depend on them."""
+    d = capi.PagedAttentionDesc()
+    _fill_paged(d, _PAGED_ATTENTION_DESC, cache, table, q, q_indptr, out, lse, workspace)
+    d.sm_scale = 0.0 if sm_scale is None else sm_scale
+    d.causal, d.window, d.max_q_len, d.max_kv_len = 1 if causal else 0, window, max_q_len, max_kv_len
+    ctx.check(ctx._lib.qs3_paged_attention(ctx.handle, C.byref(d)))

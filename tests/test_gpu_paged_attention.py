@@ -1,0 +1,167 @@
+"""Attention of new tokens over a paged cache against the formula in 64 bits: head sizes, groups, types, page sizes, lengths
+from none to several splits, windows, rows that see nothing, stale memory around everything."""
+import math
+
+import pytest
+import torch
+
+from paged_helpers import attention_reference, check_attention, ints, make_case, run_attention
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from qs3_b200 import ops as m
+    return m
+
+
+@pytest.fixture(scope="module")
+def ctx(ops):
+    return ops.Context()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 4), (4, 2), (5, 1), (16, 2), (16, 1), (40, 2)])
+def test_single_tokens(ops, ctx, dim, fp8, heads, kv_heads):
+    kv = [0, 1, 2, 15, 16, 17, 63, 64, 65, 127, 129, 200, 1000, 0]
+    c = make_case(ops, [1] * len(kv), kv, heads=heads, kv_heads=kv_heads, dim=dim, fp8=fp8, seed=dim + heads, tail=2)
+    out, lse = run_attention(ops, ctx, c, decode=True)
+    check_attention(out, lse, c)
+    assert ctx.read_device_error() == 0
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("page", [1, 7, 16, 24, 128])
+def test_page_sizes(ops, ctx, page, fp8):
+    c = make_case(ops, [1, 3, 1, 9], [50, 131, 7, 300], heads=8, kv_heads=2, dim=128, page=page, fp8=fp8, seed=page)
+    out, lse = run_attention(ops, ctx, c)
+    check_attention(out, lse, c)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 2), (128, 32, 8), (128, 7, 1), (256, 16, 2), (256, 3, 3)])
+@pytest.mark.parametrize("q_len,kv_len", [
+    ([1, 0, 5, 33, 130], [1, 0, 700, 40, 130]),
+    ([300], [300]),
+    ([257, 1, 1], [1030, 513, 2]),
+    ([0, 0, 64, 0], [10, 0, 65, 0]),
+    ([2, 3, 4], [2000, 1, 3]),          # the second sequence has more new tokens than cache: its first rows see nothing
+])
+def test_chunks(ops, ctx, q_len, kv_len, dim, heads, kv_heads, fp8):
+    c = make_case(ops, q_len, kv_len, heads=heads, kv_heads=kv_heads, dim=dim, fp8=fp8, seed=len(q_len) + dim, tail=3)
+    out, lse = run_attention(ops, ctx, c)
+    check_attention(out, lse, c)
+    out2, _ = run_attention(ops, ctx, c, max_q_len=max(q_len), max_kv_len=max(kv_len))
+    check_attention(out2, None, c)
+
+
+@pytest.mark.parametrize("dim,fp8", [(64, False), (128, True), (256, False)])
+@pytest.mark.parametrize("window", [1, 5, 64, 100, 5000])
+def test_windows(ops, ctx, window, dim, fp8):
+    c = make_case(ops, [1, 90, 7, 200], [500, 300, 3, 200], heads=8, kv_heads=2, dim=dim, fp8=fp8, seed=window)
+    out, lse = run_attention(ops, ctx, c, window=window)
+    check_attention(out, lse, c, window=window)
+
+
+@pytest.mark.parametrize("dim,fp8", [(64, True), (128, False), (256, False)])
+def test_without_causal_mask(ops, ctx, dim, fp8):
+    c = make_case(ops, [1, 90, 7, 40], [500, 300, 3, 0], heads=8, kv_heads=2, dim=dim, fp8=fp8, seed=3)
+    out, lse = run_attention(ops, ctx, c, causal=False, sm_scale=0.05)
+    check_attention(out, lse, c, causal=False, scale=0.05)
+
+
+@pytest.mark.parametrize("dim,fp8,heads", [(64, False, 2), (128, False, 8), (128, True, 4), (256, False, 16), (256, True, 8)])
+@pytest.mark.parametrize("kv", [[9001], [64, 8192, 3], [4097, 0, 1, 6000]])
+def test_contexts_split_over_blocks(ops, ctx, kv, dim, fp8, heads):
+    c = make_case(ops, [1] * len(kv), kv, heads=heads, kv_heads=2, dim=dim, fp8=fp8, seed=sum(kv))
+    out, lse = run_attention(ops, ctx, c, decode=True)
+    check_attention(out, lse, c)
+
+
+def test_many_short_sequences(ops, ctx):
+    kv = [(37 * i) % 90 for i in range(700)]
+    c = make_case(ops, [1] * len(kv), kv, heads=4, kv_heads=2, dim=64, seed=1)
+    out, lse = run_attention(ops, ctx, c, decode=True)
+    check_attention(out, lse, c)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_layouts_and_strides(ops, ctx, fp8):
+    """A pool of [pages, slots, heads, dim], q and out inside wider rows, heads before tokens."""
+    c = make_case(ops, [4, 70], [200, 90], heads=8, kv_heads=2, dim=64, fp8=fp8, seed=5, slots_first=True, q_pad=64)
+    wide = torch.full((8, 74, 192), 7.0, dtype=torch.bfloat16, device="cuda")
+    out, lse = run_attention(ops, ctx, c, out=wide.transpose(0, 1)[..., 64:128])
+    check_attention(out, lse, c)
+    assert bool((wide[..., :64] == 7.0).all()) and bool((wide[..., 128:] == 7.0).all())
+
+
+def test_large_scores_and_minus_infinity(ops, ctx):
+    """Scores of several thousand, and keys of -infinity times a positive query: weights of exactly zero."""
+    c = make_case(ops, [1, 40], [70, 100], heads=4, kv_heads=2, dim=64, seed=6)
+    c.q.mul_(200.0)
+    check_attention(*run_attention(ops, ctx, c), c)
+    c = make_case(ops, [1, 1], [70, 100], heads=4, kv_heads=2, dim=64, seed=7)
+    c.q.abs_()
+    page, slot = int(c.table.kv_indices[0]), 3
+    c.cache.k[page, :, slot, 0] = -math.inf
+    c.keys[0][slot, :, 0] = -math.inf
+    out, lse = run_attention(ops, ctx, c, decode=True)
+    want, want_lse, bound, _ = attention_reference(c)
+    bound = torch.where(torch.isfinite(bound), bound, 2.0 ** -6 * c.values[0].abs().max())   # (the bound sums |k|)
+    assert bool(((out.double() - want).abs() <= bound).all()) and bool(torch.isfinite(lse).all())
+
+
+def test_pages_that_are_not_there(ops, ctx):
+    """Ids outside the pool and lengths beyond the pages are reported, touch nothing and leave the others' results alone."""
+    c = make_case(ops, [1, 1, 1], [100, 200, 300], heads=4, kv_heads=2, dim=64, seed=8)
+    good, _ = run_attention(ops, ctx, c, decode=True)
+    c.table.kv_indices[8] = 1 << 20
+    c.table.kv_len[2] = 5000
+    out, lse = run_attention(ops, ctx, c, decode=True)
+    # (the third sequence's result takes in the stale slots of its last page: its length says that they are tokens)
+    assert torch.equal(out[0], good[0]) and bool(torch.isfinite(out[1].float()).all())
+    assert ctx.read_device_error() == 0x5b000001
+    assert ctx.read_device_error() == 0
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_replayed_graph_follows_the_tables(ops, fp8):
+    """A captured call reads lengths and pages anew at each replay; two graphs may share one workspace."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        ctx = ops.Context()
+        cases = [make_case(ops, [1, 1, 1], kv, heads=16, kv_heads=2, dim=128, fp8=fp8, seed=9 + i)
+                 for i, kv in enumerate(([3000, 5, 700], [64, 2000, 1]))]
+        ws = torch.empty(ops.paged_attention_workspace_size(ctx, cases[0].q, cases[0].cache, batch=3), dtype=torch.uint8, device="cuda")
+        outs, graphs = [], []
+        for c in cases:
+            out = torch.zeros_like(c.q)
+            ops.paged_attention(ctx, c.q, c.cache, c.table, out, ws)
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                ops.paged_attention(ctx, c.q, c.cache, c.table, out, ws)
+            outs.append(out)
+            graphs.append(graph)
+        for short in (False, True):
+            if short:
+                for c in cases:
+                    c.kv_len = [max(1, n // 3) for n in c.kv_len]
+                    c.table.kv_len.copy_(ints(c.kv_len))
+                    c.keys, c.values = ([x[:n] for x, n in zip(v, c.kv_len)] for v in (c.keys, c.values))
+            for out, graph in zip(outs, graphs):
+                out.fill_(7.0)
+                graph.replay()
+            stream.synchronize()
+            for c, out in zip(cases, outs):
+                check_attention(out, None, c)
+
+
+def test_results_do_not_depend_on_the_run(ops, ctx):
+    c = make_case(ops, [1, 300, 20], [9000, 300, 2222], heads=16, kv_heads=2, dim=128, seed=10)
+    first = run_attention(ops, ctx, c)
+    for _ in range(3):
+        again = run_attention(ops, ctx, c)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])

@@ -1,0 +1,290 @@
+"""The paged cache's operators without a GPU: the arithmetic that cuts a batch into ranges of key tiles (compiled for the host),
+and the refusals, which come before any device addressing (made-up device pointers)."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+
+from qs3_b200 import capi
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "qs3_b200", "csrc")
+
+PROGRAM = r"""
+#include "paged_schedule.h"
+#include <cstdio>
+#include <cstdlib>
+#include <initializer_list>
+using namespace qs3;
+#define CHECK(x) do { if (!(x)) { std::printf("line %d: %s\n", __LINE__, #x); return 1; } } while (0)
+int main()
+{
+    // division by multiplication, at the places where it could round wrongly
+    for (uint32_t d = 1; d < 5000; d = d < 70 ? d + 1 : d * 5 / 4 + 1) {
+        const FastDiv f(d);
+        for (uint64_t k = 0; k * d < (1ull << 31); k = k < 100 ? k + 1 : k + (1ull << 31) / d / 97 + 1)
+            for (int64_t n : { int64_t(k * d) - 1, int64_t(k * d), int64_t(k * d) + 1 })
+                if (n >= 0 && n < (int64_t(1) << 31))
+                    CHECK(f.div(uint32_t(n)) == uint32_t(n) / d);
+        CHECK(f.div(0x7fffffffu) == 0x7fffffffu / d);
+    }
+    // every key that a row sees lies in its item's key tiles, every key tile holds one, an item has one at least
+    for (uint32_t group : { 1u, 2u, 5u, 16u })
+    for (uint32_t rows : { 8u, 16u, 128u })
+    for (uint32_t keys : { 64u, 128u })
+    for (uint32_t window : { 0u, 1u, 7u, 200u })
+    for (uint32_t causal : { 0u, 1u })
+    for (uint32_t fresh : { 1u, 2u, 3u, 70u, 257u })
+    for (uint32_t length : { 0u, 1u, 2u, 63u, 64u, 65u, 300u, 1000u }) {
+        if (window != 0 && causal == 0)
+            continue;
+        const AttnTiling a { group, rows, keys, 2, window, causal };
+        const uint32_t tiles = row_tiles(a, fresh);
+        CHECK(uint64_t(tiles) * rows >= uint64_t(fresh) * group && uint64_t(tiles - 1) * rows < uint64_t(fresh) * group);
+        for (uint32_t t = 0; t < tiles; ++t) {
+            const KeyTiles k = key_tiles(a, fresh, length, t);
+            CHECK(k.end > k.first);
+            uint32_t low = ~0u, high = 0;
+            for (uint32_t r = t * rows; r < (t + 1) * rows && r < fresh * group; ++r) {
+                uint32_t lo, hi;
+                visible_keys(a, fresh, length, r / group, &lo, &hi);
+                const int64_t pos = int64_t(length) - fresh + r / group;
+                for (int64_t j = 0; j < length; ++j) {
+                    const bool seen = (!causal || j <= pos) && (!window || j > pos - int64_t(window));
+                    CHECK(seen == (j >= lo && j < hi));
+                }
+                if (hi > lo) {
+                    low = lo < low ? lo : low;
+                    high = hi > high ? hi : high;
+                }
+            }
+            if (high > 0)
+                CHECK(k.first <= low / keys && k.end == (high + keys - 1) / keys);
+        }
+    }
+    // ranges follow each other, hold everything and differ by one at most
+    for (uint64_t total : { 1ull, 2ull, 147ull, 148ull, 149ull, 12345ull, 1ull << 52 })
+        for (uint32_t blocks : { 1u, 148u, 1184u })
+            for (uint32_t least : { 1u, 2u, 5u }) {
+                const uint32_t n = active_blocks(total, blocks, least);
+                CHECK(n >= 1 && n <= blocks && block_begin(total, n, 0) == 0 && block_begin(total, n, n) == total);
+                for (uint32_t c = 0; c < n; ++c) {
+                    const uint64_t size = block_begin(total, n, c + 1) - block_begin(total, n, c);
+                    CHECK(size == total / n || size == total / n + 1);
+                }
+            }
+    return 0;
+}
+"""
+
+
+def test_division_into_ranges(tmp_path):
+    src, exe = tmp_path / "schedule.cpp", tmp_path / "schedule"
+    src.write_text(PROGRAM)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-Werror", f"-I{CSRC}", str(src), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout
+
+
+BF16, F32, I32, I64, U8, F64, E4M3 = (capi.DTYPE_BF16, capi.DTYPE_F32, capi.DTYPE_I32, capi.DTYPE_I64, capi.DTYPE_U8,
+                                      capi.DTYPE_F64, capi.DTYPE_FP8_E4M3)
+
+
+def t(dtype, *shape, ptr=0x10000, stride=None):
+    d = (capi.Tensor1, capi.Tensor2, capi.Tensor3, capi.Tensor4)[len(shape) - 1]()
+    d.data, d.dtype = ptr, dtype
+    strides = [1] * len(shape)
+    for i in range(len(shape) - 2, -1, -1):
+        strides[i] = strides[i + 1] * max(1, shape[i + 1])
+    for i, n in enumerate(shape):
+        d.shape[i] = n
+        d.stride[i] = strides[i] if stride is None else stride[i]
+    return d
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return capi.load()
+
+
+@pytest.fixture()
+def ctx(lib):
+    handle = C.c_void_p()
+    desc = capi.ContextDesc(-1, None)
+    assert lib.qsfi_context_create(C.byref(desc), C.byref(handle)) == capi.STATUS_OK
+    yield handle
+    lib.qsfi_context_destroy(handle)
+
+
+def refused(lib, ctx, fn, desc, status, fragment):
+    assert getattr(lib, fn)(ctx, C.byref(desc)) == status, fragment
+    info = capi.ErrorInfo()
+    lib.qsfi_context_get_last_error(ctx, C.byref(info))
+    assert info.status == status and fragment in info.message.decode(), (fragment, info.message.decode())
+
+
+INVALID, UNSUPPORTED = capi.STATUS_INVALID_ARGUMENT, capi.STATUS_UNSUPPORTED
+
+
+def test_null_arguments(lib, ctx):
+    for fn in ("qs3_rope", "qs3_kv_append", "qs3_kv_gather", "qs3_paged_attention"):
+        assert getattr(lib, fn)(None, None) == INVALID
+        assert getattr(lib, fn)(ctx, None) == INVALID
+
+
+def rope_desc(**kw):
+    d = capi.RopeDesc()
+    d.q, d.positions, d.inv_freq, d.scale = t(BF16, 4, 2, 64), t(I32, 4), t(F64, 16), 1.0
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("kw,status,fragment", [
+    (dict(q=t(BF16, 4, 2, 64, ptr=0)), INVALID, "q.data must not be null"),
+    (dict(q=t(U8, 4, 2, 64)), UNSUPPORTED, "bf16/f32"),
+    (dict(q=t(BF16, 4, 2, 60)), INVALID, "16-byte aligned rows"),
+    (dict(q=t(F32, 4, 2, 60)), UNSUPPORTED, "multiple of 8"),
+    (dict(q=t(BF16, 4, 2, 264)), UNSUPPORTED, "at most 256"),
+    (dict(q=t(BF16, 0, 2, 64)), INVALID, "positive"),
+    (dict(q=t(BF16, 4, 2, 64, ptr=0x10008)), INVALID, "16-byte aligned rows"),
+    (dict(q=t(BF16, 4, 2, 64, stride=(128, 64, 2))), INVALID, "contiguous head dimension"),
+    (dict(q=t(BF16, 4, 2, 64, stride=(0, 64, 1))), INVALID, "must not overlap"),
+    (dict(q=t(BF16, 4, 2, 64, stride=(64, 64, 1))), INVALID, "must not overlap"),
+    (dict(k=t(BF16, 5, 2, 64)), INVALID, "same tokens"),
+    (dict(k=t(F32, 4, 2, 64)), INVALID, "k dtype"),
+    (dict(k_out=t(BF16, 4, 2, 64)), INVALID, "k_out needs k"),
+    (dict(q_out=t(BF16, 4, 3, 64)), INVALID, "shape must match"),
+    (dict(q_out=t(F32, 4, 2, 64)), INVALID, "q_out dtype"),
+    (dict(q_out=t(BF16, 4, 2, 64, ptr=0x10010)), INVALID, "overlaps its input"),
+    (dict(positions=t(I32, 4, ptr=0)), INVALID, "positions.data"),
+    (dict(positions=t(F32, 4)), INVALID, "i32 or i64"),
+    (dict(positions=t(I64, 3)), INVALID, "one per row"),
+    (dict(inv_freq=t(F32, 16)), INVALID, "f64"),
+    (dict(inv_freq=t(F64, 33)), INVALID, "between 1 and head_dim / 2"),
+    (dict(scale=float("nan")), INVALID, "finite"),
+])
+def test_rope_refusals(lib, ctx, kw, status, fragment):
+    refused(lib, ctx, "qs3_rope", rope_desc(**kw), status, fragment)
+
+
+def cache(fp8=False, pages=10, heads=2, page=16, dim=64, **kw):
+    c = capi.PagedKvCache()
+    c.k = c.v = t(E4M3 if fp8 else BF16, pages, heads, page, dim)
+    if fp8:
+        c.k_scale = c.v_scale = t(F32, pages, heads, page)
+    for k, v in kw.items():
+        setattr(c, k, v)
+    return c
+
+
+def table(batch=3, **kw):
+    p = capi.PageTable()
+    p.kv_indptr, p.kv_indices, p.kv_len = t(I32, batch + 1), t(I32, 8), t(I32, batch)
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+PAGED = [
+    (dict(cache=cache(k=t(BF16, 10, 2, 16, 64, ptr=0))), INVALID, "must not be null"),
+    (dict(cache=cache(k=t(F32, 10, 2, 16, 64))), UNSUPPORTED, "bf16 and e4m3"),
+    (dict(cache=cache(v=t(E4M3, 10, 2, 16, 64))), INVALID, "same dtype"),
+    (dict(cache=cache(v=t(BF16, 10, 2, 8, 64))), INVALID, "same shape"),
+    (dict(cache=cache(k=t(BF16, 10, 0, 16, 64))), INVALID, "positive"),
+    (dict(cache=cache(k=t(BF16, 10, 2, 16, 64, ptr=0x10004))), INVALID, "16-byte aligned rows"),
+    (dict(cache=cache(k=t(BF16, 10, 2, 16, 64, stride=(2048, 1024, 60, 1)))), INVALID, "16-byte aligned rows"),
+    (dict(cache=cache(fp8=True, k_scale=t(F32, 10, 2, 16, ptr=0))), INVALID, "needs f32 k_scale"),
+    (dict(cache=cache(fp8=True, v_scale=t(F32, 10, 2, 8))), INVALID, "k_scale and v_scale must be"),
+    (dict(cache=cache(k_scale=t(F32, 10, 2, 16))), INVALID, "takes no scales"),
+    (dict(table=table(kv_len=t(I64, 3))), INVALID, "kv_len must be i32"),
+    (dict(table=table(kv_indptr=t(I32, 3))), INVALID, "kv_indptr must be contiguous"),
+    (dict(table=table(kv_indices=t(I32, 8, ptr=0))), INVALID, "kv_indices.data"),
+    (dict(table=table(batch=4097)), UNSUPPORTED, "at most 4096"),
+]
+
+
+def append_desc(**kw):
+    d = capi.KvAppendDesc()
+    d.cache, d.table, d.k, d.v, d.rope_scale = cache(), table(), t(BF16, 3, 2, 64), t(BF16, 3, 2, 64), 1.0
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("kw,status,fragment", PAGED + [
+    (dict(cache=cache(dim=12)), UNSUPPORTED, "multiple of 8"),
+    (dict(cache=cache(fp8=True, dim=24)), UNSUPPORTED, "multiple of 16"),
+    (dict(k=t(BF16, 3, 1, 64)), INVALID, "of the cache"),
+    (dict(v=t(BF16, 4, 2, 64)), INVALID, "of the cache"),
+    (dict(k=t(F32, 3, 2, 64)), INVALID, "k dtype"),
+    (dict(k=t(BF16, 2, 2, 64), v=t(BF16, 2, 2, 64)), INVALID, "a row per sequence"),
+    (dict(q_indptr=t(I32, 3)), INVALID, "q_indptr"),
+    (dict(q=t(BF16, 3, 4, 64)), INVALID, "need inv_freq"),
+    (dict(positions=t(I32, 3)), INVALID, "need inv_freq"),
+    (dict(inv_freq=t(F64, 33)), INVALID, "between 1"),
+    (dict(inv_freq=t(F64, 8), q=t(BF16, 2, 4, 64)), INVALID, "rows and head_dim of k"),
+    (dict(inv_freq=t(F64, 8), q_out=t(BF16, 3, 4, 64)), INVALID, "q_out needs q"),
+    (dict(inv_freq=t(F64, 8), positions=t(I32, 2)), INVALID, "one per row"),
+])
+def test_append_refusals(lib, ctx, kw, status, fragment):
+    refused(lib, ctx, "qs3_kv_append", append_desc(**kw), status, fragment)
+
+
+def gather_desc(**kw):
+    d = capi.KvGatherDesc()
+    d.cache, d.table, d.out_indptr, d.k_out, d.v_out = cache(), table(), t(I32, 4), t(BF16, 9, 2, 64), t(BF16, 9, 2, 64)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("kw,status,fragment", PAGED + [
+    (dict(out_indptr=t(I32, 3)), INVALID, "out_indptr"),
+    (dict(kv_start=t(I32, 2)), INVALID, "kv_start"),
+    (dict(v_out=t(BF16, 8, 2, 64)), INVALID, "of the cache"),
+    (dict(k_out=t(BF16, 9, 2, 64, stride=(64, 64, 1))), INVALID, "of the cache"),
+    (dict(k_out=t(F32, 9, 2, 64)), INVALID, "k_out dtype"),
+])
+def test_gather_refusals(lib, ctx, kw, status, fragment):
+    refused(lib, ctx, "qs3_kv_gather", gather_desc(**kw), status, fragment)
+
+
+def attention_desc(**kw):
+    d = capi.PagedAttentionDesc()
+    d.q, d.out, d.cache, d.table, d.causal = t(BF16, 3, 4, 64), t(BF16, 3, 4, 64), cache(), table(), 1
+    d.workspace = t(U8, 1 << 30)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("kw,status,fragment", PAGED + [
+    (dict(cache=cache(dim=96), q=t(BF16, 3, 4, 96), out=t(BF16, 3, 4, 96)), UNSUPPORTED, "64, 128 or 256"),
+    (dict(q=t(BF16, 3, 4, 128)), INVALID, "cache's head_dim"),
+    (dict(q=t(F32, 3, 4, 64)), INVALID, "q dtype"),
+    (dict(out=t(BF16, 3, 2, 64)), INVALID, "out shape"),
+    (dict(out=t(BF16, 3, 4, 64, stride=(64, 64, 1))), INVALID, "must not overlap"),
+    (dict(q=t(BF16, 3, 3, 64), out=t(BF16, 3, 3, 64)), INVALID, "multiple of kv_heads"),
+    (dict(q=t(BF16, 2, 4, 64), out=t(BF16, 2, 4, 64)), INVALID, "a row per sequence"),
+    (dict(q=t(BF16, 1 << 25, 4, 64), out=t(BF16, 1 << 25, 4, 64)), UNSUPPORTED, "2^24 rows"),
+    (dict(q_indptr=t(I32, 3)), INVALID, "q_indptr"),
+    (dict(lse=t(F32, 3, 3)), INVALID, "lse"),
+    (dict(window=4, causal=0), UNSUPPORTED, "window needs causal"),
+    (dict(sm_scale=float("inf")), INVALID, "sm_scale"),
+    (dict(sm_scale=-1.0), INVALID, "sm_scale"),
+    (dict(workspace=t(U8, 1000)), INVALID, "workspace has"),
+    (dict(workspace=t(U8, 1 << 30, ptr=0x10080)), INVALID, "256-byte aligned"),
+    (dict(workspace=t(F32, 1 << 30)), INVALID, "u8"),
+])
+def test_attention_refusals(lib, ctx, kw, status, fragment):
+    refused(lib, ctx, "qs3_paged_attention", attention_desc(**kw), status, fragment)
+
+
+def test_workspace_size(lib, ctx):
+    n = C.c_size_t(0)
+    assert lib.qs3_paged_attention_workspace_size(ctx, 8, 8, 16, 2, 256, C.byref(n)) == capi.STATUS_OK and n.value > 0
+    for args in ((0, 8, 16, 2, 256), (8, 8, 15, 2, 256), (8, 0, 16, 2, 256)):
+        assert lib.qs3_paged_attention_workspace_size(ctx, *args, C.byref(n)) == INVALID
+    assert lib.qs3_paged_attention_workspace_size(ctx, 8, 8, 16, 2, 80, C.byref(n)) == UNSUPPORTED
+    assert lib.qs3_paged_attention_workspace_size(ctx, 8, 8, 16, 2, 64, None) == INVALID
