@@ -627,7 +627,8 @@ qsfi_status qs3_paged_attention_workspace_size(qsfi_context* ctx, uint32_t rows,
     if (!head_dim_ok(head_dim))
         return set_unsupported(ctx, "paged_attention head_dim must be 64, 128 or 256");
     const size_t a = stream_bytes(8, head_dim), b = stream_bytes(16, head_dim);
-    *bytes = a > b ? a : b;
+    const size_t c = attn_sizes(kSmCount, attn_prefill_rows(head_dim), head_dim).bytes;
+    *bytes = a > b ? (a > c ? a : c) : b > c ? b : c;
     return QSFI_STATUS_OK;
 }
 
@@ -723,9 +724,16 @@ qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_des
     p.tiling.kv_heads = p.view.kv_heads;
     p.tiling.window = d->window;
     p.tiling.causal = d->causal;
-    p.tiling.tile_rows = attn_stream_rows(fresh * group > 16 ? 16 : static_cast<uint32_t>(fresh * group), dim);
-    p.tiling.key_tile = kStreamKeys;
-    p.blocks = attn_stream_blocks(p.tiling.tile_rows, dim, fp8);
+    const bool chunks = !fp8 && fresh * group > 16;
+    if (chunks) {
+        p.tiling.tile_rows = attn_prefill_rows(dim);
+        p.tiling.key_tile = 128;
+        p.blocks = kSmCount;
+    } else {
+        p.tiling.tile_rows = attn_stream_rows(fresh * group > 16 ? 16 : static_cast<uint32_t>(fresh * group), dim);
+        p.tiling.key_tile = kStreamKeys;
+        p.blocks = attn_stream_blocks(p.tiling.tile_rows, dim, fp8);
+    }
     p.least = 2;
     (void)longest;
     const AttnSizes at = attn_sizes(p.blocks, p.tiling.tile_rows, dim);
@@ -733,7 +741,7 @@ qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_des
     p.notes = reinterpret_cast<SplitNote*>(ws + at.notes);
     p.part_ml = reinterpret_cast<float2*>(ws + at.ml);
     p.part_o = reinterpret_cast<float*>(ws + at.o);
-    cudaError_t err = launch_attn_stream(p, fp8, ctx->stream);
+    cudaError_t err = chunks ? launch_attn_prefill(p, ctx->stream) : launch_attn_stream(p, fp8, ctx->stream);
     if (err == cudaSuccess)
         err = launch_attn_join(p, ctx->stream);
     return set_cuda_error(ctx, err, "paged_attention");
