@@ -724,7 +724,11 @@ qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_des
     p.tiling.kv_heads = p.view.kv_heads;
     p.tiling.window = d->window;
     p.tiling.causal = d->causal;
-    const bool chunks = !fp8 && fresh * group > 16;
+    // the kernel for chunks counts rows of the cache in units of 16 bytes, 32 bits of them
+    const auto reach = [&](const PagedPool& pool) {
+        return static_cast<int64_t>(p.view.pages - 1) * pool.page_stride + static_cast<int64_t>(p.view.page_size - 1) * pool.slot_stride;
+    };
+    const bool chunks = !fp8 && fresh * group > 16 && reach(p.view.k) < (int64_t { 1 } << 36) && reach(p.view.v) < (int64_t { 1 } << 36);
     if (chunks) {
         p.tiling.tile_rows = attn_prefill_rows(dim);
         p.tiling.key_tile = 128;

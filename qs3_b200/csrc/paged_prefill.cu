@@ -16,6 +16,7 @@
 #include "tcgen05.cuh"
 
 #include <cmath>
+#include <type_traits>
 
 namespace qs3 {
 
@@ -27,8 +28,8 @@ constexpr uint32_t kRowTile = 128;
 constexpr uint32_t kKeyTile = 128;
 constexpr uint32_t kPiece = 16384;
 constexpr uint32_t kPieces = 9;   // of the ring
-constexpr uint32_t kInFlight = 4; // pieces whose arrival is awaited later
 constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kNone = 0xffffffffu;
 constexpr float kGrowth = 8.0f; // of a row's maximum, in powers of two, before O is rescaled
 
 enum : uint32_t {
@@ -98,6 +99,19 @@ __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t* r)
                  : "memory");
 }
 
+// Waits for loads from tensor memory, of which `r` is the last: what is computed from the registers stays behind the wait only
+// because they pass through it.
+__device__ __forceinline__ void tc_ld_wait32(uint32_t* r)
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+
 __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r)
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16],"
@@ -154,46 +168,47 @@ __device__ __forceinline__ uint32_t v_piece(uint32_t i, uint32_t n, uint32_t pan
     return panels * (i + 1 < n ? 2 * i + 2 : 2 * i + 1);
 }
 
-// Loads of pieces under way and their barriers: the arrival of the oldest is signalled when kInFlight newer ones are out, or
-// before a wait that might depend on it.
-struct Pending {
-    uint64_t* bar[kInFlight];
-    __device__ __forceinline__ Pending()
+// The copies of a warp that are under way. What they wrote has to be handed to the tensor core by the threads that copied, so a
+// piece is reported when the warp's next one is out, or before a wait.
+struct Copies {
+    uint64_t* bar = nullptr;
+    __device__ __forceinline__ void report()
     {
-#pragma unroll
-        for (uint32_t i = 0; i < kInFlight; ++i)
-            bar[i] = nullptr;
-    }
-    static __device__ __forceinline__ void signal(uint64_t* b)
-    {
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the tensor core reads what was written here
-        mbar_arrive(b);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0)
+            mbar_arrive(bar);
+        bar = nullptr;
     }
     __device__ __forceinline__ void push(uint64_t* b)
     {
         asm volatile("cp.async.commit_group;" ::: "memory");
-        if (bar[0] != nullptr) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kInFlight) : "memory");
-            signal(bar[0]);
+        if (bar != nullptr) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            report();
         }
-#pragma unroll
-        for (uint32_t i = 0; i + 1 < kInFlight; ++i)
-            bar[i] = bar[i + 1];
-        bar[kInFlight - 1] = b;
+        bar = b;
     }
     __device__ __forceinline__ void drain()
     {
         asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll
-        for (uint32_t i = 0; i < kInFlight; ++i)
-            if (bar[i] != nullptr) {
-                signal(bar[i]);
-                bar[i] = nullptr;
-            }
+        if (bar != nullptr)
+            report();
     }
 };
 
-template <uint32_t D> __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) attn_prefill_kernel(const AttnParams p)
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int slot, int head, int page)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+                 " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(slot), "r"(head), "r"(page)
+                 : "memory");
+}
+
+template <uint32_t D>
+__global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1)
+attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap k_map,
+                    const __grid_constant__ CUtensorMap v_map, const uint32_t k_box, const uint32_t v_box)
 {
     using Shape = PrefillShape<D>;
     constexpr uint32_t TILES = Shape::kTiles, PANELS = Shape::kPanels, PIECE_KEYS = Shape::kPieceKeys;
@@ -206,10 +221,10 @@ template <uint32_t D> __global__ void __launch_bounds__(PrefillShape<D>::kThread
 
     if (tid == 0) {
         for (uint32_t i = 0; i < kPieces; ++i) {
-            mbar_init(&bar.full[i], 128);
+            mbar_init(&bar.full[i], 1);
             mbar_init(&bar.empty[i], 1);
         }
-        mbar_init(&bar.q_full, 128);
+        mbar_init(&bar.q_full, 4);
         mbar_init(&bar.q_free, 1);
         for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(&bar.s_full[i], 1);
@@ -247,17 +262,16 @@ template <uint32_t D> __global__ void __launch_bounds__(PrefillShape<D>::kThread
 
     if (warp >= Shape::kLoadWarp && warp < Shape::kLoadWarp + 4) {
         // ------------------------------------------------------------------------------ fetching --
-        const uint32_t t = tid - Shape::kLoadWarp * 32, row = t / 8, unit = t & 7; // rows row + 16 j, unit of 16 bytes
-        const uint32_t place = row * 128 + ((unit ^ (row & 7)) * 16);
-        const uint32_t q_base = smem_u32(smem) + place, ring_base = smem_u32(ring) + place;
-        Pending pending;
+        // A piece is one warp's, so that a warp looks up the pages of its next piece while the others copy.
+        const uint32_t w = warp - Shape::kLoadWarp;
+        Copies copies;
         uint32_t piece = 0, segments = 0;
         bool ok = true;
         const auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
-            if (mbar_try_wait(b, parity))
+            if (__all_sync(0xffffffffu, mbar_test_wait(b, parity)))
                 return true;
-            pending.drain();
-            return mbar_wait(b, parity, &bar.abort, p.err, code);
+            copies.drain();
+            return __all_sync(0xffffffffu, mbar_wait(b, parity, &bar.abort, p.err, code)) != 0;
         };
         while (ok && next_segment<Shape::kRows>(p, at, left, &seg)) {
             uint32_t seen_lo, seen_hi, unused;
@@ -270,64 +284,86 @@ template <uint32_t D> __global__ void __launch_bounds__(PrefillShape<D>::kThread
                 break;
 #pragma unroll 1
             for (uint32_t j = 0; j < Shape::kRows / 16; ++j) {
-                const uint32_t r = row + 16 * j, in_tile = r & (kRowTile - 1);
+                const uint32_t r = w * 4 + lane / 8 + 16 * j, in_tile = r & (kRowTile - 1);
                 const bool there = r < seg.nrows;
                 const uint32_t flat = seg.row0 + (there ? r : 0), token = p.group_div.div(flat);
                 const uint8_t* src = p.q + (seg.rows.row0 + token) * p.q_token
-                    + (at.head * p.tiling.group + flat - token * p.tiling.group) * p.q_head + unit * 16;
+                    + (at.head * p.tiling.group + flat - token * p.tiling.group) * p.q_head + (lane & 7) * 16;
+                const uint32_t dst = smem_u32(smem) + (r / kRowTile) * (kRowTile * D * 2) + in_tile * 128 + (((lane & 7) ^ (r & 7)) * 16);
 #pragma unroll
                 for (uint32_t panel = 0; panel < PANELS; ++panel)
-                    cp_async16z(q_base + (r / kRowTile) * (kRowTile * D * 2) + panel * kPiece + (in_tile - row) * 128, src + panel * 128, there);
+                    cp_async16z(dst + panel * kPiece, src + panel * 128, there);
             }
-            pending.push(&bar.q_full);
+            copies.push(&bar.q_full);
 
-            // 8 of a tile's keys each: where their rows of this head begin
-            const uint8_t* rows[8];
-            const auto find = [&](uint32_t tile, const PagedPool& pool) {
-                uint32_t there = 0;
-#pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) {
-                    const uint32_t key = (seg.tile0 + tile) * kKeyTile + row + 16 * j;
+            // KEYS keys from `key0` on, UNITS units of 16 bytes of each from `skip` bytes on, to panels of 64 elements
+            const auto load = [&](const PagedPool& pool, const CUtensorMap& map, uint32_t box, uint32_t key0, auto keys, auto units,
+                                  uint32_t skip) {
+                constexpr uint32_t KEYS = decltype(keys)::value, UNITS = decltype(units)::value, AT_ONCE = 32 / UNITS;
+                const uint32_t s = piece % kPieces;
+                if (box != 0 && key0 >= seen_lo && key0 + KEYS <= seg.pages.length) {
+                    // whole boxes of cached tokens: a lane each
+                    const uint32_t per_panel = KEYS / box, boxes = per_panel * (UNITS / 8);
+                    const uint32_t panel = lane / per_panel, first = (lane - panel * per_panel) * box;
                     uint32_t slot = 0;
-                    int32_t page = -1;
-                    if (key >= seen_lo && key < seen_hi)
-                        page = page_of(p.view, seg.pages, key, &slot);
-                    there |= (page >= 0 ? 1u : 0u) << j;
-                    rows[j] = pool.data + static_cast<int64_t>(page < 0 ? 0 : page) * pool.page_stride
-                        + static_cast<int64_t>(slot) * pool.slot_stride + at.head * pool.head_stride + unit * 16;
+                    int32_t page = 0;
+                    if (lane < boxes)
+                        page = page_of(p.view, seg.pages, key0 + first, &slot);
+                    if (__all_sync(0xffffffffu, page >= 0)) {
+                        if (!wait(&bar.empty[s], ((piece / kPieces) & 1) ^ 1, ERR_PF_EMPTY_WAIT))
+                            return false;
+                        if (lane == 0)
+                            mbar_expect_tx(&bar.full[s], kPiece);
+                        __syncwarp();
+                        if (lane < boxes)
+                            tma_load_page(smem_u32(ring) + s * kPiece + panel * (KEYS * 128) + first * 128, &map, &bar.full[s],
+                                          static_cast<int>(skip / 2 + panel * 64), static_cast<int>(slot), static_cast<int>(at.head), page);
+                        return true;
+                    }
                 }
-                return there;
+                // where the rows of keys lane + 32 a begin, in units of 16 bytes; none: zeros
+                uint32_t row[KEYS / 32];
+#pragma unroll
+                for (uint32_t a = 0; a < KEYS / 32; ++a) {
+                    const uint32_t key = key0 + a * 32 + lane;
+                    row[a] = kNone;
+                    if (key >= seen_lo && key < seen_hi) {
+                        uint32_t slot;
+                        const int32_t page = page_of(p.view, seg.pages, key, &slot);
+                        if (page >= 0)
+                            row[a] = static_cast<uint32_t>((page * pool.page_stride + slot * pool.slot_stride) >> 4);
+                    }
+                }
+                if (!wait(&bar.empty[s], ((piece / kPieces) & 1) ^ 1, ERR_PF_EMPTY_WAIT))
+                    return false;
+                const uint8_t* const from = pool.data + at.head * pool.head_stride + skip + (lane % UNITS) * 16;
+                const uint32_t to = smem_u32(ring) + s * kPiece + (lane % UNITS / 8) * (KEYS * 128);
+#pragma unroll
+                for (uint32_t j = 0; j < KEYS / AT_ONCE; ++j) {
+                    const uint32_t key = j * AT_ONCE + lane / UNITS;
+                    const uint32_t r = __shfl_sync(0xffffffffu, row[j * AT_ONCE / 32], key & 31);
+                    cp_async16z(to + key * 128 + (((lane & 7) ^ (key & 7)) * 16),
+                                from + static_cast<uint64_t>(r == kNone ? 0 : r) * 16, r != kNone);
+                }
+                copies.push(&bar.full[s]);
+                return true;
             };
             const auto load_k = [&](uint32_t tile) {
-                const uint32_t there = find(tile, p.view.k);
 #pragma unroll 1
-                for (uint32_t panel = 0; panel < PANELS; ++panel, ++piece) {
-                    const uint32_t s = piece % kPieces;
-                    if (!wait(&bar.empty[s], ((piece / kPieces) & 1) ^ 1, ERR_PF_EMPTY_WAIT))
+                for (uint32_t panel = 0; panel < PANELS; ++panel, ++piece)
+                    if ((piece & 3) == w
+                        && !load(p.view.k, k_map, k_box, (seg.tile0 + tile) * kKeyTile, std::integral_constant<uint32_t, kKeyTile> {},
+                                 std::integral_constant<uint32_t, 8> {}, panel * 128))
                         return false;
-#pragma unroll
-                    for (uint32_t j = 0; j < 8; ++j)
-                        cp_async16z(ring_base + s * kPiece + j * 2048, rows[j] + panel * 128, there >> j & 1);
-                    pending.push(&bar.full[s]);
-                }
                 return true;
             };
             const auto load_v = [&](uint32_t tile) {
-                const uint32_t there = find(tile, p.view.v);
-                constexpr uint32_t KEYS = PIECE_KEYS / 16; // of a thread in a piece
-#pragma unroll
-                for (uint32_t v = 0; v < PANELS; ++v, ++piece) {
-                    const uint32_t s = piece % kPieces;
-                    if (!wait(&bar.empty[s], ((piece / kPieces) & 1) ^ 1, ERR_PF_EMPTY_WAIT))
+#pragma unroll 1
+                for (uint32_t v = 0; v < PANELS; ++v, ++piece)
+                    if ((piece & 3) == w
+                        && !load(p.view.v, v_map, v_box, (seg.tile0 + tile) * kKeyTile + v * PIECE_KEYS,
+                                 std::integral_constant<uint32_t, PIECE_KEYS> {}, std::integral_constant<uint32_t, D / 8> {}, 0))
                         return false;
-#pragma unroll
-                    for (uint32_t j = 0; j < KEYS; ++j)
-#pragma unroll
-                        for (uint32_t panel = 0; panel < PANELS; ++panel)
-                            cp_async16z(ring_base + s * kPiece + panel * (PIECE_KEYS * 128) + j * 2048,
-                                        rows[v * KEYS + j] + panel * 128, there >> (v * KEYS + j) & 1);
-                    pending.push(&bar.full[s]);
-                }
                 return true;
             };
             ok = load_k(0);
@@ -340,7 +376,7 @@ template <uint32_t D> __global__ void __launch_bounds__(PrefillShape<D>::kThread
             left -= seg.count;
             next_item(p, &at, row_tiles(p.tiling, seg.rows.fresh));
         }
-        pending.drain();
+        copies.drain();
     } else if (warp == Shape::kMmaWarp) {
         // ------------------------------------------------------------------------------- products --
         if (elect_one()) {
@@ -472,24 +508,31 @@ template <uint32_t D> __global__ void __launch_bounds__(PrefillShape<D>::kThread
                     const uint32_t key0 = (seg.tile0 + i) * kKeyTile;
                     const bool part = __any_sync(0xffffffffu, lo > key0 || hi < key0 + kKeyTile);
 
-                    float top = -INFINITY;
                     uint32_t x[32];
+                    // both passes once with and once without the mask: a test inside them costs a branch per element
+                    const auto largest = [&](auto masked) {
+                        float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-                    for (uint32_t c = 0; c < kKeyTile / 32; ++c) {
-                        tc_ld32(s_addr + c * 32, x);
-                        tc_ld_wait();
-                        if (part) {
+                        for (uint32_t c = 0; c < kKeyTile / 32; ++c) {
+                            tc_ld32(s_addr + c * 32, x);
+                            tc_ld_wait32(x);
 #pragma unroll
-                            for (uint32_t j = 0; j < 32; ++j) {
-                                const uint32_t key = key0 + c * 32 + j;
-                                top = fmaxf(top, key >= lo && key < hi ? __uint_as_float(x[j]) : -INFINITY);
+                            for (uint32_t j = 0; j < 32; j += 2) {
+                                float a = __uint_as_float(x[j]), b = __uint_as_float(x[j + 1]);
+                                if constexpr (decltype(masked)::value) {
+                                    const uint32_t key = key0 + c * 32 + j;
+                                    a = key >= lo && key < hi ? a : -INFINITY;
+                                    b = key + 1 >= lo && key + 1 < hi ? b : -INFINITY;
+                                }
+                                if ((j & 2) == 0)
+                                    top0 = fmaxf(top0, fmaxf(a, b));
+                                else
+                                    top1 = fmaxf(top1, fmaxf(a, b));
                             }
-                        } else {
-#pragma unroll
-                            for (uint32_t j = 0; j < 32; j += 2)
-                                top = fmaxf(top, fmaxf(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
                         }
-                    }
+                        return fmaxf(top0, top1);
+                    };
+                    float top = part ? largest(std::true_type {}) : largest(std::false_type {});
                     top *= p.scale_log2;
                     const bool grow = top > m + kGrowth; // (m = -inf: whenever something is seen)
                     if (__any_sync(0xffffffffu, grow)) {
@@ -505,7 +548,7 @@ template <uint32_t D> __global__ void __launch_bounds__(PrefillShape<D>::kThread
 #pragma unroll 1
                             for (uint32_t c = 0; c < D / 32; ++c) {
                                 tc_ld32(o_col(q) + lanes + c * 32, x);
-                                tc_ld_wait();
+                                tc_ld_wait32(x);
 #pragma unroll
                                 for (uint32_t j = 0; j < 32; ++j)
                                     x[j] = __float_as_uint(__uint_as_float(x[j]) * keep);
@@ -515,30 +558,33 @@ template <uint32_t D> __global__ void __launch_bounds__(PrefillShape<D>::kThread
                         }
                     }
                     const float base = m == -INFINITY ? 0.0f : m;
-                    float sum0 = 0.0f, sum1 = 0.0f;
+                    const auto weights = [&](auto masked) {
+                        float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-                    for (uint32_t c = 0; c < kKeyTile / 32; ++c) {
-                        tc_ld32(s_addr + c * 32, x);
-                        tc_ld_wait();
-                        uint32_t w[16];
+                        for (uint32_t c = 0; c < kKeyTile / 32; ++c) {
+                            tc_ld32(s_addr + c * 32, x);
+                            tc_ld_wait32(x);
+                            uint32_t w[16];
 #pragma unroll
-                        for (uint32_t j = 0; j < 16; ++j) {
-                            float a = fmaf(__uint_as_float(x[2 * j]), p.scale_log2, -base);
-                            float b = fmaf(__uint_as_float(x[2 * j + 1]), p.scale_log2, -base);
-                            if (part) {
-                                const uint32_t key = key0 + c * 32 + 2 * j;
-                                a = key >= lo && key < hi ? a : -INFINITY;
-                                b = key + 1 >= lo && key + 1 < hi ? b : -INFINITY;
+                            for (uint32_t j = 0; j < 16; ++j) {
+                                float a = fmaf(__uint_as_float(x[2 * j]), p.scale_log2, -base);
+                                float b = fmaf(__uint_as_float(x[2 * j + 1]), p.scale_log2, -base);
+                                if constexpr (decltype(masked)::value) {
+                                    const uint32_t key = key0 + c * 32 + 2 * j;
+                                    a = key >= lo && key < hi ? a : -INFINITY;
+                                    b = key + 1 >= lo && key + 1 < hi ? b : -INFINITY;
+                                }
+                                a = exp2_approx(a);
+                                b = exp2_approx(b);
+                                sum0 += a;
+                                sum1 += b;
+                                w[j] = pack_bf16x2(a, b);
                             }
-                            a = exp2_approx(a);
-                            b = exp2_approx(b);
-                            sum0 += a;
-                            sum1 += b;
-                            w[j] = pack_bf16x2(a, b);
+                            tc_st16(s_addr + c * 16, w);
                         }
-                        tc_st16(s_addr + c * 16, w);
-                    }
-                    l += sum0 + sum1;
+                        return sum0 + sum1;
+                    };
+                    l += part ? weights(std::true_type {}) : weights(std::false_type {});
                     tc_st_wait();
                     tc_fence_before();
                     __syncwarp();
@@ -547,7 +593,11 @@ template <uint32_t D> __global__ void __launch_bounds__(PrefillShape<D>::kThread
                 }
                 if (!ok)
                     break;
-                ok = __all_sync(0xffffffffu, mbar_wait(&bar.pv_done[q], (tiles - 1) & 1, &bar.abort, p.err, ERR_PF_SUM_WAIT));
+                // The last two products: a barrier's parity tells one phase from the next only, and with one query tile the
+                // scores that were waited for last are issued before the product of the tile before.
+                if (TILES == 1 && n > 1)
+                    ok = __all_sync(0xffffffffu, mbar_wait(&bar.pv_done[q], (tiles - 2) & 1, &bar.abort, p.err, ERR_PF_SUM_WAIT));
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar.pv_done[q], (tiles - 1) & 1, &bar.abort, p.err, ERR_PF_SUM_WAIT));
                 if (!ok)
                     break;
                 tc_fence_after();
@@ -561,7 +611,7 @@ template <uint32_t D> __global__ void __launch_bounds__(PrefillShape<D>::kThread
 #pragma unroll 1
                 for (uint32_t c = 0; c < D / 32; ++c) {
                     tc_ld32(o_col(q) + lanes + c * 32, x);
-                    tc_ld_wait();
+                    tc_ld_wait32(x);
                     if (!live)
                         continue;
                     if (whole) {
@@ -605,7 +655,20 @@ template <uint32_t D> cudaError_t launch_prefill_as(const AttnParams& p, cudaStr
     const cudaError_t err = cudaFuncSetAttribute(attn_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
     if (err != cudaSuccess)
         return err;
-    return launch_chained(attn_prefill_kernel<D>, dim3(p.blocks), Shape::kThreads, Shape::kSmem, stream, p);
+    // Pages that a box fits into a whole number of times are fetched by TMA, others and the ends of sequences row by row.
+    const auto box = [&](CUtensorMap* map, const PagedPool& pool, uint32_t most) {
+        const uint32_t size = p.view.page_size;
+        const uint32_t rows = size < most ? size : most;
+        const uint64_t dims[4] = { D, size, p.view.kv_heads, p.view.pages };
+        const uint64_t strides[3] = { static_cast<uint64_t>(pool.slot_stride), static_cast<uint64_t>(pool.head_stride),
+                                      static_cast<uint64_t>(pool.page_stride) };
+        if (rows < 8 || size % rows != 0 || most % rows != 0 || !make_page_map(map, pool.data, dims, strides, rows))
+            return 0u;
+        return rows;
+    };
+    CUtensorMap k_map {}, v_map {};
+    const uint32_t k_box = box(&k_map, p.view.k, kKeyTile), v_box = box(&v_map, p.view.v, Shape::kPieceKeys);
+    return launch_chained(attn_prefill_kernel<D>, dim3(p.blocks), Shape::kThreads, Shape::kSmem, stream, p, k_map, v_map, k_box, v_box);
 }
 
 } // namespace
