@@ -128,25 +128,17 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
     AttnPlace at = range.place;
     uint8_t* const ring = smem + warp * kStreamStages * Shape::kStage;
     const uint32_t ring_u32 = tc::smem_u32(ring);
-    bool first = true;
+    if (tid == 0)
+        note_split(p, range);
 
-    while (left > 0 && at.seq < p.view.batch) {
-        const SeqRows rows = seq_rows(p, at.seq);
-        const SeqPages pages = seq_pages(p.view, at.seq);
-        const KeyTiles keys = key_tiles(p.tiling, rows.fresh, pages.length, at.tile);
-        const uint32_t item_tiles = keys.end - keys.first;
-        const uint32_t count = static_cast<uint32_t>(min(static_cast<uint64_t>(item_tiles - at.offset), left));
-        const uint32_t tile0 = keys.first + at.offset;
-        if (rows.fresh == 0 || at.offset >= item_tiles)
-            break; // (the tables changed under the kernel)
-        if (first && tid == 0 && p.notes != nullptr)
-            note_split(p, range, item_tiles);
+    Segment seg;
+    while (this_segment(p, at, left, &seg)) {
+        const SeqRows& rows = seg.rows;
+        const SeqPages& pages = seg.pages;
+        const uint32_t count = seg.count, tile0 = seg.tile0, row0 = seg.row0, nrows = seg.nrows;
 
         // query rows; a row past the last one is zeros
         __syncthreads();
-        const uint64_t seq_row_count = static_cast<uint64_t>(rows.fresh) * p.tiling.group;
-        const uint32_t row0 = at.tile * ROWS;
-        const uint32_t nrows = static_cast<uint32_t>(min(static_cast<uint64_t>(ROWS), seq_row_count - row0));
         for (uint32_t i = tid; i < ROWS * D / 8; i += kStreamThreads) {
             const uint32_t r = i / (D / 8), c = i % (D / 8);
             uint4 w = make_uint4(0, 0, 0, 0);
@@ -407,8 +399,8 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
                 }
             }
         __syncthreads();
-        const bool whole = count == item_tiles;
-        const uint32_t slot = blockIdx.x * 2 + (at.offset == 0 ? 1 : 0);
+        const bool whole = seg.whole;
+        const uint32_t slot = blockIdx.x * 2 + (seg.starts ? 1 : 0);
         for (uint32_t i = tid; i < nrows * (D / 4); i += kStreamThreads) {
             const uint32_t r = i / (D / 4), e = i % (D / 4) * 4;
             float top = -INFINITY, sum = 0.0f;
@@ -438,91 +430,99 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
                     p.part_ml[static_cast<size_t>(slot) * ROWS + r] = make_float2(top, sum);
             }
         }
-        left -= count;
-        first = false;
-        next_item(p, &at, row_tiles(p.tiling, rows.fresh));
-    }
-    if (first && tid == 0 && p.notes != nullptr) { // no work: the joining launch finds nothing here either
-        SplitNote n {};
-        n.active = range.active;
-        n.total = range.total;
-        p.notes[blockIdx.x] = n;
+        next_segment(p, seg, &at, &left);
     }
 }
 
-// Joins the parts of items that were split. Block (c, y) of the launch looks at the item in which the range of block c + 1
-// began, and takes it when it is the first to begin there; y numbers groups of its rows, a warp each.
-constexpr uint32_t kJoinWarps = 4;
+// Joins the parts of items that were split: slot 1 of block c - 1, slots 0 of c and the blocks after it. SHARED: a block per
+// row, its warps with a part each in turn (few rows, a long context over many blocks); else a warp per row.
+constexpr uint32_t kJoinWarps = 8;
 
-template <uint32_t D> __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(AttnParams p)
+template <uint32_t D, bool SHARED> __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(AttnParams p)
 {
-    chain_begin();
-    const uint32_t c = blockIdx.x + 1;
-    const SplitNote n = p.notes[c];
-    if (c >= n.active)
-        return;
-    const uint64_t begin = block_begin(n.total, n.active, c), end = n.item_begin + n.item_tiles;
-    if (n.item_begin >= begin || n.item_begin < block_begin(n.total, n.active, c - 1))
-        return; // not split here, or split by an earlier block already
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    const SeqRows rows = seq_rows(p, n.seq);
-    const uint64_t all = static_cast<uint64_t>(rows.fresh) * p.tiling.group;
-    const uint32_t row0 = n.tile * p.tiling.tile_rows;
-    const uint32_t r = blockIdx.y * kJoinWarps + warp;
-    if (r >= p.tiling.tile_rows || row0 + r >= all)
-        return;
-    // parts: slot 1 of block c - 1, slots 0 of c .. last
-    uint32_t last = c;
-    while (last + 1 < n.active && block_begin(n.total, n.active, last + 1) < end)
-        ++last;
-    const auto slot_of = [&](uint32_t b) { return static_cast<size_t>(b < c ? 2 * b + 1 : 2 * b) * p.tiling.tile_rows + r; };
-    float top = -INFINITY;
-    for (uint32_t b = c - 1 + lane; b <= last; b += 32)
-        top = fmaxf(top, p.part_ml[slot_of(b)].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float base = top == -INFINITY ? 0.0f : top;
     constexpr uint32_t E = D / 32; // elements of a lane
-    float acc[E], sum = 0.0f;
+    __shared__ float s_acc[SHARED ? kJoinWarps * D : 1];
+    chain_begin();
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const uint32_t r = SHARED ? blockIdx.y : blockIdx.y * kJoinWarps + warp;
+    for (uint32_t c = blockIdx.x + 1; c < p.blocks; c += gridDim.x) {
+        const SplitNote n = p.notes[c];
+        if (n.parts == 0)
+            continue;
+        const SeqRows rows = seq_rows(p, n.seq);
+        const uint32_t row0 = n.tile * p.tiling.tile_rows;
+        if (r >= p.tiling.tile_rows || row0 + r >= static_cast<uint64_t>(rows.fresh) * p.tiling.group)
+            continue;
+        const auto slot_of = [&](uint32_t i) {
+            return static_cast<size_t>(i == 0 ? 2 * c - 1 : 2 * (c + i - 1)) * p.tiling.tile_rows + r;
+        };
+        float top = -INFINITY, sum = 0.0f;
+        for (uint32_t i = lane; i <= n.parts; i += 32)
+            top = fmaxf(top, p.part_ml[slot_of(i)].x);
 #pragma unroll
-    for (uint32_t j = 0; j < E; ++j)
-        acc[j] = 0.0f;
-#pragma unroll 4
-    for (uint32_t b = c - 1; b <= last; ++b) {
-        const size_t s = slot_of(b);
-        const float2 ml = p.part_ml[s];
-        const float w = exp2_fast(ml.x - base);
-        sum += ml.y * w;
-        const float* x = p.part_o + s * D + lane * E;
-        float v[E];
-        if constexpr (E == 2) {
-            *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(x);
-        } else {
-#pragma unroll
-            for (uint32_t j = 0; j < E; j += 4)
-                *reinterpret_cast<float4*>(v + j) = *reinterpret_cast<const float4*>(x + j);
+        for (int o = 16; o > 0; o >>= 1)
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float base = top == -INFINITY ? 0.0f : top;
+        for (uint32_t i = lane; i <= n.parts; i += 32) {
+            const float2 ml = p.part_ml[slot_of(i)];
+            sum += ml.y * exp2_fast(ml.x - base);
         }
 #pragma unroll
-        for (uint32_t j = 0; j < E; ++j)
-            acc[j] += v[j] * w;
-    }
-    const float inv = top == -INFINITY ? 0.0f : 1.0f / sum;
-    const uint32_t token = p.group_div.div(row0 + r), h = n.head * p.tiling.group + row0 + r - token * p.tiling.group;
-    uint8_t* out = p.out + (rows.row0 + token) * p.out_token + h * p.out_head + lane * E * 2;
-    uint32_t w[E / 2];
+        for (int o = 16; o > 0; o >>= 1)
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        float acc[E];
 #pragma unroll
-    for (uint32_t j = 0; j < E / 2; ++j)
-        w[j] = tc::pack_bf16x2(acc[2 * j] * inv, acc[2 * j + 1] * inv);
-    if constexpr (E == 2)
-        *reinterpret_cast<uint32_t*>(out) = w[0];
-    else if constexpr (E == 4)
-        *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
-    else
-        *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
-    if (lane == 0 && p.lse != nullptr)
-        p.lse[(rows.row0 + token) * p.lse_token + h * p.lse_head]
-            = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
+        for (uint32_t j = 0; j < E; ++j)
+            acc[j] = 0.0f;
+        constexpr uint32_t STEP = SHARED ? kJoinWarps : 1;
+#pragma unroll 4
+        for (uint32_t i = SHARED ? warp : 0; i <= n.parts; i += STEP) {
+            const size_t s = slot_of(i);
+            const float w = exp2_fast(p.part_ml[s].x - base);
+            const float* x = p.part_o + s * D + lane * E;
+            float v[E];
+            if constexpr (E == 2) {
+                *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(x);
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < E; j += 4)
+                    *reinterpret_cast<float4*>(v + j) = *reinterpret_cast<const float4*>(x + j);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < E; ++j)
+                acc[j] += v[j] * w;
+        }
+        if constexpr (SHARED) {
+            __syncthreads(); // (the row before)
+#pragma unroll
+            for (uint32_t j = 0; j < E; ++j)
+                s_acc[warp * D + lane * E + j] = acc[j];
+            __syncthreads();
+            if (warp != 0)
+                continue;
+#pragma unroll
+            for (uint32_t j = 0; j < E; ++j)
+#pragma unroll
+                for (uint32_t w = 1; w < kJoinWarps; ++w)
+                    acc[j] += s_acc[w * D + lane * E + j];
+        }
+        const float inv = top == -INFINITY ? 0.0f : 1.0f / sum;
+        const uint32_t token = p.group_div.div(row0 + r), h = n.head * p.tiling.group + row0 + r - token * p.tiling.group;
+        uint8_t* out = p.out + (rows.row0 + token) * p.out_token + h * p.out_head + lane * E * 2;
+        uint32_t w[E / 2];
+#pragma unroll
+        for (uint32_t j = 0; j < E / 2; ++j)
+            w[j] = tc::pack_bf16x2(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+        if constexpr (E == 2)
+            *reinterpret_cast<uint32_t*>(out) = w[0];
+        else if constexpr (E == 4)
+            *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+        else
+            *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (lane == 0 && p.lse != nullptr)
+            p.lse[(rows.row0 + token) * p.lse_token + h * p.lse_head]
+                = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
+    }
 }
 
 template <uint32_t D, uint32_t NT, bool FP8> cudaError_t launch_stream_as(const AttnParams& p, cudaStream_t stream)
@@ -570,10 +570,13 @@ cudaError_t launch_attn_stream(const AttnParams& p, bool fp8, cudaStream_t strea
 
 cudaError_t launch_attn_join(const AttnParams& p, cudaStream_t stream)
 {
-    const dim3 grid(p.blocks - 1, (p.tiling.tile_rows + kJoinWarps - 1) / kJoinWarps);
     const uint32_t d = p.view.head_dim;
-    return launch_chained(d == 64 ? attn_join_kernel<64> : d == 128 ? attn_join_kernel<128> : attn_join_kernel<256>, grid,
-                          kJoinWarps * 32, 0, stream, p);
+    const uint32_t wide = p.blocks - 1 < kSmCount ? p.blocks - 1 : kSmCount;
+    if (p.tiling.tile_rows <= 16)
+        return launch_chained(d == 64 ? attn_join_kernel<64, true> : d == 128 ? attn_join_kernel<128, true> : attn_join_kernel<256, true>,
+                              dim3(wide, p.tiling.tile_rows), kJoinWarps * 32, 0, stream, p);
+    return launch_chained(d == 64 ? attn_join_kernel<64, false> : d == 128 ? attn_join_kernel<128, false> : attn_join_kernel<256, false>,
+                          dim3(wide, p.tiling.tile_rows / kJoinWarps), kJoinWarps * 32, 0, stream, p);
 }
 
 } // namespace qs3
@@ -732,13 +735,15 @@ qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_des
     if (chunks) {
         p.tiling.tile_rows = attn_prefill_rows(dim);
         p.tiling.key_tile = 128;
+        p.tiling.item_cost = 4;
         p.blocks = kSmCount;
     } else {
         p.tiling.tile_rows = attn_stream_rows(fresh * group > 16 ? 16 : static_cast<uint32_t>(fresh * group), dim);
         p.tiling.key_tile = kStreamKeys;
+        p.tiling.item_cost = 1;
         p.blocks = attn_stream_blocks(p.tiling.tile_rows, dim, fp8);
     }
-    p.least = 2;
+    p.least = p.tiling.item_cost + 1;
     (void)longest;
     const AttnSizes at = attn_sizes(p.blocks, p.tiling.tile_rows, dim);
     char* ws = static_cast<char*>(d->workspace.data);

@@ -29,14 +29,10 @@ struct AttnParams {
     uint32_t* err;
 };
 
-// What block c leaves for the joining launch about the item that its range begins in.
+// What block c leaves for the joining launch when its range begins inside the key tiles of an item and no earlier block's does:
+// the item, and how many blocks after c - 1 hold parts of it. 0: nothing to join here.
 struct SplitNote {
-    uint64_t item_begin; // key tile with which the item begins
-    uint32_t item_tiles;
-    uint32_t seq, head, tile;
-    uint32_t active; // blocks with work
-    uint32_t pad;
-    uint64_t total;
+    uint32_t seq, head, tile, parts;
 };
 
 #ifdef __CUDACC__
@@ -59,19 +55,19 @@ __device__ __forceinline__ SeqRows seq_rows(const AttnParams& p, uint32_t seq)
 // The search for where a block's range begins. `cost` [batch] is shared memory that nothing else uses meanwhile; every thread of
 // the block takes part and gets the same answer, warps at their own time (a barrier comes before `cost` is used again).
 struct BlockRange {
-    uint64_t begin, end; // key tiles
+    uint64_t begin, end;
     uint64_t total;
     uint32_t active;
     AttnPlace place;     // of `begin`
 };
 
-// Key tiles of the items of a (sequence, KV head), by one warp.
+// Cost of the items of a (sequence, KV head), by one warp.
 __device__ __forceinline__ uint64_t warp_tiles_cost(const AttnTiling& a, uint32_t fresh, uint32_t length, uint32_t tiles)
 {
     uint64_t sum = 0;
     for (uint32_t t = threadIdx.x & 31; t < tiles; t += 32) {
         const KeyTiles k = key_tiles(a, fresh, length, t);
-        sum += k.end - k.first;
+        sum += k.end - k.first + a.item_cost;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
@@ -94,7 +90,7 @@ __device__ BlockRange find_range(const AttnParams& p, uint64_t* cost, uint32_t b
             const uint32_t length = seq_pages(p.view, b).length;
             for (uint32_t t = 0; t < tiles; ++t) {
                 const KeyTiles k = key_tiles(p.tiling, fresh, length, t);
-                sum += k.end - k.first;
+                sum += k.end - k.first + p.tiling.item_cost;
             }
         } else {
             sum = kUnknown;
@@ -160,7 +156,7 @@ __device__ BlockRange find_range(const AttnParams& p, uint64_t* cost, uint32_t b
         uint32_t mine = 0;
         if (t0 + lane < tiles) {
             const KeyTiles k = key_tiles(p.tiling, fresh, length, t0 + lane);
-            mine = k.end - k.first;
+            mine = k.end - k.first + p.tiling.item_cost;
         }
         uint64_t run = mine;
 #pragma unroll
@@ -196,18 +192,57 @@ __device__ __forceinline__ void next_item(const AttnParams& p, AttnPlace* at, ui
     while (at->seq < p.view.batch && seq_rows(p, at->seq).fresh == 0);
 }
 
-__device__ __forceinline__ void note_split(const AttnParams& p, const BlockRange& r, uint32_t item_tiles)
+// By one thread of every block.
+__device__ __forceinline__ void note_split(const AttnParams& p, const BlockRange& r)
 {
-    SplitNote n;
-    n.item_begin = r.begin - r.place.offset;
-    n.item_tiles = item_tiles;
-    n.seq = r.place.seq;
-    n.head = r.place.head;
-    n.tile = r.place.tile;
-    n.active = r.active;
-    n.pad = 0;
-    n.total = r.total;
+    SplitNote n { r.place.seq, r.place.head, r.place.tile, 0 };
+    if (r.begin < r.end && r.place.offset > p.tiling.item_cost) {
+        const uint64_t item = r.begin - r.place.offset;
+        const KeyTiles k = key_tiles(p.tiling, seq_rows(p, n.seq).fresh, seq_pages(p.view, n.seq).length, n.tile);
+        if (block_begin(r.total, r.active, blockIdx.x - 1) <= item + p.tiling.item_cost) // (block 0 begins with an item)
+            n.parts = block_of_end(r.total, r.active, item + p.tiling.item_cost + (k.end - k.first)) - blockIdx.x + 1;
+    }
     p.notes[blockIdx.x] = n;
+}
+
+// A block's part of an item. `at` moves along the block's range with `left`; false: the range is through.
+struct Segment {
+    SeqRows rows;
+    SeqPages pages;
+    uint32_t row0, nrows;  // of the item, among the sequence's
+    uint32_t tile0, count; // key tiles
+    bool starts, whole;    // with the item's first key tile; with all of them
+};
+
+__device__ __forceinline__ bool this_segment(const AttnParams& p, const AttnPlace& at, uint64_t left, Segment* s)
+{
+    if (left == 0 || at.seq >= p.view.batch)
+        return false;
+    s->rows = seq_rows(p, at.seq);
+    s->pages = seq_pages(p.view, at.seq);
+    if (s->rows.fresh == 0)
+        return false;
+    const KeyTiles keys = key_tiles(p.tiling, s->rows.fresh, s->pages.length, at.tile);
+    const uint32_t tiles = keys.end - keys.first;
+    const uint32_t from = tiles_before(p.tiling, at.offset, tiles), to = tiles_before(p.tiling, at.offset + left, tiles);
+    if (from >= to)
+        return false; // the range ends before the item's first key tile
+    s->count = to - from;
+    s->tile0 = keys.first + from;
+    s->starts = from == 0;
+    s->whole = s->count == tiles;
+    s->row0 = at.tile * p.tiling.tile_rows;
+    s->nrows = static_cast<uint32_t>(min(static_cast<uint64_t>(p.tiling.tile_rows),
+                                         static_cast<uint64_t>(s->rows.fresh) * p.tiling.group - s->row0));
+    return true;
+}
+
+__device__ __forceinline__ void next_segment(const AttnParams& p, const Segment& s, AttnPlace* at, uint64_t* left)
+{
+    const KeyTiles keys = key_tiles(p.tiling, s.rows.fresh, s.pages.length, at->tile);
+    const uint64_t rest = static_cast<uint64_t>(p.tiling.item_cost) + (keys.end - keys.first) - at->offset;
+    *left = *left > rest ? *left - rest : 0;
+    next_item(p, at, row_tiles(p.tiling, s.rows.fresh));
 }
 
 #endif

@@ -1,17 +1,23 @@
 // Attention of chunks of new tokens over a paged KV cache, on the tensor cores with accumulators in tensor memory.
 //
 // A block holds 128 query rows (heads of 256 elements) or two tiles of 128 (smaller heads); a row is a new token and one of the
-// query heads that share a KV head, so that a short chunk still fills a tile. Keys pass by 128 at a time:
-//   S = Q K^T           tcgen05.mma 128 x 128, both operands in shared memory
-//   P = exp2(c S - m)   a thread per row: tensor memory -> registers -> tensor memory, where P (16 bits) takes the place of S
+// query heads that share a KV head, so that a short chunk still fills a tile. Keys arrive by 128 and pass in steps of 128 (one
+// query tile) or 64 (two):
+//   S = Q K^T           tcgen05.mma 128 x 128 or 128 x 64, both operands in shared memory
+//   P = exp2(c S - m)   tensor memory -> registers -> tensor memory, where P (16 bits) takes the place of S; a thread has 64 keys
+//                       of a row: half a step with one query tile, whose row two threads share, else a step of its own row
 //   O += P V            tcgen05.mma 128 x head_dim, P from tensor memory, V as it lies in the cache (its rows along k)
-// Two score tiles are under way at a time, so that the products of one run beside the exponentials of the other: the next key
-// tile's with one query tile, the other query tile's with two. m follows the row's maximum only when that has grown by 2^8
-// (the weights stay below 256, the sums take the difference): tiles that rescale O in tensor memory are then few.
+// Two score tiles of each query tile fit beside O (512 columns), so that scores run ahead of the weights and products beside
+// exponentials, which eight warps share because one alone waits longer for each of its instructions than they take. One warp
+// issues the scores and another the sums: every wait, product and commit costs its thread 50 to 100 cycles, together twice as
+// much as the products take.
+// m follows the row's maximum only when that has grown by 2^8 (the weights stay below 256, the sums take the difference):
+// steps that rescale O in tensor memory are then few.
 //
-// Four warps fetch: K in panels of 64 elements, V in groups of keys, both in pieces of 16 KB through one ring, with cp.async
-// rather than TMA, because a page may hold any number of tokens and end anywhere inside a tile, and 16 bytes are the unit in
-// which every page size, stride and swizzled place works. Keys that no row sees are filled with zeros.
+// Five warps fetch, three K in panels of 64 elements and two V in groups of keys, in pieces of 32 KB, each warp its own slots of
+// K's or V's ring: a slot's barriers then pass their phases in one order for all, which parities need. Pages that a box of TMA
+// divides come that way; other page sizes, the ends of sequences and windows row by row with cp.async, 16 bytes being the unit
+// in which every page size, stride and swizzled place works. Keys that no row sees are zeros then.
 #include "paged_attention.cuh"
 #include "tcgen05.cuh"
 
@@ -26,8 +32,9 @@ using namespace tc;
 
 constexpr uint32_t kRowTile = 128;
 constexpr uint32_t kKeyTile = 128;
-constexpr uint32_t kPiece = 16384;
-constexpr uint32_t kPieces = 9;   // of the ring
+constexpr uint32_t kMine = 64;     // keys of a step that a thread has
+constexpr uint32_t kSoftmaxWarps = 8;
+constexpr uint32_t kWarpsK = 3, kWarpsV = 2, kLoadWarps = kWarpsK + kWarpsV;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kNone = 0xffffffffu;
 constexpr float kGrowth = 8.0f; // of a row's maximum, in powers of two, before O is rescaled
@@ -41,28 +48,37 @@ enum : uint32_t {
     ERR_PF_SUM_WAIT = 0x5a000006u,
 };
 
-template <uint32_t D> struct PrefillShape {
-    static constexpr uint32_t kTiles = D == 256 ? 1 : 2; // query tiles
-    static constexpr uint32_t kRows = kTiles * kRowTile;
-    static constexpr uint32_t kPanels = D / 64;                     // pieces of a K tile, and of a V tile
-    static constexpr uint32_t kPieceKeys = kPiece / (2 * D);        // keys of a piece of V
-    static constexpr uint32_t kQ = kRows * D * 2;
-    static constexpr uint32_t kSoftmaxWarps = 4 * kTiles;
-    static constexpr uint32_t kLoadWarp = kSoftmaxWarps;            // first of four
-    static constexpr uint32_t kMmaWarp = kSoftmaxWarps + 4;
-    static constexpr uint32_t kThreads = (kSoftmaxWarps + 5) * 32;
-    static constexpr uint32_t kSmem = 1024 + kQ + kPieces * kPiece + 512;
-    static_assert(kSmem <= 227 * 1024, "shared memory of a block");
-    static_assert(kPieces * kPiece >= kMaxBatch * 8, "the search for the block's range uses the ring");
-};
-
 struct Barriers {
-    uint64_t full[kPieces], empty[kPieces];
+    uint64_t k_full[6], k_empty[6], v_full[4], v_empty[4];
     uint64_t q_full, q_free;
-    uint64_t s_full[2], p_full[2], pv_done[2], o_free[2];
+    uint64_t s_full[4], p_full[4], pv_done[4], o_free[2]; // of the score tiles, and of the query tiles
     uint64_t drain;
+    float share[2][kRowTile]; // between the two threads of a row
     uint32_t tmem;
     volatile uint32_t abort;
+};
+
+template <uint32_t D> struct PrefillShape {
+    static constexpr uint32_t kTiles = D == 256 ? 1 : 2; // query tiles
+    static constexpr uint32_t kStep = kTiles == 1 ? 128 : 64; // keys of a score tile
+    static constexpr uint32_t kSteps = kKeyTile / kStep;      // of a key tile
+    static constexpr uint32_t kBuffers = 2;                   // score tiles of a query tile
+    static constexpr uint32_t kRows = kTiles * kRowTile;
+    static constexpr uint32_t kPiece = D == 64 ? 16384 : 32768;
+    static constexpr uint32_t kSlotsK = D == 64 ? 6 : 3, kSlotsV = D == 64 ? 4 : 2; // of the rings
+    static constexpr uint32_t kPanels = kPiece / (kKeyTile * 128);  // panels of 64 elements in a piece of K
+    static constexpr uint32_t kPieceKeys = kPiece / (2 * D);        // keys of a piece of V
+    static constexpr uint32_t kPerTile = kKeyTile / kPieceKeys;     // pieces of a tile of K, and of V
+    static constexpr uint32_t kQ = kRows * D * 2;
+    static constexpr uint32_t kLoadWarp = kSoftmaxWarps;            // first of five
+    static constexpr uint32_t kScoreWarp = kSoftmaxWarps + kLoadWarps;
+    static constexpr uint32_t kThreads = (kSoftmaxWarps + kLoadWarps + 2) * 32;
+    static constexpr uint32_t kRing = (kSlotsK + kSlotsV) * kPiece;
+    static constexpr uint32_t kSmem = 1024 + kQ + kRing + sizeof(Barriers);
+    static_assert(kSlotsK % kWarpsK == 0 && kSlotsV % kWarpsV == 0, "a slot is one warp's");
+    static_assert(kSmem <= 227 * 1024, "shared memory of a block");
+    static_assert(kRing >= kMaxBatch * 8, "the search for the block's range uses the ring");
+    static_assert(kPanels * 64 * kPerTile == D, "a tile of K has as many pieces as one of V");
 };
 
 __device__ __forceinline__ void cp_async16z(uint32_t dst, const void* src, bool there)
@@ -76,14 +92,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
                  "r"(a), "l"(b), "r"(idesc), "r"(acc)
                  : "memory");
-}
-
-// V as the B operand with its n side contiguous: panels of 64 elements (`panel` bytes apart), keys 128 bytes apart, groups of
-// eight keys 1024, 128-byte swizzle.
-__device__ __forceinline__ uint64_t value_desc(uint32_t smem_addr, uint32_t panel)
-{
-    return static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4) | (static_cast<uint64_t>(panel >> 4) << 16)
-        | (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t* r)
@@ -130,44 +138,6 @@ __device__ __forceinline__ float exp2_approx(float x)
     return r;
 }
 
-// What every role of the block has to know of its next piece of work: it follows the items for itself.
-struct Segment {
-    SeqRows rows;
-    SeqPages pages;
-    uint32_t row0, nrows; // of the item, among the sequence's
-    uint32_t tile0, count; // key tiles
-    uint32_t item_tiles;
-    bool second; // the second query tile has rows
-};
-
-template <uint32_t ROWS>
-__device__ __forceinline__ bool next_segment(const AttnParams& p, const AttnPlace& at, uint64_t left, Segment* s)
-{
-    if (left == 0 || at.seq >= p.view.batch)
-        return false;
-    s->rows = seq_rows(p, at.seq);
-    s->pages = seq_pages(p.view, at.seq);
-    if (s->rows.fresh == 0)
-        return false;
-    const KeyTiles keys = key_tiles(p.tiling, s->rows.fresh, s->pages.length, at.tile);
-    s->item_tiles = keys.end - keys.first;
-    if (at.offset >= s->item_tiles)
-        return false; // (the tables changed under the kernel)
-    s->count = static_cast<uint32_t>(min(static_cast<uint64_t>(s->item_tiles - at.offset), left));
-    s->tile0 = keys.first + at.offset;
-    s->row0 = at.tile * ROWS;
-    s->nrows = static_cast<uint32_t>(min(static_cast<uint64_t>(ROWS), static_cast<uint64_t>(s->rows.fresh) * p.tiling.group - s->row0));
-    s->second = s->nrows > kRowTile;
-    return true;
-}
-
-// Pieces of a segment in the order in which they are fetched: K 0, K 1, V 0, K 2, V 1, ... V n-1.
-__device__ __forceinline__ uint32_t k_piece(uint32_t i, uint32_t panels) { return i == 0 ? 0 : panels * (2 * i - 1); }
-__device__ __forceinline__ uint32_t v_piece(uint32_t i, uint32_t n, uint32_t panels)
-{
-    return panels * (i + 1 < n ? 2 * i + 2 : 2 * i + 1);
-}
-
 // The copies of a warp that are under way. What they wrote has to be handed to the tensor core by the threads that copied, so a
 // piece is reported when the warp's next one is out, or before a wait.
 struct Copies {
@@ -211,33 +181,38 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     const __grid_constant__ CUtensorMap v_map, const uint32_t k_box, const uint32_t v_box)
 {
     using Shape = PrefillShape<D>;
-    constexpr uint32_t TILES = Shape::kTiles, PANELS = Shape::kPanels, PIECE_KEYS = Shape::kPieceKeys;
+    constexpr uint32_t TILES = Shape::kTiles, STEP = Shape::kStep, STEPS = Shape::kSteps, BUFFERS = Shape::kBuffers, PANELS = Shape::kPanels, PIECE_KEYS = Shape::kPieceKeys;
+    constexpr uint32_t PER_TILE = Shape::kPerTile, kPiece = Shape::kPiece, SLOTS_K = Shape::kSlotsK, SLOTS_V = Shape::kSlotsV;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* const ring = smem + Shape::kQ;
-    Barriers& bar = *reinterpret_cast<Barriers*>(ring + kPieces * kPiece);
-    static_assert(sizeof(Barriers) <= 512, "room for the barriers");
+    Barriers& bar = *reinterpret_cast<Barriers*>(ring + Shape::kRing);
     const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
 
     if (tid == 0) {
-        for (uint32_t i = 0; i < kPieces; ++i) {
-            mbar_init(&bar.full[i], 1);
-            mbar_init(&bar.empty[i], 1);
+        for (uint32_t i = 0; i < 6; ++i) {
+            mbar_init(&bar.k_full[i], 1);
+            mbar_init(&bar.k_empty[i], 1);
         }
-        mbar_init(&bar.q_full, 4);
+        for (uint32_t i = 0; i < 4; ++i) {
+            mbar_init(&bar.v_full[i], 1);
+            mbar_init(&bar.v_empty[i], 1);
+        }
+        mbar_init(&bar.q_full, kWarpsK);
         mbar_init(&bar.q_free, 1);
-        for (uint32_t i = 0; i < 2; ++i) {
+        for (uint32_t i = 0; i < 4; ++i) {
             mbar_init(&bar.s_full[i], 1);
-            mbar_init(&bar.p_full[i], 4);
+            mbar_init(&bar.p_full[i], kSoftmaxWarps / TILES);
             mbar_init(&bar.pv_done[i], 1);
-            mbar_init(&bar.o_free[i], 4);
         }
-        mbar_init(&bar.drain, 1);
+        for (uint32_t i = 0; i < 2; ++i)
+            mbar_init(&bar.o_free[i], kSoftmaxWarps / TILES);
+        mbar_init(&bar.drain, 2);
         bar.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == Shape::kMmaWarp) {
+    if (warp == Shape::kScoreWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar.tmem)), "r"(kTmemCols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -247,25 +222,27 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
     tc_fence_after();
     const uint32_t tmem = bar.tmem;
     const auto o_col = [&](uint32_t q) { return tmem + q * D; };
-    const auto s_col = [&](uint32_t slot) { return tmem + 256 + slot * kKeyTile; };
+    const auto s_col = [&](uint32_t slot) { return tmem + 256 + slot * STEP; };
     chain_begin();
 
     const BlockRange range = find_range<Shape::kThreads>(p, reinterpret_cast<uint64_t*>(ring), blockIdx.x);
     __syncthreads();
     uint64_t left = range.end - range.begin;
     AttnPlace at = range.place;
-    Segment seg;
-    if (tid == 0) {
-        const bool work = next_segment<Shape::kRows>(p, at, left, &seg);
-        note_split(p, range, work ? seg.item_tiles : 0);
-    }
+    Segment seg; // every role follows the range for itself
+    if (tid == 0)
+        note_split(p, range);
 
-    if (warp >= Shape::kLoadWarp && warp < Shape::kLoadWarp + 4) {
+    if (warp >= Shape::kLoadWarp && warp < Shape::kScoreWarp) {
         // ------------------------------------------------------------------------------ fetching --
-        // A piece is one warp's, so that a warp looks up the pages of its next piece while the others copy.
-        const uint32_t w = warp - Shape::kLoadWarp;
+        const bool value = warp - Shape::kLoadWarp >= kWarpsK; // fetches V
+        const uint32_t w = value ? warp - Shape::kLoadWarp - kWarpsK : warp - Shape::kLoadWarp, warps = value ? kWarpsV : kWarpsK;
+        const uint32_t slots = value ? SLOTS_V : SLOTS_K;
+        uint64_t* const full_bar = value ? bar.v_full : bar.k_full;
+        uint64_t* const empty_bar = value ? bar.v_empty : bar.k_empty;
+        const uint32_t ring_at = smem_u32(ring) + (value ? SLOTS_K * kPiece : 0);
         Copies copies;
-        uint32_t piece = 0, segments = 0;
+        uint32_t before = 0, segments = 0; // pieces of earlier segments
         bool ok = true;
         const auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
             if (__all_sync(0xffffffffu, mbar_test_wait(b, parity)))
@@ -273,71 +250,89 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
             copies.drain();
             return __all_sync(0xffffffffu, mbar_wait(b, parity, &bar.abort, p.err, code)) != 0;
         };
-        while (ok && next_segment<Shape::kRows>(p, at, left, &seg)) {
+        while (ok && this_segment(p, at, left, &seg)) {
             uint32_t seen_lo, seen_hi, unused;
             visible_keys(p.tiling, seg.rows.fresh, seg.pages.length, p.group_div.div(seg.row0), &seen_lo, &unused);
             visible_keys(p.tiling, seg.rows.fresh, seg.pages.length, p.group_div.div(seg.row0 + seg.nrows - 1), &unused, &seen_hi);
             seen_hi = min(seen_hi, seg.pages.length);
 
-            ok = wait(&bar.q_free, (segments & 1) ^ 1, ERR_PF_QUERY_WAIT);
-            if (!ok)
-                break;
+            const auto load_query = [&] {
+                if (!wait(&bar.q_free, (segments & 1) ^ 1, ERR_PF_QUERY_WAIT))
+                    return false;
 #pragma unroll 1
-            for (uint32_t j = 0; j < Shape::kRows / 16; ++j) {
-                const uint32_t r = w * 4 + lane / 8 + 16 * j, in_tile = r & (kRowTile - 1);
-                const bool there = r < seg.nrows;
-                const uint32_t flat = seg.row0 + (there ? r : 0), token = p.group_div.div(flat);
-                const uint8_t* src = p.q + (seg.rows.row0 + token) * p.q_token
-                    + (at.head * p.tiling.group + flat - token * p.tiling.group) * p.q_head + (lane & 7) * 16;
-                const uint32_t dst = smem_u32(smem) + (r / kRowTile) * (kRowTile * D * 2) + in_tile * 128 + (((lane & 7) ^ (r & 7)) * 16);
+                for (uint32_t r = w * 4 + lane / 8; r < Shape::kRows; r += kWarpsK * 4) {
+                    const uint32_t in_tile = r & (kRowTile - 1);
+                    const bool there = r < seg.nrows;
+                    const uint32_t flat = seg.row0 + (there ? r : 0), token = p.group_div.div(flat);
+                    const uint8_t* src = p.q + (seg.rows.row0 + token) * p.q_token
+                        + (at.head * p.tiling.group + flat - token * p.tiling.group) * p.q_head + (lane & 7) * 16;
+                    const uint32_t dst = smem_u32(smem) + (r / kRowTile) * (kRowTile * D * 2) + in_tile * 128 + (((lane & 7) ^ (r & 7)) * 16);
 #pragma unroll
-                for (uint32_t panel = 0; panel < PANELS; ++panel)
-                    cp_async16z(dst + panel * kPiece, src + panel * 128, there);
-            }
-            copies.push(&bar.q_full);
+                    for (uint32_t panel = 0; panel < D / 64; ++panel)
+                        cp_async16z(dst + panel * (kRowTile * 128), src + panel * 128, there);
+                }
+                __syncwarp();
+                copies.push(&bar.q_full);
+                return true;
+            };
 
-            // KEYS keys from `key0` on, UNITS units of 16 bytes of each from `skip` bytes on, to panels of 64 elements
-            const auto load = [&](const PagedPool& pool, const CUtensorMap& map, uint32_t box, uint32_t key0, auto keys, auto units,
+            // A warp looks up the pages of its next piece before it waits for room.
+            struct Ahead {
+                uint32_t key0, slot; // slot, page: of this lane's box
+                int32_t page;
+                bool boxes;          // whole boxes of cached tokens
+            };
+            const auto look = [&](uint32_t piece) { // of the segment
+                Ahead a;
+                a.key0 = seg.tile0 * kKeyTile + (value ? piece * PIECE_KEYS : piece / PER_TILE * kKeyTile);
+                const uint32_t keys = value ? PIECE_KEYS : kKeyTile, box = value ? v_box : k_box;
+                a.slot = 0;
+                a.page = 0;
+                a.boxes = box != 0 && a.key0 >= seen_lo && a.key0 + keys <= seg.pages.length;
+                if (a.boxes) {
+                    const uint32_t per_panel = keys / box, panels = value ? D / 64 : PANELS;
+                    if (lane < per_panel * panels)
+                        a.page = page_of(p.view, seg.pages, a.key0 + lane % per_panel * box, &a.slot);
+                }
+                return a;
+            };
+            // KEYS keys, UNITS units of 16 bytes of each from `skip` bytes on, to panels of 64 elements
+            const auto load = [&](uint32_t piece, const Ahead& a, const PagedPool& pool, const CUtensorMap& map, uint32_t box, auto keys, auto units,
                                   uint32_t skip) {
                 constexpr uint32_t KEYS = decltype(keys)::value, UNITS = decltype(units)::value, AT_ONCE = 32 / UNITS;
-                const uint32_t s = piece % kPieces;
-                if (box != 0 && key0 >= seen_lo && key0 + KEYS <= seg.pages.length) {
-                    // whole boxes of cached tokens: a lane each
-                    const uint32_t per_panel = KEYS / box, boxes = per_panel * (UNITS / 8);
-                    const uint32_t panel = lane / per_panel, first = (lane - panel * per_panel) * box;
-                    uint32_t slot = 0;
-                    int32_t page = 0;
-                    if (lane < boxes)
-                        page = page_of(p.view, seg.pages, key0 + first, &slot);
-                    if (__all_sync(0xffffffffu, page >= 0)) {
-                        if (!wait(&bar.empty[s], ((piece / kPieces) & 1) ^ 1, ERR_PF_EMPTY_WAIT))
-                            return false;
-                        if (lane == 0)
-                            mbar_expect_tx(&bar.full[s], kPiece);
-                        __syncwarp();
-                        if (lane < boxes)
-                            tma_load_page(smem_u32(ring) + s * kPiece + panel * (KEYS * 128) + first * 128, &map, &bar.full[s],
-                                          static_cast<int>(skip / 2 + panel * 64), static_cast<int>(slot), static_cast<int>(at.head), page);
-                        return true;
-                    }
-                }
-                // where the rows of keys lane + 32 a begin, in units of 16 bytes; none: zeros
+                const uint32_t s = (before + piece) % slots;
+                const bool boxes = a.boxes && __all_sync(0xffffffffu, a.page >= 0);
+                // otherwise where the rows of keys lane + 32 j begin, in units of 16 bytes; none: zeros
                 uint32_t row[KEYS / 32];
+                if (!boxes) {
 #pragma unroll
-                for (uint32_t a = 0; a < KEYS / 32; ++a) {
-                    const uint32_t key = key0 + a * 32 + lane;
-                    row[a] = kNone;
-                    if (key >= seen_lo && key < seen_hi) {
-                        uint32_t slot;
-                        const int32_t page = page_of(p.view, seg.pages, key, &slot);
-                        if (page >= 0)
-                            row[a] = static_cast<uint32_t>((page * pool.page_stride + slot * pool.slot_stride) >> 4);
+                    for (uint32_t j = 0; j < KEYS / 32; ++j) {
+                        const uint32_t key = a.key0 + j * 32 + lane;
+                        row[j] = kNone;
+                        if (key >= seen_lo && key < seen_hi) {
+                            uint32_t slot;
+                            const int32_t page = page_of(p.view, seg.pages, key, &slot);
+                            if (page >= 0)
+                                row[j] = static_cast<uint32_t>((page * pool.page_stride + slot * pool.slot_stride) >> 4);
+                        }
                     }
                 }
-                if (!wait(&bar.empty[s], ((piece / kPieces) & 1) ^ 1, ERR_PF_EMPTY_WAIT))
+                if (!wait(&empty_bar[s], (((before + piece) / slots) & 1) ^ 1, ERR_PF_EMPTY_WAIT))
                     return false;
+                if (boxes) {
+                    const uint32_t per_panel = KEYS / box;
+                    if (lane == 0)
+                        mbar_expect_tx(&full_bar[s], kPiece);
+                    __syncwarp();
+                    if (lane < per_panel * (UNITS / 8)) {
+                        const uint32_t panel = lane / per_panel, first = (lane - panel * per_panel) * box;
+                        tma_load_page(ring_at + s * kPiece + panel * (KEYS * 128) + first * 128, &map, &full_bar[s],
+                                      static_cast<int>(skip / 2 + panel * 64), static_cast<int>(a.slot), static_cast<int>(at.head), a.page);
+                    }
+                    return true;
+                }
                 const uint8_t* const from = pool.data + at.head * pool.head_stride + skip + (lane % UNITS) * 16;
-                const uint32_t to = smem_u32(ring) + s * kPiece + (lane % UNITS / 8) * (KEYS * 128);
+                const uint32_t to = ring_at + s * kPiece + (lane % UNITS / 8) * (KEYS * 128);
 #pragma unroll
                 for (uint32_t j = 0; j < KEYS / AT_ONCE; ++j) {
                     const uint32_t key = j * AT_ONCE + lane / UNITS;
@@ -345,151 +340,167 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     cp_async16z(to + key * 128 + (((lane & 7) ^ (key & 7)) * 16),
                                 from + static_cast<uint64_t>(r == kNone ? 0 : r) * 16, r != kNone);
                 }
-                copies.push(&bar.full[s]);
+                copies.push(&full_bar[s]);
                 return true;
             };
-            const auto load_k = [&](uint32_t tile) {
-#pragma unroll 1
-                for (uint32_t panel = 0; panel < PANELS; ++panel, ++piece)
-                    if ((piece & 3) == w
-                        && !load(p.view.k, k_map, k_box, (seg.tile0 + tile) * kKeyTile, std::integral_constant<uint32_t, kKeyTile> {},
-                                 std::integral_constant<uint32_t, 8> {}, panel * 128))
-                        return false;
-                return true;
-            };
-            const auto load_v = [&](uint32_t tile) {
-#pragma unroll 1
-                for (uint32_t v = 0; v < PANELS; ++v, ++piece)
-                    if ((piece & 3) == w
-                        && !load(p.view.v, v_map, v_box, (seg.tile0 + tile) * kKeyTile + v * PIECE_KEYS,
-                                 std::integral_constant<uint32_t, PIECE_KEYS> {}, std::integral_constant<uint32_t, D / 8> {}, 0))
-                        return false;
-                return true;
-            };
-            ok = load_k(0);
-            for (uint32_t i = 0; ok && i < seg.count; ++i) {
-                if (i + 1 < seg.count)
-                    ok = load_k(i + 1);
-                ok = ok && load_v(i);
+            const uint32_t pieces = seg.count * PER_TILE;
+            uint32_t mine = (w + warps - before % warps) % warps; // the first that goes to one of this warp's slots
+            bool query = value; // loaded, or not this warp's business
+            Ahead ahead;
+            if (mine < pieces)
+                ahead = look(mine);
+            for (; ok && mine < pieces; mine += warps) {
+                const Ahead a = ahead;
+                if (mine + warps < pieces)
+                    ahead = look(mine + warps);
+                ok = value ? load(mine, a, p.view.v, v_map, v_box, std::integral_constant<uint32_t, PIECE_KEYS> {},
+                                  std::integral_constant<uint32_t, D / 8> {}, 0)
+                           : load(mine, a, p.view.k, k_map, k_box, std::integral_constant<uint32_t, kKeyTile> {},
+                                  std::integral_constant<uint32_t, 8 * PANELS> {}, mine % PER_TILE * (PANELS * 128));
+                if (ok && !query) { // behind the first piece, which may find room before the queries do
+                    ok = load_query();
+                    query = true;
+                }
             }
+            if (ok && !query)
+                ok = load_query();
+            before += pieces;
             ++segments;
-            left -= seg.count;
-            next_item(p, &at, row_tiles(p.tiling, seg.rows.fresh));
+            next_segment(p, seg, &at, &left);
         }
         copies.drain();
-    } else if (warp == Shape::kMmaWarp) {
+    } else if (warp >= Shape::kScoreWarp) {
         // ------------------------------------------------------------------------------- products --
-        if (elect_one()) {
-            constexpr uint32_t kFormat = (1u << 4) | (1u << 7) | (1u << 10) | ((kRowTile >> 4) << 24); // bf16 x bf16 -> f32
-            constexpr uint32_t kScores = kFormat | ((kKeyTile >> 3) << 17);
-            constexpr uint32_t kSums = kFormat | ((D >> 3) << 17) | (1u << 16);
-            uint32_t piece0 = 0, segments = 0, tiles[TILES] = {}, segs[TILES] = {}, weights[2] = {};
-            bool ok = true;
-            const auto wait_full = [&](uint32_t piece) {
-                const bool r = mbar_wait<true>(&bar.full[piece % kPieces], (piece / kPieces) & 1, &bar.abort, p.err, ERR_PF_FULL_WAIT);
-                tc_fence_after();
-                return r;
-            };
-            // scores of key tile i; the last query tile to use K lets go of it
-            const auto scores = [&](uint32_t i, uint32_t q, uint32_t slot, bool release) {
-                const uint32_t first = piece0 + k_piece(i, PANELS);
-#pragma unroll 1
-                for (uint32_t panel = 0; panel < PANELS; ++panel) {
-                    if (!wait_full(first + panel))
-                        return false;
-                    const uint32_t s = (first + panel) % kPieces;
-                    const uint64_t a = operand_desc(smem_u32(smem) + q * (kRowTile * D * 2) + panel * kPiece);
-                    const uint64_t b = operand_desc(smem_u32(ring) + s * kPiece);
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j)
-                        tc_mma_bf16(s_col(slot), a + 2 * j, b + 2 * j, kScores, panel > 0 || j > 0);
-                    if (release)
-                        tc_commit(&bar.empty[s]);
-                }
-                tc_commit(&bar.s_full[slot]);
-                return true;
-            };
-            const auto sums = [&](uint32_t i, uint32_t n, uint32_t q, uint32_t slot, bool release) {
-                if (!mbar_wait<true>(&bar.p_full[slot], weights[slot] & 1, &bar.abort, p.err, ERR_PF_WEIGHT_WAIT))
-                    return false;
-                ++weights[slot];
-                if (i == 0 && !mbar_wait<true>(&bar.o_free[q], (segs[q] & 1) ^ 1, &bar.abort, p.err, ERR_PF_SUM_WAIT))
-                    return false;
-                tc_fence_after();
-                const uint32_t first = piece0 + v_piece(i, n, PANELS);
-#pragma unroll 1
-                for (uint32_t v = 0; v < PANELS; ++v) {
-                    if (!wait_full(first + v))
-                        return false;
-                    const uint32_t s = (first + v) % kPieces;
-                    const uint64_t b = value_desc(smem_u32(ring) + s * kPiece, PIECE_KEYS * 128);
-                    constexpr uint32_t STEPS = PIECE_KEYS / 16;
-#pragma unroll
-                    for (uint32_t j = 0; j < STEPS; ++j) // 16 keys: 2048 bytes of V, eight columns of P
-                        mma_ts(o_col(q), s_col(slot) + (v * STEPS + j) * 8, b + j * (2048 >> 4), kSums, i > 0 || v > 0 || j > 0);
-                    if (release)
-                        tc_commit(&bar.empty[s]);
-                }
-                tc_commit(&bar.pv_done[q]);
-                return true;
-            };
-            while (ok && next_segment<Shape::kRows>(p, at, left, &seg)) {
-                const uint32_t n = seg.count;
-                ok = mbar_wait<true>(&bar.q_full, segments & 1, &bar.abort, p.err, ERR_PF_QUERY_WAIT);
-                tc_fence_after();
-                if constexpr (TILES == 1) {
-                    ok = ok && scores(0, 0, tiles[0] & 1, true);
-                    for (uint32_t i = 0; ok && i < n; ++i, ++tiles[0]) {
-                        if (i + 1 < n)
-                            ok = scores(i + 1, 0, (tiles[0] + 1) & 1, true);
-                        if (i + 2 == n || n == 1) // the segment's last scores are on their way
-                            tc_commit(&bar.q_free);
-                        ok = ok && sums(i, n, 0, tiles[0] & 1, true);
-                    }
-                } else {
-                    const bool second = seg.second;
-                    ok = ok && scores(0, 0, 0, !second);
-                    if (second)
-                        ok = ok && scores(0, 1, 1, true);
-                    for (uint32_t i = 0; ok && i < n; ++i) {
-                        const bool more = i + 1 < n;
-                        if (!more)
-                            tc_commit(&bar.q_free);
-                        ok = sums(i, n, 0, 0, !second);
-                        if (more)
-                            ok = ok && scores(i + 1, 0, 0, !second);
-                        if (second) {
-                            ok = ok && sums(i, n, 1, 1, true);
-                            if (more)
-                                ok = ok && scores(i + 1, 1, 1, true);
-                        }
-                    }
-                    if (second)
-                        ++segs[TILES - 1];
-                }
-                ++segs[0];
-                ++segments;
-                piece0 += 2 * n * PANELS;
-                left -= n;
-                next_item(p, &at, row_tiles(p.tiling, seg.rows.fresh));
-            }
-            // whatever was issued is complete before the tensor memory goes back
-            volatile uint32_t never = 0;
-            tc_commit(&bar.drain);
-            mbar_wait<true>(&bar.drain, 0, &never, p.err, ERR_PF_SUM_WAIT);
-        }
-        __syncwarp();
-    } else if (warp < Shape::kSoftmaxWarps) {
-        // -------------------------------------------------------------------------------- weights --
-        const uint32_t q = warp / 4;
-        const uint32_t lanes = (warp & 3) << 21; // this warp's 32 lanes of tensor memory
-        uint32_t tiles = 0;
+        // The whole warp goes through the loops and one lane issues.
+        constexpr uint32_t kFormat = (1u << 4) | (1u << 7) | (1u << 10) | ((kRowTile >> 4) << 24); // bf16 x bf16 -> f32
+        constexpr uint32_t kScores = kFormat | ((STEP >> 3) << 17);
+        constexpr uint32_t kSums = kFormat | ((D >> 3) << 17) | (1u << 16);
+        constexpr uint64_t kOperand = (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+        // V as the B operand with its n side contiguous: panels of 64 elements, keys 128 bytes apart, groups of eight keys 1024
+        constexpr uint64_t kValue = kOperand | (static_cast<uint64_t>(PIECE_KEYS * 128 >> 4) << 16);
+        const auto uniform = [](uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); };
+        const uint32_t ring_lo = uniform(smem_u32(ring) >> 4), query_lo = uniform(smem_u32(smem) >> 4), columns = uniform(tmem);
+        uint32_t before = 0, segments = 0;   // pieces of earlier segments, of K and as many of V
+        uint32_t done[2] = {}, segs[2] = {}; // steps and segments of a query tile
         bool ok = true;
-        while (ok && next_segment<Shape::kRows>(p, at, left, &seg)) {
-            const uint32_t n = seg.count;
-            if (q == 0 || seg.second) {
-                const uint32_t r = q * kRowTile + (warp & 3) * 32 + lane;
-                const bool live = r < seg.nrows;
+        const auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
+            return __all_sync(0xffffffffu, mbar_wait<true>(b, parity, &bar.abort, p.err, code)) != 0;
+        };
+        // Scores of step u of the segment, into a buffer whose weights have been used. The last to use a piece of K lets go of it.
+        const auto scores = [&](uint32_t u, uint32_t q, bool last) {
+            const uint32_t slot = q * BUFFERS + done[q] % BUFFERS, d = columns + 256 + slot * STEP;
+            if (done[q] >= BUFFERS && !wait(&bar.pv_done[slot], (done[q] / BUFFERS - 1) & 1, ERR_PF_SUM_WAIT))
+                return false;
+            tc_fence_after();
+            const uint32_t part = u % STEPS; // of the key tile
+#pragma unroll
+            for (uint32_t i = 0; i < PER_TILE; ++i) {
+                const uint32_t piece = before + u / STEPS * PER_TILE + i, s = piece % SLOTS_K;
+                if (part == 0 && q == 0 && !wait(&bar.k_full[s], (piece / SLOTS_K) & 1, ERR_PF_FULL_WAIT))
+                    return false;
+                const uint32_t a_lo = query_lo + (q * (kRowTile * D * 2) + i * (PANELS * kRowTile * 128)) / 16;
+                const uint32_t b_lo = uniform(ring_lo + s * (kPiece / 16) + part * (STEP * 128 / 16));
+                if (elect_one()) {
+#pragma unroll
+                    for (uint32_t j = 0; j < 4 * PANELS; ++j) {
+                        const uint32_t k = j / 4 * (kKeyTile * 128 / 16) + j % 4 * 2; // (query tiles are as high as key tiles)
+                        tc_mma_bf16(d, kOperand | (a_lo + k), kOperand | (b_lo + k), kScores, i > 0 || j > 0);
+                    }
+                    if (last && part + 1 == STEPS)
+                        tc_commit(&bar.k_empty[s]);
+                    if (i + 1 == PER_TILE)
+                        tc_commit(&bar.s_full[slot]);
+                }
+            }
+            ++done[q];
+            return true;
+        };
+        // The step's keys are PER_TILE pieces of V (one step per key tile), or a part of one piece.
+        static_assert(STEPS == 1 || PER_TILE == 1, "");
+        const auto sums = [&](uint32_t u, uint32_t q, bool last) {
+            const uint32_t slot = q * BUFFERS + done[q] % BUFFERS, part = u % STEPS;
+            const uint32_t d = columns + q * D, a = columns + 256 + slot * STEP;
+            if (u == 0 && !wait(&bar.o_free[q], (segs[q] & 1) ^ 1, ERR_PF_SUM_WAIT))
+                return false;
+#pragma unroll
+            for (uint32_t i = 0; i < PER_TILE; ++i) {
+                const uint32_t piece = before + u / STEPS * PER_TILE + i, s = piece % SLOTS_V;
+                if (part == 0 && q == 0 && !wait(&bar.v_full[s], (piece / SLOTS_V) & 1, ERR_PF_FULL_WAIT))
+                    return false;
+                if (i == 0) {
+                    if (!wait(&bar.p_full[slot], (done[q] / BUFFERS) & 1, ERR_PF_WEIGHT_WAIT))
+                        return false;
+                    tc_fence_after();
+                }
+                const uint32_t b_lo = uniform(ring_lo + (SLOTS_K + s) * (kPiece / 16) + part * (STEP * 128 / 16));
+                constexpr uint32_t COUNT = STEP / PER_TILE / 16; // products of 16 keys: 2048 bytes of V, eight columns of P
+                if (elect_one()) {
+#pragma unroll
+                    for (uint32_t j = 0; j < COUNT; ++j)
+                        mma_ts(d, a + (i * COUNT + j) * 8, kValue | (b_lo + j * (2048 >> 4)), kSums, u > 0 || i > 0 || j > 0);
+                    if (i + 1 == PER_TILE)
+                        tc_commit(&bar.pv_done[slot]);
+                    if (last && part + 1 == STEPS)
+                        tc_commit(&bar.v_empty[s]);
+                }
+            }
+            ++done[q];
+            return true;
+        };
+        while (ok && this_segment(p, at, left, &seg)) {
+            const uint32_t n = uniform(seg.count);
+            const bool second = TILES == 2 && uniform(seg.nrows) > kRowTile, score = warp == Shape::kScoreWarp;
+            if (score)
+                ok = wait(&bar.q_full, segments & 1, ERR_PF_QUERY_WAIT);
+            for (uint32_t u = 0; ok && u < n * STEPS; ++u)
+#pragma unroll
+                for (uint32_t q = 0; q < TILES; ++q)
+                    if (ok && (q == 0 || second))
+                        ok = score ? scores(u, q, q == 1 || !second) : sums(u, q, q == 1 || !second);
+            if (score && elect_one())
+                tc_commit(&bar.q_free);
+            ++segs[0];
+            segs[1] += second ? 1 : 0;
+            ++segments;
+            before += n * PER_TILE;
+            next_segment(p, seg, &at, &left);
+        }
+        // whatever was issued is complete before the tensor memory goes back
+        volatile uint32_t never = 0;
+        if (elect_one())
+            tc_commit(&bar.drain);
+        mbar_wait<true>(&bar.drain, 0, &never, p.err, ERR_PF_SUM_WAIT);
+        __syncwarp();
+    } else if (warp < kSoftmaxWarps) {
+        // -------------------------------------------------------------------------------- weights --
+        const uint32_t q = TILES == 1 ? 0 : warp / 4, half = TILES == 1 ? warp / 4 : 0;
+        const uint32_t lanes = (warp & 3) << 21, tile_row = (warp & 3) * 32 + lane; // 32 lanes of tensor memory
+        uint32_t done = 0;                                                          // steps
+        bool ok = true;
+        const auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
+            const bool r = __all_sync(0xffffffffu, mbar_wait(b, parity, &bar.abort, p.err, code)) != 0;
+            tc_fence_after();
+            return r;
+        };
+        // The sums of step `d`: its buffer's scores were not overwritten before those of d - BUFFERS were through, so the
+        // barrier's parity stands for this step.
+        const auto wait_sums = [&](uint32_t d) {
+            return wait(&bar.pv_done[q * BUFFERS + d % BUFFERS], (d / BUFFERS) & 1, ERR_PF_SUM_WAIT);
+        };
+        // True in all threads of the rows that this warp has a part in, where `v` is in any.
+        const auto any = [&](bool v) {
+            if constexpr (TILES == 2)
+                return __any_sync(0xffffffffu, v) != 0;
+            tc_fence_before(); // (the other warp's weights take the place of scores that this one has read)
+            const bool r = !group_all(1 + (warp & 3), 64, !v);
+            tc_fence_after();
+            return r;
+        };
+        while (ok && this_segment(p, at, left, &seg)) {
+            const uint32_t steps = seg.count * STEPS;
+            if (q * kRowTile < seg.nrows) {
+                const uint32_t r = q * kRowTile + tile_row;
+                const bool live = r < seg.nrows, idle = !__any_sync(0xffffffffu, live);
                 const uint32_t flat = seg.row0 + (live ? r : 0), token = p.group_div.div(flat);
                 uint32_t lo = 0, hi = 0xffffffffu; // (rows past the last one need no mask)
                 if (live) {
@@ -497,119 +508,105 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     hi = min(hi, seg.pages.length);
                 }
                 float m = -INFINITY, l = 0.0f;
-                for (uint32_t i = 0; i < n; ++i, ++tiles) {
-                    const uint32_t slot = TILES == 1 ? tiles & 1 : q;
-                    const uint32_t parity = TILES == 1 ? (tiles >> 1) & 1 : tiles & 1;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&bar.s_full[slot], parity, &bar.abort, p.err, ERR_PF_SCORE_WAIT));
+                for (uint32_t u = 0; u < steps; ++u, ++done) {
+                    const uint32_t slot = q * BUFFERS + done % BUFFERS;
+                    ok = wait(&bar.s_full[slot], (done / BUFFERS) & 1, ERR_PF_SCORE_WAIT);
+                    if constexpr (TILES == 1) // (the two warps of a row stop together)
+                        ok = group_all(1 + (warp & 3), 64, ok);
                     if (!ok)
                         break;
-                    tc_fence_after();
-                    const uint32_t s_addr = s_col(slot) + lanes;
-                    const uint32_t key0 = (seg.tile0 + i) * kKeyTile;
-                    const bool part = __any_sync(0xffffffffu, lo > key0 || hi < key0 + kKeyTile);
-
-                    uint32_t x[32];
-                    // both passes once with and once without the mask: a test inside them costs a branch per element
-                    const auto largest = [&](auto masked) {
+                    if (!idle) {
+                        const uint32_t s_addr = s_col(slot) + lanes;
+                        const uint32_t key0 = seg.tile0 * kKeyTile + u * STEP + half * kMine;
+                        const bool part = __any_sync(0xffffffffu, lo > key0 || hi < key0 + kMine);
+                        uint32_t x[kMine];
+                        tc_ld32(s_addr + half * kMine, x);
+                        tc_ld32(s_addr + half * kMine + 32, x + 32);
+                        tc_ld_wait32(x);
+                        tc_ld_wait32(x + 32);
+                        if (part) {
+#pragma unroll
+                            for (uint32_t j = 0; j < kMine; ++j)
+                                x[j] = key0 + j >= lo && key0 + j < hi ? x[j] : 0xff800000u; // -infinity
+                        }
                         float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-                        for (uint32_t c = 0; c < kKeyTile / 32; ++c) {
-                            tc_ld32(s_addr + c * 32, x);
-                            tc_ld_wait32(x);
-#pragma unroll
-                            for (uint32_t j = 0; j < 32; j += 2) {
-                                float a = __uint_as_float(x[j]), b = __uint_as_float(x[j + 1]);
-                                if constexpr (decltype(masked)::value) {
-                                    const uint32_t key = key0 + c * 32 + j;
-                                    a = key >= lo && key < hi ? a : -INFINITY;
-                                    b = key + 1 >= lo && key + 1 < hi ? b : -INFINITY;
-                                }
-                                if ((j & 2) == 0)
-                                    top0 = fmaxf(top0, fmaxf(a, b));
-                                else
-                                    top1 = fmaxf(top1, fmaxf(a, b));
-                            }
+                        for (uint32_t j = 0; j < kMine; j += 4) {
+                            top0 = fmaxf(top0, fmaxf(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
+                            top1 = fmaxf(top1, fmaxf(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])));
                         }
-                        return fmaxf(top0, top1);
-                    };
-                    float top = part ? largest(std::true_type {}) : largest(std::false_type {});
-                    top *= p.scale_log2;
-                    const bool grow = top > m + kGrowth; // (m = -inf: whenever something is seen)
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float next = grow ? top : m;
-                        const float keep = grow ? exp2_approx(m - next) : 1.0f;
-                        m = next;
-                        l *= keep;
-                        if (i > 0) { // O holds the sums up to tile i - 1 once its product is through
-                            ok = __all_sync(0xffffffffu, mbar_wait(&bar.pv_done[q], (tiles - 1) & 1, &bar.abort, p.err, ERR_PF_SUM_WAIT));
-                            if (!ok)
-                                break;
-                            tc_fence_after();
+                        float top = fmaxf(top0, top1) * p.scale_log2;
+                        if (any(top > m + kGrowth)) { // (m = -inf: whenever something is seen)
+                            if constexpr (TILES == 1) {
+                                bar.share[half][tile_row] = top;
+                                group_all(1 + (warp & 3), 64, true);
+                                top = fmaxf(top, bar.share[half ^ 1][tile_row]);
+                            }
+                            const bool grow = top > m + kGrowth;
+                            const float next = grow ? top : m;
+                            const float keep = grow ? exp2_approx(m - next) : 1.0f;
+                            m = next;
+                            l *= keep;
+                            if (u > 0) { // O holds the sums up to step u - 1 once they are through
+                                ok = wait_sums(done - 1);
+                                if (ok) {
+                                    uint32_t o[32];
 #pragma unroll 1
-                            for (uint32_t c = 0; c < D / 32; ++c) {
-                                tc_ld32(o_col(q) + lanes + c * 32, x);
-                                tc_ld_wait32(x);
+                                    for (uint32_t c = 0; c < D / 32 / (TILES == 1 ? 2 : 1); ++c) {
+                                        const uint32_t o_addr = o_col(q) + half * (D / 2) + lanes + c * 32;
+                                        tc_ld32(o_addr, o);
+                                        tc_ld_wait32(o);
 #pragma unroll
-                                for (uint32_t j = 0; j < 32; ++j)
-                                    x[j] = __float_as_uint(__uint_as_float(x[j]) * keep);
-                                tc_st16(o_col(q) + lanes + c * 32, x);
-                                tc_st16(o_col(q) + lanes + c * 32 + 16, x + 16);
+                                        for (uint32_t j = 0; j < 32; ++j)
+                                            o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                                        tc_st16(o_addr, o);
+                                        tc_st16(o_addr + 16, o + 16);
+                                    }
+                                }
                             }
                         }
-                    }
-                    const float base = m == -INFINITY ? 0.0f : m;
-                    const auto weights = [&](auto masked) {
+                        const float base = m == -INFINITY ? 0.0f : m;
                         float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-                        for (uint32_t c = 0; c < kKeyTile / 32; ++c) {
-                            tc_ld32(s_addr + c * 32, x);
-                            tc_ld_wait32(x);
+                        for (uint32_t c = 0; c < kMine / 32; ++c) {
                             uint32_t w[16];
 #pragma unroll
                             for (uint32_t j = 0; j < 16; ++j) {
-                                float a = fmaf(__uint_as_float(x[2 * j]), p.scale_log2, -base);
-                                float b = fmaf(__uint_as_float(x[2 * j + 1]), p.scale_log2, -base);
-                                if constexpr (decltype(masked)::value) {
-                                    const uint32_t key = key0 + c * 32 + 2 * j;
-                                    a = key >= lo && key < hi ? a : -INFINITY;
-                                    b = key + 1 >= lo && key + 1 < hi ? b : -INFINITY;
-                                }
-                                a = exp2_approx(a);
-                                b = exp2_approx(b);
+                                const float a = exp2_approx(fmaf(__uint_as_float(x[c * 32 + 2 * j]), p.scale_log2, -base));
+                                const float b = exp2_approx(fmaf(__uint_as_float(x[c * 32 + 2 * j + 1]), p.scale_log2, -base));
                                 sum0 += a;
                                 sum1 += b;
                                 w[j] = pack_bf16x2(a, b);
                             }
-                            tc_st16(s_addr + c * 16, w);
+                            tc_st16(s_addr + half * (kMine / 2) + c * 16, w);
                         }
-                        return sum0 + sum1;
-                    };
-                    l += part ? weights(std::true_type {}) : weights(std::false_type {});
-                    tc_st_wait();
+                        l += sum0 + sum1;
+                        tc_st_wait();
+                    }
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0)
                         mbar_arrive(&bar.p_full[slot]);
                 }
+                ok = ok && wait_sums(done - 1);
+                if constexpr (TILES == 1) {
+                    ok = group_all(1 + (warp & 3), 64, ok);
+                    bar.share[half][tile_row] = l;
+                    group_all(1 + (warp & 3), 64, true);
+                    l += bar.share[half ^ 1][tile_row];
+                }
                 if (!ok)
                     break;
-                // The last two products: a barrier's parity tells one phase from the next only, and with one query tile the
-                // scores that were waited for last are issued before the product of the tile before.
-                if (TILES == 1 && n > 1)
-                    ok = __all_sync(0xffffffffu, mbar_wait(&bar.pv_done[q], (tiles - 2) & 1, &bar.abort, p.err, ERR_PF_SUM_WAIT));
-                ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar.pv_done[q], (tiles - 1) & 1, &bar.abort, p.err, ERR_PF_SUM_WAIT));
-                if (!ok)
-                    break;
-                tc_fence_after();
-                const bool whole = n == seg.item_tiles;
+                const bool whole = seg.whole;
                 const uint32_t h = at.head * p.tiling.group + flat - token * p.tiling.group;
-                const size_t part_row = static_cast<size_t>(blockIdx.x * 2 + (at.offset == 0 ? 1 : 0)) * Shape::kRows + r;
+                const size_t part_row = static_cast<size_t>(blockIdx.x * 2 + (seg.starts ? 1 : 0)) * Shape::kRows + r;
                 uint8_t* const out = p.out + (seg.rows.row0 + token) * p.out_token + h * p.out_head;
                 float* const part_o = p.part_o + part_row * D;
                 const float inv = whole ? (m == -INFINITY ? 0.0f : 1.0f / l) : 1.0f;
                 uint32_t x[32];
 #pragma unroll 1
-                for (uint32_t c = 0; c < D / 32; ++c) {
+                for (uint32_t i = 0; i < D / 32 / (TILES == 1 ? 2 : 1); ++i) {
+                    const uint32_t c = half * (D / 64) + i;
                     tc_ld32(o_col(q) + lanes + c * 32, x);
                     tc_ld_wait32(x);
                     if (!live)
@@ -633,19 +630,18 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 __syncwarp();
                 if (lane == 0)
                     mbar_arrive(&bar.o_free[q]);
-                if (live && whole && p.lse != nullptr)
+                if (live && whole && half == 0 && p.lse != nullptr)
                     p.lse[(seg.rows.row0 + token) * p.lse_token + h * p.lse_head]
                         = m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
-                if (live && !whole)
+                if (live && !whole && half == 0)
                     p.part_ml[part_row] = make_float2(m, l);
             }
-            left -= n;
-            next_item(p, &at, row_tiles(p.tiling, seg.rows.fresh));
+            next_segment(p, seg, &at, &left);
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == Shape::kMmaWarp)
+    if (warp == Shape::kScoreWarp)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
 }
 

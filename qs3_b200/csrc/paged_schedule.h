@@ -2,10 +2,11 @@
 //
 // An item is a tile of query rows of one sequence and KV head: the rows of a sequence and KV head are its new tokens times the
 // query heads that share the KV head, row = token * group + head, cut into tiles of `tile_rows`. Its cost is the number of key
-// tiles that hold a key some row of it sees, at least one (an item without keys still writes its output). Items follow each
-// other by sequence, KV head, tile; their key tiles, laid end to end, are cut into equal ranges, one per block of the launch.
-// A range ends where it ends, inside an item as well, so that lengths which differ leave no block idle and a single long
-// context is spread over all SMs; an item cut this way leaves partial results that a second launch joins.
+// tiles that hold a key some row of it sees, at least one (an item without keys still writes its output), and `item_cost`
+// more for its start and end. Items follow each other by sequence, KV head, tile; their costs, laid end to end, are cut into
+// equal ranges, one per block of the launch. A range ends where it ends, inside an item as well, so that lengths which differ
+// leave no block idle and a single long context is spread over all SMs; an item whose key tiles are cut this way leaves
+// partial results that a second launch joins.
 #pragma once
 
 #include <cstdint>
@@ -44,6 +45,7 @@ struct AttnTiling {
     uint32_t kv_heads;
     uint32_t window;    // 0: none
     uint32_t causal;
+    uint32_t item_cost; // in key tiles
 };
 
 struct KeyTiles {
@@ -89,13 +91,27 @@ QS3_HD uint32_t active_blocks(uint64_t total, uint32_t blocks, uint32_t least)
     return n < blocks ? static_cast<uint32_t>(n) : blocks;
 }
 
-// First key tile of block `c` of `blocks`. (c * total stays below 2^63: total <= 2^52 and blocks < 2^11 by the limits of the entry point.)
+// Where the range of block `c` of `blocks` begins. (c * total stays below 2^63: total <= 2^52 and blocks < 2^11 by the limits of the entry point.)
 QS3_HD uint64_t block_begin(uint64_t total, uint32_t blocks, uint32_t c) { return total * c / blocks; }
 
-// Where a position in the row of all key tiles lies.
+// The last block whose range begins before `end`.
+QS3_HD uint32_t block_of_end(uint64_t total, uint32_t blocks, uint64_t end)
+{
+    // total * c / blocks < end exactly when total * c < end * blocks
+    return static_cast<uint32_t>((end * blocks - 1) / total);
+}
+
+// Key tiles of an item that lie before a position `offset` from its beginning.
+QS3_HD uint32_t tiles_before(const AttnTiling& a, uint64_t offset, uint32_t tiles)
+{
+    const uint64_t t = offset > a.item_cost ? offset - a.item_cost : 0;
+    return t < tiles ? static_cast<uint32_t>(t) : tiles;
+}
+
+// Where a position in the row of all items lies.
 struct AttnPlace {
     uint32_t seq, head, tile;
-    uint32_t offset; // key tiles of the item before the position
+    uint32_t offset; // from the item's beginning
 };
 
 } // namespace qs3

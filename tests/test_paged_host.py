@@ -38,7 +38,7 @@ int main()
     for (uint32_t length : { 0u, 1u, 2u, 63u, 64u, 65u, 300u, 1000u }) {
         if (window != 0 && causal == 0)
             continue;
-        const AttnTiling a { group, rows, keys, 2, window, causal };
+        const AttnTiling a { group, rows, keys, 2, window, causal, 0 };
         const uint32_t tiles = row_tiles(a, fresh);
         CHECK(uint64_t(tiles) * rows >= uint64_t(fresh) * group && uint64_t(tiles - 1) * rows < uint64_t(fresh) * group);
         for (uint32_t t = 0; t < tiles; ++t) {
@@ -62,6 +62,12 @@ int main()
                 CHECK(k.first <= low / keys && k.end == (high + keys - 1) / keys);
         }
     }
+    // key tiles of an item before a place in it
+    for (uint32_t cost : { 0u, 1u, 3u }) {
+        const AttnTiling a { 1, 8, 64, 1, 0, 1, cost };
+        for (uint64_t offset = 0; offset < 20; ++offset)
+            CHECK(tiles_before(a, offset, 10) == (offset <= cost ? 0 : offset - cost < 10 ? offset - cost : 10));
+    }
     // ranges follow each other, hold everything and differ by one at most
     for (uint64_t total : { 1ull, 2ull, 147ull, 148ull, 149ull, 12345ull, 1ull << 52 })
         for (uint32_t blocks : { 1u, 148u, 1184u })
@@ -71,6 +77,9 @@ int main()
                 for (uint32_t c = 0; c < n; ++c) {
                     const uint64_t size = block_begin(total, n, c + 1) - block_begin(total, n, c);
                     CHECK(size == total / n || size == total / n + 1);
+                    // the last block that begins before some place
+                    for (uint64_t end : { block_begin(total, n, c) + 1, block_begin(total, n, c + 1) })
+                        CHECK(block_of_end(total, n, end) == c);
                 }
             }
     return 0;
