@@ -143,7 +143,7 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
             const uint32_t r = i / (D / 8), c = i % (D / 8);
             uint4 w = make_uint4(0, 0, 0, 0);
             if (r < nrows) {
-                const uint32_t token = p.group_div.div(row0 + r), h = at.head * p.tiling.group + row0 + r - token * p.tiling.group;
+                const uint32_t token = p.tiling.group.div(row0 + r), h = at.head * p.tiling.group.d + row0 + r - token * p.tiling.group.d;
                 w = *reinterpret_cast<const uint4*>(p.q + (rows.row0 + token) * p.q_token + h * p.q_head + c * 16);
             }
             *reinterpret_cast<uint4*>(s_q + swizzled<D * 2>(r, c)) = w;
@@ -152,8 +152,8 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
 
         // keys that any row sees: others are not fetched, and whatever they hold does not count
         uint32_t seen_lo, seen_hi, unused;
-        visible_keys(p.tiling, rows.fresh, pages.length, p.group_div.div(row0), &seen_lo, &unused);
-        visible_keys(p.tiling, rows.fresh, pages.length, p.group_div.div(row0 + nrows - 1), &unused, &seen_hi);
+        visible_keys(p.tiling, rows.fresh, pages.length, p.tiling.group.div(row0), &seen_lo, &unused);
+        visible_keys(p.tiling, rows.fresh, pages.length, p.tiling.group.div(row0 + nrows - 1), &unused, &seen_hi);
         seen_hi = min(seen_hi, pages.length);
         // keys that the rows of this lane's columns see
         uint32_t lo[NT][2], hi[NT][2];
@@ -164,7 +164,7 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
                 const uint32_t r = n * 8 + (lane & 3) * 2 + j;
                 lo[n][j] = hi[n][j] = 0;
                 if (r < nrows) {
-                    visible_keys(p.tiling, rows.fresh, pages.length, p.group_div.div(row0 + r), &lo[n][j], &hi[n][j]);
+                    visible_keys(p.tiling, rows.fresh, pages.length, p.tiling.group.div(row0 + r), &lo[n][j], &hi[n][j]);
                     hi[n][j] = min(hi[n][j], pages.length);
                 }
             }
@@ -417,7 +417,7 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
                 acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
             }
             if (whole) {
-                const uint32_t token = p.group_div.div(row0 + r), h = at.head * p.tiling.group + row0 + r - token * p.tiling.group;
+                const uint32_t token = p.tiling.group.div(row0 + r), h = at.head * p.tiling.group.d + row0 + r - token * p.tiling.group.d;
                 const float inv = top == -INFINITY ? 0.0f : 1.0f / sum;
                 const uint2 w = make_uint2(tc::pack_bf16x2(acc.x * inv, acc.y * inv), tc::pack_bf16x2(acc.z * inv, acc.w * inv));
                 *reinterpret_cast<uint2*>(p.out + (rows.row0 + token) * p.out_token + h * p.out_head + e * 2) = w;
@@ -444,17 +444,17 @@ template <uint32_t D, bool SHARED> __global__ void __launch_bounds__(kJoinWarps 
     __shared__ float s_acc[SHARED ? kJoinWarps * D : 1];
     chain_begin();
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    const uint32_t r = SHARED ? blockIdx.y : blockIdx.y * kJoinWarps + warp;
+    const uint32_t r = SHARED ? blockIdx.y : blockIdx.y * kJoinWarps + warp, rows_of_item = 1u << p.tiling.row_shift;
     for (uint32_t c = blockIdx.x + 1; c < p.blocks; c += gridDim.x) {
         const SplitNote n = p.notes[c];
         if (n.parts == 0)
             continue;
         const SeqRows rows = seq_rows(p, n.seq);
-        const uint32_t row0 = n.tile * p.tiling.tile_rows;
-        if (r >= p.tiling.tile_rows || row0 + r >= static_cast<uint64_t>(rows.fresh) * p.tiling.group)
+        const uint32_t row0 = n.tile << p.tiling.row_shift;
+        if (row0 + r >= rows.fresh * p.tiling.group.d)
             continue;
         const auto slot_of = [&](uint32_t i) {
-            return static_cast<size_t>(i == 0 ? 2 * c - 1 : 2 * (c + i - 1)) * p.tiling.tile_rows + r;
+            return static_cast<size_t>(i == 0 ? 2 * c - 1 : 2 * (c + i - 1)) * rows_of_item + r;
         };
         float top = -INFINITY, sum = 0.0f;
         for (uint32_t i = lane; i <= n.parts; i += 32)
@@ -507,7 +507,7 @@ template <uint32_t D, bool SHARED> __global__ void __launch_bounds__(kJoinWarps 
                     acc[j] += s_acc[w * D + lane * E + j];
         }
         const float inv = top == -INFINITY ? 0.0f : 1.0f / sum;
-        const uint32_t token = p.group_div.div(row0 + r), h = n.head * p.tiling.group + row0 + r - token * p.tiling.group;
+        const uint32_t token = p.tiling.group.div(row0 + r), h = n.head * p.tiling.group.d + row0 + r - token * p.tiling.group.d;
         uint8_t* out = p.out + (rows.row0 + token) * p.out_token + h * p.out_head + lane * E * 2;
         uint32_t w[E / 2];
 #pragma unroll
@@ -556,7 +556,7 @@ uint32_t attn_stream_blocks(uint32_t tile_rows, uint32_t head_dim, bool fp8)
 cudaError_t launch_attn_stream(const AttnParams& p, bool fp8, cudaStream_t stream)
 {
     const uint32_t d = p.view.head_dim;
-    const bool two = p.tiling.tile_rows == 16;
+    const bool two = p.tiling.row_shift == 4;
 #define QS3_STREAM(DIM)                                                                                                      \
     if (d == DIM)                                                                                                            \
         return two ? (fp8 ? launch_stream_as<DIM, 2, true>(p, stream) : launch_stream_as<DIM, 2, false>(p, stream))          \
@@ -572,11 +572,12 @@ cudaError_t launch_attn_join(const AttnParams& p, cudaStream_t stream)
 {
     const uint32_t d = p.view.head_dim;
     const uint32_t wide = p.blocks - 1 < kSmCount ? p.blocks - 1 : kSmCount;
-    if (p.tiling.tile_rows <= 16)
+    const uint32_t rows = 1u << p.tiling.row_shift;
+    if (rows <= 16)
         return launch_chained(d == 64 ? attn_join_kernel<64, true> : d == 128 ? attn_join_kernel<128, true> : attn_join_kernel<256, true>,
-                              dim3(wide, p.tiling.tile_rows), kJoinWarps * 32, 0, stream, p);
+                              dim3(wide, rows), kJoinWarps * 32, 0, stream, p);
     return launch_chained(d == 64 ? attn_join_kernel<64, false> : d == 128 ? attn_join_kernel<128, false> : attn_join_kernel<256, false>,
-                          dim3(wide, p.tiling.tile_rows / kJoinWarps), kJoinWarps * 32, 0, stream, p);
+                          dim3(wide, rows / kJoinWarps), kJoinWarps * 32, 0, stream, p);
 }
 
 } // namespace qs3
@@ -710,8 +711,6 @@ qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_des
     p.out_head = d->out.stride[1] * 2;
     p.rows = static_cast<uint32_t>(rows);
     p.heads = static_cast<uint32_t>(heads);
-    p.group_div = FastDiv(static_cast<uint32_t>(group));
-    p.head_div = FastDiv(p.view.kv_heads);
     p.scale_log2 = (d->sm_scale == 0.0f ? 1.0f / sqrtf(static_cast<float>(dim)) : d->sm_scale) * 1.4426950408889634f;
     p.err = p.view.err = device_error_word();
     if (p.err == nullptr)
@@ -723,7 +722,7 @@ qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_des
                                                        : static_cast<uint64_t>(rows);
     const uint64_t room = static_cast<uint64_t>(p.view.num_indices) * p.view.page_size;
     const uint64_t longest = d->max_kv_len != 0 && d->max_kv_len < room ? d->max_kv_len : room;
-    p.tiling.group = static_cast<uint32_t>(group);
+    p.tiling.group = FastDiv(static_cast<uint32_t>(group));
     p.tiling.kv_heads = p.view.kv_heads;
     p.tiling.window = d->window;
     p.tiling.causal = d->causal;
@@ -732,20 +731,23 @@ qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_des
         return static_cast<int64_t>(p.view.pages - 1) * pool.page_stride + static_cast<int64_t>(p.view.page_size - 1) * pool.slot_stride;
     };
     const bool chunks = !fp8 && fresh * group > 16 && reach(p.view.k) < (int64_t { 1 } << 36) && reach(p.view.v) < (int64_t { 1 } << 36);
+    uint32_t item_rows;
     if (chunks) {
-        p.tiling.tile_rows = attn_prefill_rows(dim);
-        p.tiling.key_tile = 128;
+        item_rows = attn_prefill_rows(dim);
+        p.tiling.key_shift = 7;
         p.tiling.item_cost = 4;
         p.blocks = kSmCount;
     } else {
-        p.tiling.tile_rows = attn_stream_rows(fresh * group > 16 ? 16 : static_cast<uint32_t>(fresh * group), dim);
-        p.tiling.key_tile = kStreamKeys;
+        item_rows = attn_stream_rows(fresh * group > 16 ? 16 : static_cast<uint32_t>(fresh * group), dim);
+        p.tiling.key_shift = 6;
         p.tiling.item_cost = 1;
-        p.blocks = attn_stream_blocks(p.tiling.tile_rows, dim, fp8);
+        p.blocks = attn_stream_blocks(item_rows, dim, fp8);
     }
+    while ((1u << p.tiling.row_shift) < item_rows)
+        ++p.tiling.row_shift;
     p.least = p.tiling.item_cost + 1;
     (void)longest;
-    const AttnSizes at = attn_sizes(p.blocks, p.tiling.tile_rows, dim);
+    const AttnSizes at = attn_sizes(p.blocks, item_rows, dim);
     char* ws = static_cast<char*>(d->workspace.data);
     p.notes = reinterpret_cast<SplitNote*>(ws + at.notes);
     p.part_ml = reinterpret_cast<float2*>(ws + at.ml);

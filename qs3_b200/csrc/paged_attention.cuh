@@ -17,12 +17,11 @@ struct AttnParams {
     int64_t lse_token, lse_head;
     const int32_t* q_indptr;
     uint32_t rows, heads;
-    FastDiv group_div, head_div; // by group, by kv_heads
     float scale_log2;            // sm_scale * log2(e)
     uint32_t blocks;             // of the launch
     uint32_t least;              // key tiles of a block
-    // Partial results. Block c has two slots of [tile_rows, head_dim] f32 weighted sums and [tile_rows] maxima (in units of
-    // log2) and sums: 0 for an item that began in an earlier block, 1 for one that begins here and goes on in the next.
+    // Partial results. Block c has two slots of [rows of an item, head_dim] f32 weighted sums and [rows] maxima (in units of log2) and
+    // sums: 0 for an item that began in an earlier block, 1 for one that begins here and goes on in the next.
     float* part_o;
     float2* part_ml;
     struct SplitNote* notes; // [blocks]
@@ -207,10 +206,12 @@ __device__ __forceinline__ void note_split(const AttnParams& p, const BlockRange
 
 // A block's part of an item. `at` moves along the block's range with `left`; false: the range is through.
 struct Segment {
+    uint32_t seq = 0xffffffffu; // of rows and pages
     SeqRows rows;
     SeqPages pages;
     uint32_t row0, nrows;  // of the item, among the sequence's
     uint32_t tile0, count; // key tiles
+    uint32_t tiles;        // of the item
     bool starts, whole;    // with the item's first key tile; with all of them
 };
 
@@ -218,12 +219,15 @@ __device__ __forceinline__ bool this_segment(const AttnParams& p, const AttnPlac
 {
     if (left == 0 || at.seq >= p.view.batch)
         return false;
-    s->rows = seq_rows(p, at.seq);
-    s->pages = seq_pages(p.view, at.seq);
+    if (s->seq != at.seq) {
+        s->seq = at.seq;
+        s->rows = seq_rows(p, at.seq);
+        s->pages = seq_pages(p.view, at.seq);
+    }
     if (s->rows.fresh == 0)
         return false;
     const KeyTiles keys = key_tiles(p.tiling, s->rows.fresh, s->pages.length, at.tile);
-    const uint32_t tiles = keys.end - keys.first;
+    const uint32_t tiles = s->tiles = keys.end - keys.first;
     const uint32_t from = tiles_before(p.tiling, at.offset, tiles), to = tiles_before(p.tiling, at.offset + left, tiles);
     if (from >= to)
         return false; // the range ends before the item's first key tile
@@ -231,16 +235,14 @@ __device__ __forceinline__ bool this_segment(const AttnParams& p, const AttnPlac
     s->tile0 = keys.first + from;
     s->starts = from == 0;
     s->whole = s->count == tiles;
-    s->row0 = at.tile * p.tiling.tile_rows;
-    s->nrows = static_cast<uint32_t>(min(static_cast<uint64_t>(p.tiling.tile_rows),
-                                         static_cast<uint64_t>(s->rows.fresh) * p.tiling.group - s->row0));
+    s->row0 = at.tile << p.tiling.row_shift;
+    s->nrows = min(1u << p.tiling.row_shift, s->rows.fresh * p.tiling.group.d - s->row0);
     return true;
 }
 
 __device__ __forceinline__ void next_segment(const AttnParams& p, const Segment& s, AttnPlace* at, uint64_t* left)
 {
-    const KeyTiles keys = key_tiles(p.tiling, s.rows.fresh, s.pages.length, at->tile);
-    const uint64_t rest = static_cast<uint64_t>(p.tiling.item_cost) + (keys.end - keys.first) - at->offset;
+    const uint64_t rest = static_cast<uint64_t>(p.tiling.item_cost) + s.tiles - at->offset;
     *left = *left > rest ? *left - rest : 0;
     next_item(p, at, row_tiles(p.tiling, s.rows.fresh));
 }

@@ -252,8 +252,8 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
         };
         while (ok && this_segment(p, at, left, &seg)) {
             uint32_t seen_lo, seen_hi, unused;
-            visible_keys(p.tiling, seg.rows.fresh, seg.pages.length, p.group_div.div(seg.row0), &seen_lo, &unused);
-            visible_keys(p.tiling, seg.rows.fresh, seg.pages.length, p.group_div.div(seg.row0 + seg.nrows - 1), &unused, &seen_hi);
+            visible_keys(p.tiling, seg.rows.fresh, seg.pages.length, p.tiling.group.div(seg.row0), &seen_lo, &unused);
+            visible_keys(p.tiling, seg.rows.fresh, seg.pages.length, p.tiling.group.div(seg.row0 + seg.nrows - 1), &unused, &seen_hi);
             seen_hi = min(seen_hi, seg.pages.length);
 
             const auto load_query = [&] {
@@ -263,9 +263,9 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 for (uint32_t r = w * 4 + lane / 8; r < Shape::kRows; r += kWarpsK * 4) {
                     const uint32_t in_tile = r & (kRowTile - 1);
                     const bool there = r < seg.nrows;
-                    const uint32_t flat = seg.row0 + (there ? r : 0), token = p.group_div.div(flat);
+                    const uint32_t flat = seg.row0 + (there ? r : 0), token = p.tiling.group.div(flat);
                     const uint8_t* src = p.q + (seg.rows.row0 + token) * p.q_token
-                        + (at.head * p.tiling.group + flat - token * p.tiling.group) * p.q_head + (lane & 7) * 16;
+                        + (at.head * p.tiling.group.d + flat - token * p.tiling.group.d) * p.q_head + (lane & 7) * 16;
                     const uint32_t dst = smem_u32(smem) + (r / kRowTile) * (kRowTile * D * 2) + in_tile * 128 + (((lane & 7) ^ (r & 7)) * 16);
 #pragma unroll
                     for (uint32_t panel = 0; panel < D / 64; ++panel)
@@ -501,7 +501,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
             if (q * kRowTile < seg.nrows) {
                 const uint32_t r = q * kRowTile + tile_row;
                 const bool live = r < seg.nrows, idle = !__any_sync(0xffffffffu, live);
-                const uint32_t flat = seg.row0 + (live ? r : 0), token = p.group_div.div(flat);
+                const uint32_t flat = seg.row0 + (live ? r : 0), token = p.tiling.group.div(flat);
                 uint32_t lo = 0, hi = 0xffffffffu; // (rows past the last one need no mask)
                 if (live) {
                     visible_keys(p.tiling, seg.rows.fresh, seg.pages.length, token, &lo, &hi);
@@ -598,7 +598,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 if (!ok)
                     break;
                 const bool whole = seg.whole;
-                const uint32_t h = at.head * p.tiling.group + flat - token * p.tiling.group;
+                const uint32_t h = at.head * p.tiling.group.d + flat - token * p.tiling.group.d;
                 const size_t part_row = static_cast<size_t>(blockIdx.x * 2 + (seg.starts ? 1 : 0)) * Shape::kRows + r;
                 uint8_t* const out = p.out + (seg.rows.row0 + token) * p.out_token + h * p.out_head;
                 float* const part_o = p.part_o + part_row * D;

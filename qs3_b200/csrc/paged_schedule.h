@@ -1,7 +1,7 @@
 // Division of attention over a paged cache into pieces of equal work. Arithmetic only, for the kernels and for the host.
 //
 // An item is a tile of query rows of one sequence and KV head: the rows of a sequence and KV head are its new tokens times the
-// query heads that share the KV head, row = token * group + head, cut into tiles of `tile_rows`. Its cost is the number of key
+// query heads that share the KV head, row = token * group + head, cut into tiles of 1 << row_shift. Its cost is the number of key
 // tiles that hold a key some row of it sees, at least one (an item without keys still writes its output), and `item_cost`
 // more for its start and end. Items follow each other by sequence, KV head, tile; their costs, laid end to end, are cut into
 // equal ranges, one per block of the launch. A range ends where it ends, inside an item as well, so that lengths which differ
@@ -39,9 +39,9 @@ struct FastDiv {
 };
 
 struct AttnTiling {
-    uint32_t group;     // query heads per KV head
-    uint32_t tile_rows; // rows of an item
-    uint32_t key_tile;  // keys of a key tile
+    FastDiv group;      // by the query heads per KV head
+    uint32_t row_shift; // log2 of the rows of an item
+    uint32_t key_shift; // log2 of the keys of a key tile
     uint32_t kv_heads;
     uint32_t window;    // 0: none
     uint32_t causal;
@@ -52,10 +52,10 @@ struct KeyTiles {
     uint32_t first, end; // end > first
 };
 
-// Row tiles of a sequence with `fresh` new tokens.
+// Row tiles of a sequence with `fresh` new tokens. (Rows, and positions, stay below 2^31 by the limits of the entry point.)
 QS3_HD uint32_t row_tiles(const AttnTiling& a, uint32_t fresh)
 {
-    return static_cast<uint32_t>((static_cast<uint64_t>(fresh) * a.group + a.tile_rows - 1) / a.tile_rows);
+    return (fresh * a.group.d + (1u << a.row_shift) - 1) >> a.row_shift;
 }
 
 // Keys [lo, hi) that new token `i` of `fresh` sees in a cache of `length` tokens (its own position: length - fresh + i).
@@ -70,15 +70,14 @@ QS3_HD void visible_keys(const AttnTiling& a, uint32_t fresh, uint32_t length, u
 
 QS3_HD KeyTiles key_tiles(const AttnTiling& a, uint32_t fresh, uint32_t length, uint32_t tile)
 {
-    const uint64_t rows = static_cast<uint64_t>(fresh) * a.group;
-    const uint64_t r0 = static_cast<uint64_t>(tile) * a.tile_rows;
-    const uint64_t r1 = (r0 + a.tile_rows < rows ? r0 + a.tile_rows : rows) - 1;
+    const uint32_t rows = fresh * a.group.d, r0 = tile << a.row_shift, next = r0 + (1u << a.row_shift);
+    const uint32_t r1 = (next < rows ? next : rows) - 1;
     uint32_t lo, hi, unused;
-    visible_keys(a, fresh, length, static_cast<uint32_t>(r0 / a.group), &lo, &unused);
-    visible_keys(a, fresh, length, static_cast<uint32_t>(r1 / a.group), &unused, &hi);
+    visible_keys(a, fresh, length, a.group.div(r0), &lo, &unused);
+    visible_keys(a, fresh, length, a.group.div(r1), &unused, &hi);
     KeyTiles k;
-    k.first = lo / a.key_tile;
-    k.end = (hi + a.key_tile - 1) / a.key_tile;
+    k.first = lo >> a.key_shift;
+    k.end = (hi + (1u << a.key_shift) - 1) >> a.key_shift;
     if (k.end <= k.first)
         k.end = k.first + 1;
     return k;

@@ -30,15 +30,16 @@ int main()
     }
     // every key that a row sees lies in its item's key tiles, every key tile holds one, an item has one at least
     for (uint32_t group : { 1u, 2u, 5u, 16u })
-    for (uint32_t rows : { 8u, 16u, 128u })
-    for (uint32_t keys : { 64u, 128u })
+    for (uint32_t row_shift : { 3u, 4u, 7u, 8u })
+    for (uint32_t key_shift : { 6u, 7u })
     for (uint32_t window : { 0u, 1u, 7u, 200u })
     for (uint32_t causal : { 0u, 1u })
     for (uint32_t fresh : { 1u, 2u, 3u, 70u, 257u })
     for (uint32_t length : { 0u, 1u, 2u, 63u, 64u, 65u, 300u, 1000u }) {
         if (window != 0 && causal == 0)
             continue;
-        const AttnTiling a { group, rows, keys, 2, window, causal, 0 };
+        const uint32_t rows = 1u << row_shift, keys = 1u << key_shift;
+        const AttnTiling a { FastDiv(group), row_shift, key_shift, 2, window, causal, 0 };
         const uint32_t tiles = row_tiles(a, fresh);
         CHECK(uint64_t(tiles) * rows >= uint64_t(fresh) * group && uint64_t(tiles - 1) * rows < uint64_t(fresh) * group);
         for (uint32_t t = 0; t < tiles; ++t) {
@@ -64,7 +65,7 @@ int main()
     }
     // key tiles of an item before a place in it
     for (uint32_t cost : { 0u, 1u, 3u }) {
-        const AttnTiling a { 1, 8, 64, 1, 0, 1, cost };
+        const AttnTiling a { FastDiv(1), 3, 6, 1, 0, 1, cost };
         for (uint64_t offset = 0; offset < 20; ++offset)
             CHECK(tiles_before(a, offset, 10) == (offset <= cost ? 0 : offset - cost < 10 ? offset - cost : 10));
     }
