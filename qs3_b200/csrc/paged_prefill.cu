@@ -4,13 +4,15 @@
 // query heads that share a KV head, so that a short chunk still fills a tile. Keys arrive by 128 and pass in steps of 128 (one
 // query tile) or 64 (two):
 //   S = Q K^T           tcgen05.mma 128 x 128 or 128 x 64, both operands in shared memory
-//   P = exp2(c S - m)   tensor memory -> registers -> tensor memory, where P (16 bits) takes the place of S; a thread has 64 keys
-//                       of a row: half a step with one query tile, whose row two threads share, else a step of its own row
+//   P = exp2(c S - m)   tensor memory -> registers -> tensor memory, in 16 bits; a thread has 64 keys of a row: half a step with
+//                       one query tile, whose row two threads share, else a step of its own row
 //   O += P V            tcgen05.mma 128 x head_dim, P from tensor memory, V as it lies in the cache (its rows along k)
-// Two score tiles of each query tile fit beside O (512 columns), so that scores run ahead of the weights and products beside
-// exponentials, which eight warps share because one alone waits longer for each of its instructions than they take. One warp
-// issues the scores and another the sums: every wait, product and commit costs its thread 50 to 100 cycles, together twice as
-// much as the products take.
+// Beside O (256 columns of 512) there is room for one score tile of each query tile and two of its weights. Scores are read into
+// registers at once, so that the next ones are on their way while their exponentials are taken: where weights took the place of
+// the scores that they came from, with two such tiles in turn, the scores waited for the sums of the step before the last
+// (8192 tokens of 16 heads of 256: 559 us). Eight warps take the exponentials, because one alone waits longer for each of its
+// instructions than they take. One warp issues the scores and another the sums: every wait, product and commit costs its thread
+// 50 to 100 cycles, together twice as much as the products take.
 // m follows the row's maximum only when that has grown by 2^8 (the weights stay below 256, the sums take the difference):
 // steps that rescale O in tensor memory are then few.
 //
@@ -51,7 +53,8 @@ enum : uint32_t {
 struct Barriers {
     uint64_t k_full[6], k_empty[6], v_full[4], v_empty[4];
     uint64_t q_full, q_free;
-    uint64_t s_full[4], p_full[4], pv_done[4], o_free[2]; // of the score tiles, and of the query tiles
+    uint64_t s_full[2], s_free[2], o_free[2]; // of a query tile
+    uint64_t p_full[2][2], pv_done[2][2];     // of its tiles of weights
     uint64_t drain;
     float share[2][kRowTile]; // between the two threads of a row
     uint32_t tmem;
@@ -62,7 +65,6 @@ template <uint32_t D> struct PrefillShape {
     static constexpr uint32_t kTiles = D == 256 ? 1 : 2; // query tiles
     static constexpr uint32_t kStep = kTiles == 1 ? 128 : 64; // keys of a score tile
     static constexpr uint32_t kSteps = kKeyTile / kStep;      // of a key tile
-    static constexpr uint32_t kBuffers = 2;                   // score tiles of a query tile
     static constexpr uint32_t kRows = kTiles * kRowTile;
     static constexpr uint32_t kPiece = D == 64 ? 16384 : 32768;
     static constexpr uint32_t kSlotsK = D == 64 ? 6 : 3, kSlotsV = D == 64 ? 4 : 2; // of the rings
@@ -131,6 +133,28 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r)
 
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two floats in a register pair, one instruction for both.
+__device__ __forceinline__ uint64_t pack2(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float low2(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float high2(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 __device__ __forceinline__ float exp2_approx(float x)
 {
     float r;
@@ -181,7 +205,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     const __grid_constant__ CUtensorMap v_map, const uint32_t k_box, const uint32_t v_box)
 {
     using Shape = PrefillShape<D>;
-    constexpr uint32_t TILES = Shape::kTiles, STEP = Shape::kStep, STEPS = Shape::kSteps, BUFFERS = Shape::kBuffers, PANELS = Shape::kPanels, PIECE_KEYS = Shape::kPieceKeys;
+    constexpr uint32_t TILES = Shape::kTiles, STEP = Shape::kStep, STEPS = Shape::kSteps, PANELS = Shape::kPanels, PIECE_KEYS = Shape::kPieceKeys;
     constexpr uint32_t PER_TILE = Shape::kPerTile, kPiece = Shape::kPiece, SLOTS_K = Shape::kSlotsK, SLOTS_V = Shape::kSlotsV;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -200,13 +224,15 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
         }
         mbar_init(&bar.q_full, kWarpsK);
         mbar_init(&bar.q_free, 1);
-        for (uint32_t i = 0; i < 4; ++i) {
+        for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(&bar.s_full[i], 1);
-            mbar_init(&bar.p_full[i], kSoftmaxWarps / TILES);
-            mbar_init(&bar.pv_done[i], 1);
-        }
-        for (uint32_t i = 0; i < 2; ++i)
+            mbar_init(&bar.s_free[i], kSoftmaxWarps / TILES);
             mbar_init(&bar.o_free[i], kSoftmaxWarps / TILES);
+            for (uint32_t j = 0; j < 2; ++j) {
+                mbar_init(&bar.p_full[i][j], kSoftmaxWarps / TILES);
+                mbar_init(&bar.pv_done[i][j], 1);
+            }
+        }
         mbar_init(&bar.drain, 2);
         bar.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -222,7 +248,8 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
     tc_fence_after();
     const uint32_t tmem = bar.tmem;
     const auto o_col = [&](uint32_t q) { return tmem + q * D; };
-    const auto s_col = [&](uint32_t slot) { return tmem + 256 + slot * STEP; };
+    const auto s_col = [&](uint32_t q) { return tmem + 256 + q * STEP; };
+    const auto p_col = [&](uint32_t q, uint32_t step) { return tmem + 256 + TILES * STEP + (q * 2 + (step & 1)) * (STEP / 2); };
     chain_begin();
 
     const BlockRange range = find_range<Shape::kThreads>(p, reinterpret_cast<uint64_t*>(ring), blockIdx.x);
@@ -386,10 +413,10 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
         const auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
             return __all_sync(0xffffffffu, mbar_wait<true>(b, parity, &bar.abort, p.err, code)) != 0;
         };
-        // Scores of step u of the segment, into a buffer whose weights have been used. The last to use a piece of K lets go of it.
+        // Scores of step u of the segment, once the last ones have been read. The last to use a piece of K lets go of it.
         const auto scores = [&](uint32_t u, uint32_t q, bool last) {
-            const uint32_t slot = q * BUFFERS + done[q] % BUFFERS, d = columns + 256 + slot * STEP;
-            if (done[q] >= BUFFERS && !wait(&bar.pv_done[slot], (done[q] / BUFFERS - 1) & 1, ERR_PF_SUM_WAIT))
+            const uint32_t d = columns + 256 + q * STEP;
+            if (!wait(&bar.s_free[q], (done[q] & 1) ^ 1, ERR_PF_SUM_WAIT))
                 return false;
             tc_fence_after();
             const uint32_t part = u % STEPS; // of the key tile
@@ -409,7 +436,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     if (last && part + 1 == STEPS)
                         tc_commit(&bar.k_empty[s]);
                     if (i + 1 == PER_TILE)
-                        tc_commit(&bar.s_full[slot]);
+                        tc_commit(&bar.s_full[q]);
                 }
             }
             ++done[q];
@@ -418,8 +445,8 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
         // The step's keys are PER_TILE pieces of V (one step per key tile), or a part of one piece.
         static_assert(STEPS == 1 || PER_TILE == 1, "");
         const auto sums = [&](uint32_t u, uint32_t q, bool last) {
-            const uint32_t slot = q * BUFFERS + done[q] % BUFFERS, part = u % STEPS;
-            const uint32_t d = columns + q * D, a = columns + 256 + slot * STEP;
+            const uint32_t half = done[q] & 1, part = u % STEPS;
+            const uint32_t d = columns + q * D, a = columns + 256 + TILES * STEP + (q * 2 + half) * (STEP / 2);
             if (u == 0 && !wait(&bar.o_free[q], (segs[q] & 1) ^ 1, ERR_PF_SUM_WAIT))
                 return false;
 #pragma unroll
@@ -428,7 +455,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 if (part == 0 && q == 0 && !wait(&bar.v_full[s], (piece / SLOTS_V) & 1, ERR_PF_FULL_WAIT))
                     return false;
                 if (i == 0) {
-                    if (!wait(&bar.p_full[slot], (done[q] / BUFFERS) & 1, ERR_PF_WEIGHT_WAIT))
+                    if (!wait(&bar.p_full[q][half], (done[q] >> 1) & 1, ERR_PF_WEIGHT_WAIT))
                         return false;
                     tc_fence_after();
                 }
@@ -439,7 +466,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     for (uint32_t j = 0; j < COUNT; ++j)
                         mma_ts(d, a + (i * COUNT + j) * 8, kValue | (b_lo + j * (2048 >> 4)), kSums, u > 0 || i > 0 || j > 0);
                     if (i + 1 == PER_TILE)
-                        tc_commit(&bar.pv_done[slot]);
+                        tc_commit(&bar.pv_done[q][half]);
                     if (last && part + 1 == STEPS)
                         tc_commit(&bar.v_empty[s]);
                 }
@@ -482,19 +509,13 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
             tc_fence_after();
             return r;
         };
-        // The sums of step `d`: its buffer's scores were not overwritten before those of d - BUFFERS were through, so the
-        // barrier's parity stands for this step.
-        const auto wait_sums = [&](uint32_t d) {
-            return wait(&bar.pv_done[q * BUFFERS + d % BUFFERS], (d / BUFFERS) & 1, ERR_PF_SUM_WAIT);
-        };
+        // The sums of step `d`. Those of d - 2 are awaited before the weights of d are written, so the parity stands for this step.
+        const auto wait_sums = [&](uint32_t d) { return wait(&bar.pv_done[q][d & 1], (d >> 1) & 1, ERR_PF_SUM_WAIT); };
         // True in all threads of the rows that this warp has a part in, where `v` is in any.
         const auto any = [&](bool v) {
             if constexpr (TILES == 2)
                 return __any_sync(0xffffffffu, v) != 0;
-            tc_fence_before(); // (the other warp's weights take the place of scores that this one has read)
-            const bool r = !group_all(1 + (warp & 3), 64, !v);
-            tc_fence_after();
-            return r;
+            return !group_all(1 + (warp & 3), 64, !v);
         };
         while (ok && this_segment(p, at, left, &seg)) {
             const uint32_t steps = seg.count * STEPS;
@@ -509,21 +530,25 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 }
                 float m = -INFINITY, l = 0.0f;
                 for (uint32_t u = 0; u < steps; ++u, ++done) {
-                    const uint32_t slot = q * BUFFERS + done % BUFFERS;
-                    ok = wait(&bar.s_full[slot], (done / BUFFERS) & 1, ERR_PF_SCORE_WAIT);
-                    if constexpr (TILES == 1) // (the two warps of a row stop together)
-                        ok = group_all(1 + (warp & 3), 64, ok);
-                    if (!ok)
-                        break;
+                    ok = wait(&bar.s_full[q], done & 1, ERR_PF_SCORE_WAIT);
+                    uint32_t x[kMine];
                     if (!idle) {
-                        const uint32_t s_addr = s_col(slot) + lanes;
-                        const uint32_t key0 = seg.tile0 * kKeyTile + u * STEP + half * kMine;
-                        const bool part = __any_sync(0xffffffffu, lo > key0 || hi < key0 + kMine);
-                        uint32_t x[kMine];
-                        tc_ld32(s_addr + half * kMine, x);
-                        tc_ld32(s_addr + half * kMine + 32, x + 32);
+                        tc_ld32(s_col(q) + lanes + half * kMine, x);
+                        tc_ld32(s_col(q) + lanes + half * kMine + 32, x + 32);
                         tc_ld_wait32(x);
                         tc_ld_wait32(x + 32);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive(&bar.s_free[q]);
+                    if (done >= 2)
+                        ok = wait_sums(done - 2) && ok;
+                    if (idle && !ok)
+                        break;
+                    if (!idle) {
+                        const uint32_t key0 = seg.tile0 * kKeyTile + u * STEP + half * kMine;
+                        const bool part = __any_sync(0xffffffffu, lo > key0 || hi < key0 + kMine);
                         if (part) {
 #pragma unroll
                             for (uint32_t j = 0; j < kMine; ++j)
@@ -536,7 +561,11 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                             top1 = fmaxf(top1, fmaxf(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])));
                         }
                         float top = fmaxf(top0, top1) * p.scale_log2;
-                        if (any(top > m + kGrowth)) { // (m = -inf: whenever something is seen)
+                        if (any(!ok || top > m + kGrowth)) { // (m = -inf: whenever something is seen)
+                            if constexpr (TILES == 1) // the two warps of a row stop together
+                                ok = group_all(1 + (warp & 3), 64, ok);
+                            if (!ok)
+                                break;
                             if constexpr (TILES == 1) {
                                 bar.share[half][tile_row] = top;
                                 group_all(1 + (warp & 3), 64, true);
@@ -566,27 +595,27 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                             }
                         }
                         const float base = m == -INFINITY ? 0.0f : m;
-                        float sum0 = 0.0f, sum1 = 0.0f;
+                        const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), base2 = pack2(-base, -base);
+                        uint64_t sum2 = pack2(0.0f, 0.0f);
 #pragma unroll
                         for (uint32_t c = 0; c < kMine / 32; ++c) {
                             uint32_t w[16];
 #pragma unroll
                             for (uint32_t j = 0; j < 16; ++j) {
-                                const float a = exp2_approx(fmaf(__uint_as_float(x[c * 32 + 2 * j]), p.scale_log2, -base));
-                                const float b = exp2_approx(fmaf(__uint_as_float(x[c * 32 + 2 * j + 1]), p.scale_log2, -base));
-                                sum0 += a;
-                                sum1 += b;
+                                const uint64_t e = fma2(pack2(__uint_as_float(x[c * 32 + 2 * j]), __uint_as_float(x[c * 32 + 2 * j + 1])), scale2, base2);
+                                const float a = exp2_approx(low2(e)), b = exp2_approx(high2(e));
+                                sum2 = add2(sum2, pack2(a, b));
                                 w[j] = pack_bf16x2(a, b);
                             }
-                            tc_st16(s_addr + half * (kMine / 2) + c * 16, w);
+                            tc_st16(p_col(q, done) + lanes + half * (kMine / 2) + c * 16, w);
                         }
-                        l += sum0 + sum1;
+                        l += low2(sum2) + high2(sum2);
                         tc_st_wait();
                     }
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0)
-                        mbar_arrive(&bar.p_full[slot]);
+                        mbar_arrive(&bar.p_full[q][done & 1]);
                 }
                 ok = ok && wait_sums(done - 1);
                 if constexpr (TILES == 1) {
