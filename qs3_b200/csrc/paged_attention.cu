@@ -730,7 +730,7 @@ qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_des
     const auto reach = [&](const PagedPool& pool) {
         return static_cast<int64_t>(p.view.pages - 1) * pool.page_stride + static_cast<int64_t>(p.view.page_size - 1) * pool.slot_stride;
     };
-    const bool chunks = !fp8 && fresh * group > 16 && reach(p.view.k) < (int64_t { 1 } << 36) && reach(p.view.v) < (int64_t { 1 } << 36);
+    const bool chunks = fresh * group > 16 && reach(p.view.k) < (int64_t { 1 } << 36) && reach(p.view.v) < (int64_t { 1 } << 36);
     uint32_t item_rows;
     if (chunks) {
         item_rows = attn_prefill_rows(dim);
@@ -752,7 +752,7 @@ qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_des
     p.notes = reinterpret_cast<SplitNote*>(ws + at.notes);
     p.part_ml = reinterpret_cast<float2*>(ws + at.ml);
     p.part_o = reinterpret_cast<float*>(ws + at.o);
-    cudaError_t err = chunks ? launch_attn_prefill(p, ctx->stream) : launch_attn_stream(p, fp8, ctx->stream);
+    cudaError_t err = chunks ? launch_attn_prefill(p, fp8, ctx->stream) : launch_attn_stream(p, fp8, ctx->stream);
     if (err == cudaSuccess)
         err = launch_attn_join(p, ctx->stream);
     return set_cuda_error(ctx, err, "paged_attention");

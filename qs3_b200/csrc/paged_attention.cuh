@@ -250,7 +250,7 @@ __device__ __forceinline__ void next_segment(const AttnParams& p, const Segment&
 #endif
 
 cudaError_t launch_attn_stream(const AttnParams& p, bool fp8, cudaStream_t stream);
-cudaError_t launch_attn_prefill(const AttnParams& p, cudaStream_t stream);
+cudaError_t launch_attn_prefill(const AttnParams& p, bool fp8, cudaStream_t stream);
 cudaError_t launch_attn_join(const AttnParams& p, cudaStream_t stream);
 // Rows of an item of the streaming kernel: 8 or 16; blocks that fit the device at once.
 uint32_t attn_stream_rows(uint32_t rows_per_seq, uint32_t head_dim);

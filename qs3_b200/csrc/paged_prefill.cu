@@ -20,6 +20,12 @@
 // K's or V's ring: a slot's barriers then pass their phases in one order for all, which parities need. Pages that a box of TMA
 // divides come that way; other page sizes, the ends of sequences and windows row by row with cp.async, 16 bytes being the unit
 // in which every page size, stride and swizzled place works. Keys that no row sees are zeros then.
+//
+// e4m3 caches are multiplied in f16, which holds every code exactly: the fetching warps copy codes to a staging area of their own,
+// and from there, converted, to the ring. A row of queries is scaled by the power of two that brings its largest element to 2^13
+// or just above, so that f16 holds it to 2^-26 of that element, below the rounding of the f32 sums. K's scales are a factor on the
+// scores. V's are part of the weights, w = exp2(s + log2(scale) - m): the largest is again at a known place, and f16 keeps 11
+// bits of them where bf16 products would keep 8. The row's sum takes the scale out again.
 #include "paged_attention.cuh"
 #include "tcgen05.cuh"
 
@@ -36,10 +42,17 @@ constexpr uint32_t kRowTile = 128;
 constexpr uint32_t kKeyTile = 128;
 constexpr uint32_t kMine = 64;     // keys of a step that a thread has
 constexpr uint32_t kSoftmaxWarps = 8;
-constexpr uint32_t kWarpsK = 3, kWarpsV = 2, kLoadWarps = kWarpsK + kWarpsV;
+constexpr uint32_t kMostSlots = 6;
+constexpr uint32_t kScaleTiles = 4; // key tiles whose scales are held
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kNone = 0xffffffffu;
-constexpr float kGrowth = 8.0f; // of a row's maximum, in powers of two, before O is rescaled
+// Growth of a row's maximum, in powers of two, before O is rescaled, and where the largest weight lies at first: f16 weights end at
+// 2^16 and lose bits below 2^-14.
+template <bool FP8> constexpr float kGrowth = FP8 ? 7.0f : 8.0f;
+template <bool FP8> constexpr float kTop = FP8 ? 8.0f : 0.0f;
+// e4m3: 1 / scale of V, at most 1e30, times this, so that sums of a long row of zeros stay finite.
+template <bool FP8> constexpr float kSumUnit = FP8 ? 20.0f : 0.0f;
+template <bool FP8> constexpr float kSumFactor = FP8 ? 1.0f / 1048576.0f : 1.0f;
 
 enum : uint32_t {
     ERR_PF_EMPTY_WAIT = 0x5a000001u,
@@ -51,23 +64,30 @@ enum : uint32_t {
 };
 
 struct Barriers {
-    uint64_t k_full[6], k_empty[6], v_full[4], v_empty[4];
+    uint64_t k_full[kMostSlots], k_empty[kMostSlots], v_full[kMostSlots], v_empty[kMostSlots];
+    uint64_t scale_full[kScaleTiles];
     uint64_t q_full, q_free;
     uint64_t s_full[2], s_free[2], o_free[2]; // of a query tile
     uint64_t p_full[2][2], pv_done[2][2];     // of its tiles of weights
     uint64_t drain;
-    float share[2][kRowTile]; // between the two threads of a row
+    float share[2][kRowTile];       // between the two threads of a row
     uint32_t tmem;
     volatile uint32_t abort;
 };
 
-template <uint32_t D> struct PrefillShape {
+template <uint32_t D, bool FP8> struct PrefillShape {
     static constexpr uint32_t kTiles = D == 256 ? 1 : 2; // query tiles
     static constexpr uint32_t kStep = kTiles == 1 ? 128 : 64; // keys of a score tile
     static constexpr uint32_t kSteps = kKeyTile / kStep;      // of a key tile
     static constexpr uint32_t kRows = kTiles * kRowTile;
-    static constexpr uint32_t kPiece = D == 64 ? 16384 : 32768;
-    static constexpr uint32_t kSlotsK = D == 64 ? 6 : 3, kSlotsV = D == 64 ? 4 : 2; // of the rings
+    static constexpr uint32_t kPiece = D == 64 || FP8 ? 16384 : 32768;
+    static constexpr uint32_t kWarpsK = FP8 ? 2 : 3, kWarpsV = 2, kLoadWarps = kWarpsK + kWarpsV;
+    static constexpr uint32_t kSlotsK = FP8 ? 2 : D == 64 ? 6 : 3, kSlotsV = FP8 ? 2 : D == 64 ? 4 : 2; // of the rings
+    // e4m3: codes of two pieces for each fetching warp, K's and V's scales of a tile beside them
+    static constexpr uint32_t kCodes = kPiece / 2, kStage = kCodes + 2 * kKeyTile * 4;
+    static constexpr uint32_t kStaging = FP8 ? kLoadWarps * 2 * kStage : 0;
+    static constexpr uint32_t kScales = FP8 ? kScaleTiles * kKeyTile * 3 * 4 : 0;
+    static constexpr uint32_t kQueryScales = FP8 ? 2 * kRows * 4 : 0;
     static constexpr uint32_t kPanels = kPiece / (kKeyTile * 128);  // panels of 64 elements in a piece of K
     static constexpr uint32_t kPieceKeys = kPiece / (2 * D);        // keys of a piece of V
     static constexpr uint32_t kPerTile = kKeyTile / kPieceKeys;     // pieces of a tile of K, and of V
@@ -76,10 +96,11 @@ template <uint32_t D> struct PrefillShape {
     static constexpr uint32_t kScoreWarp = kSoftmaxWarps + kLoadWarps;
     static constexpr uint32_t kThreads = (kSoftmaxWarps + kLoadWarps + 2) * 32;
     static constexpr uint32_t kRing = (kSlotsK + kSlotsV) * kPiece;
-    static constexpr uint32_t kSmem = 1024 + kQ + kRing + sizeof(Barriers);
+    static constexpr uint32_t kSmem = 1024 + kQ + kRing + kStaging + kScales + kQueryScales + sizeof(Barriers);
     static_assert(kSlotsK % kWarpsK == 0 && kSlotsV % kWarpsV == 0, "a slot is one warp's");
     static_assert(kSmem <= 227 * 1024, "shared memory of a block");
     static_assert(kRing >= kMaxBatch * 8, "the search for the block's range uses the ring");
+    static_assert(kSlotsK <= kMostSlots && kSlotsV <= kMostSlots, "barriers of the slots");
     static_assert(kPanels * 64 * kPerTile == D, "a tile of K has as many pieces as one of V");
 };
 
@@ -133,6 +154,20 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r)
 
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+// Two codes in the low half of x.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t x)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(x)));
+    return r;
+}
+
 // Two floats in a register pair, one instruction for both.
 __device__ __forceinline__ uint64_t pack2(float a, float b)
 {
@@ -146,6 +181,12 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
 {
     uint64_t r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
@@ -199,29 +240,33 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* m
                  : "memory");
 }
 
-template <uint32_t D>
-__global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1)
+template <uint32_t D, bool FP8>
+__global__ void __launch_bounds__(PrefillShape<D, FP8>::kThreads, 1)
 attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap k_map,
                     const __grid_constant__ CUtensorMap v_map, const uint32_t k_box, const uint32_t v_box)
 {
-    using Shape = PrefillShape<D>;
+    using Shape = PrefillShape<D, FP8>;
+    constexpr uint32_t kWarpsK = Shape::kWarpsK, kWarpsV = Shape::kWarpsV;
     constexpr uint32_t TILES = Shape::kTiles, STEP = Shape::kStep, STEPS = Shape::kSteps, PANELS = Shape::kPanels, PIECE_KEYS = Shape::kPieceKeys;
     constexpr uint32_t PER_TILE = Shape::kPerTile, kPiece = Shape::kPiece, SLOTS_K = Shape::kSlotsK, SLOTS_V = Shape::kSlotsV;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* const ring = smem + Shape::kQ;
-    Barriers& bar = *reinterpret_cast<Barriers*>(ring + Shape::kRing);
+    uint8_t* const staging = ring + Shape::kRing;
+    float* const scales = reinterpret_cast<float*>(staging + Shape::kStaging); // of a tile's key pairs: K's, log2 of V's; then 1 / V's
+    float* const q_scales = scales + Shape::kScales / 4; // what the rows of queries were divided by, of this segment and the next
+    Barriers& bar = *reinterpret_cast<Barriers*>(staging + Shape::kStaging + Shape::kScales + Shape::kQueryScales);
     const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
 
     if (tid == 0) {
-        for (uint32_t i = 0; i < 6; ++i) {
+        for (uint32_t i = 0; i < kMostSlots; ++i) {
             mbar_init(&bar.k_full[i], 1);
             mbar_init(&bar.k_empty[i], 1);
-        }
-        for (uint32_t i = 0; i < 4; ++i) {
             mbar_init(&bar.v_full[i], 1);
             mbar_init(&bar.v_empty[i], 1);
         }
+        for (uint32_t i = 0; i < kScaleTiles; ++i)
+            mbar_init(&bar.scale_full[i], 1);
         mbar_init(&bar.q_full, kWarpsK);
         mbar_init(&bar.q_free, 1);
         for (uint32_t i = 0; i < 2; ++i) {
@@ -274,8 +319,61 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
         const auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
             if (__all_sync(0xffffffffu, mbar_test_wait(b, parity)))
                 return true;
-            copies.drain();
+            if constexpr (!FP8)
+                copies.drain();
             return __all_sync(0xffffffffu, mbar_wait(b, parity, &bar.abort, p.err, code)) != 0;
+        };
+        // e4m3: pieces that this warp has fetched so far, of all segments; the last one or two wait in its staging area. Its n-th
+        // is number n * warps + w of all. `newer`: another one has been fetched since.
+        uint32_t staged = 0, converted = 0;
+        const auto convert = [&](uint32_t n, bool newer) {
+            const uint32_t piece = n * warps + w, s = piece % slots;
+            if (!wait(&empty_bar[s], ((piece / slots) & 1) ^ 1, ERR_PF_EMPTY_WAIT))
+                return false;
+            if (newer)
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            else
+                asm volatile("cp.async.wait_all;" ::: "memory");
+            const uint8_t* const from = staging + ((warp - Shape::kLoadWarp) * 2 + (n & 1)) * Shape::kStage;
+            const uint32_t units = value ? D / 16 : 4, panel = value ? PIECE_KEYS * 128 : 0; // 16 codes each; bytes of a panel
+            uint8_t* const to = ring + (value ? SLOTS_K * kPiece : 0) + s * kPiece;
+#pragma unroll 4
+            for (uint32_t j = 0; j < Shape::kCodes / 512; ++j) {
+                const uint32_t i = j * 32 + lane, key = i / units, u = i % units;
+                const uint4 c = *reinterpret_cast<const uint4*>(from + i * 16); // (fetched by this lane)
+                const uint32_t x[4] = { c.x, c.y, c.z, c.w };
+                uint32_t y[8];
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k)
+                    y[k] = e4m3x2_to_f16x2(x[k / 2] >> (16 * (k & 1)));
+                uint8_t* const row = to + u / 4 * panel + key * 128;
+                const uint32_t first = u % 4 * 2;
+                *reinterpret_cast<uint4*>(row + ((first ^ (key & 7)) * 16)) = make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(row + (((first + 1) ^ (key & 7)) * 16)) = make_uint4(y[4], y[5], y[6], y[7]);
+            }
+            if (!value && piece % PER_TILE == 0) {
+                // These need no barrier for their way back: K of four tiles on is not fetched before the scores of two tiles on have
+                // been read.
+                const uint32_t tile = piece / PER_TILE % kScaleTiles;
+                const float* const raw = reinterpret_cast<const float*>(from + Shape::kCodes);
+                float* const out = scales + tile * (kKeyTile * 3);
+#pragma unroll
+                for (uint32_t j = 0; j < kKeyTile / 32; ++j) {
+                    const uint32_t key = j * 32 + lane;
+                    const float v = raw[kKeyTile + key];
+                    out[key / 2 * 4 + (key & 1)] = raw[key] * p.scale_log2;
+                    out[key / 2 * 4 + 2 + (key & 1)] = log2f(v < 1.0e-30f ? 1.0e-30f : v); // (a NaN stays one)
+                    out[kKeyTile * 2 + key] = kSumFactor<FP8> / (v < 1.0e-30f ? 1.0e-30f : v);
+                }
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&bar.scale_full[tile]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the tensor core reads what was written here
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(&full_bar[s]);
+            return true;
         };
         while (ok && this_segment(p, at, left, &seg)) {
             uint32_t seen_lo, seen_hi, unused;
@@ -286,23 +384,153 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
             const auto load_query = [&] {
                 if (!wait(&bar.q_free, (segments & 1) ^ 1, ERR_PF_QUERY_WAIT))
                     return false;
+                static_assert(Shape::kRows % 4 == 0, "four rows of a warp at a time");
 #pragma unroll 1
-                for (uint32_t r = w * 4 + lane / 8; r < Shape::kRows; r += kWarpsK * 4) {
-                    const uint32_t in_tile = r & (kRowTile - 1);
+                for (uint32_t r0 = w * 4; r0 < Shape::kRows; r0 += kWarpsK * 4) {
+                    const uint32_t r = r0 + lane / 8, in_tile = r & (kRowTile - 1);
                     const bool there = r < seg.nrows;
                     const uint32_t flat = seg.row0 + (there ? r : 0), token = p.tiling.group.div(flat);
                     const uint8_t* src = p.q + (seg.rows.row0 + token) * p.q_token
                         + (at.head * p.tiling.group.d + flat - token * p.tiling.group.d) * p.q_head + (lane & 7) * 16;
-                    const uint32_t dst = smem_u32(smem) + (r / kRowTile) * (kRowTile * D * 2) + in_tile * 128 + (((lane & 7) ^ (r & 7)) * 16);
+                    const uint32_t dst = (r / kRowTile) * (kRowTile * D * 2) + in_tile * 128 + (((lane & 7) ^ (r & 7)) * 16);
+                    if constexpr (!FP8) {
 #pragma unroll
-                    for (uint32_t panel = 0; panel < D / 64; ++panel)
-                        cp_async16z(dst + panel * (kRowTile * 128), src + panel * 128, there);
+                        for (uint32_t panel = 0; panel < D / 64; ++panel)
+                            cp_async16z(smem_u32(smem) + dst + panel * (kRowTile * 128), src + panel * 128, there);
+                    } else {
+                        uint4 v[D / 64];
+                        uint32_t most = 0; // of the magnitudes, which are in the order of their bits
+#pragma unroll
+                        for (uint32_t panel = 0; panel < D / 64; ++panel) {
+                            v[panel] = there ? *reinterpret_cast<const uint4*>(src + panel * 128) : make_uint4(0, 0, 0, 0);
+                            const uint32_t a[4] = { v[panel].x, v[panel].y, v[panel].z, v[panel].w };
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; ++j)
+                                most = max(most, max(a[j] & 0x7fffu, a[j] >> 16 & 0x7fffu));
+                        }
+#pragma unroll
+                        for (uint32_t o = 1; o < 8; o <<= 1)
+                            most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                        // the power of two and its reciprocal are both f32's; an infinity or NaN stays one
+                        const int power = most >= 0x7f80u ? 0 : max(-126, min(126, 127 + 13 - static_cast<int>(most >> 7)));
+                        const float up = __uint_as_float(static_cast<uint32_t>(127 + power) << 23);
+                        if ((lane & 7) == 0)
+                            q_scales[(segments & 1) * Shape::kRows + r] = __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
+#pragma unroll
+                        for (uint32_t panel = 0; panel < D / 64; ++panel) {
+                            uint32_t a[4] = { v[panel].x, v[panel].y, v[panel].z, v[panel].w };
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; ++j)
+                                a[j] = pack_f16x2(bf16_bits_to_f32(a[j] & 0xffffu) * up, bf16_bits_to_f32(a[j] >> 16) * up);
+                            *reinterpret_cast<uint4*>(smem + dst + panel * (kRowTile * 128)) = make_uint4(a[0], a[1], a[2], a[3]);
+                        }
+                    }
                 }
-                __syncwarp();
-                copies.push(&bar.q_full);
+                if constexpr (FP8) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive(&bar.q_full);
+                } else {
+                    __syncwarp();
+                    copies.push(&bar.q_full);
+                }
                 return true;
             };
 
+            const uint32_t pieces = seg.count * PER_TILE;
+            uint32_t mine = (w + warps - before % warps) % warps; // the first that goes to one of this warp's slots
+            bool query = value; // loaded, or not this warp's business
+            if constexpr (FP8) {
+                struct Places { // of keys lane + 32 j of a piece
+                    int32_t page[kKeyTile / 32];
+                    uint32_t slot[kKeyTile / 32];
+                };
+                const auto key_of = [&](uint32_t piece, uint32_t j) {
+                    return seg.tile0 * kKeyTile + (value ? piece * PIECE_KEYS : piece / PER_TILE * kKeyTile) + j * 32 + lane;
+                };
+                const auto look = [&](uint32_t piece) {
+                    Places l;
+#pragma unroll
+                    for (uint32_t j = 0; j < kKeyTile / 32; ++j) {
+                        const uint32_t key = key_of(piece, j);
+                        l.page[j] = -1;
+                        l.slot[j] = 0;
+                        if (j < (value ? PIECE_KEYS : kKeyTile) / 32 && key >= seen_lo && key < seen_hi) {
+                            const uint32_t i = p.view.page_div.div(key);
+                            l.slot[j] = key - i * p.view.page_size;
+                            l.page[j] = __ldg(p.view.indices + seg.pages.first + i);
+                        }
+                    }
+                    return l;
+                };
+                const auto fetch = [&](uint32_t piece, Places l, auto keys, auto units, uint32_t skip) {
+                    constexpr uint32_t KEYS = decltype(keys)::value, UNITS = decltype(units)::value, AT_ONCE = 32 / UNITS;
+                    const PagedPool& pool = value ? p.view.v : p.view.k;
+                    uint32_t row[KEYS / 32]; // in units of 16 bytes; none: zeros
+#pragma unroll
+                    for (uint32_t j = 0; j < KEYS / 32; ++j) {
+                        const uint32_t key = key_of(piece, j);
+                        if (static_cast<uint32_t>(l.page[j]) >= p.view.pages) {
+                            if (key >= seen_lo && key < seen_hi)
+                                atomicCAS(p.err, 0u, static_cast<uint32_t>(ERR_PAGE_TABLE));
+                            l.page[j] = -1;
+                        }
+                        row[j] = l.page[j] < 0 ? kNone : static_cast<uint32_t>((l.page[j] * pool.page_stride + l.slot[j] * pool.slot_stride) >> 4);
+                    }
+                    const uint8_t* const from = pool.data + at.head * pool.head_stride + skip + (lane % UNITS) * 16;
+                    const uint32_t to = smem_u32(staging) + ((warp - Shape::kLoadWarp) * 2 + (staged & 1)) * Shape::kStage;
+                    __syncwarp();
+#pragma unroll
+                    for (uint32_t j = 0; j < KEYS / AT_ONCE; ++j) {
+                        const uint32_t r = __shfl_sync(0xffffffffu, row[j * AT_ONCE / 32], (j * AT_ONCE + lane / UNITS) & 31);
+                        cp_async16z(to + (j * 32 + lane) * 16, from + static_cast<uint64_t>(r == kNone ? 0 : r) * 16, r != kNone);
+                    }
+                    if (!value && piece % PER_TILE == 0) // the tile's scales, of K and V
+#pragma unroll
+                        for (uint32_t j = 0; j < KEYS / 32; ++j)
+#pragma unroll
+                            for (uint32_t v = 0; v < 2; ++v) {
+                                const PagedPool& of = v ? p.view.v : p.view.k;
+                                const bool there = l.page[j] >= 0;
+                                const float* from_scale = of.scale + at.head * of.scale_head_stride
+                                    + (there ? l.page[j] * of.scale_page_stride + l.slot[j] * of.scale_slot_stride : 0);
+                                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
+                                                 to + Shape::kCodes + (v * kKeyTile + j * 32 + lane) * 4),
+                                             "l"(from_scale), "r"(there ? 4u : 0u)
+                                             : "memory");
+                            }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                };
+                Places ahead;
+                if (mine < pieces)
+                    ahead = look(mine);
+                for (; ok && mine < pieces; mine += warps) { // a piece's codes are fetched while the one before is converted
+                    const Places l = ahead;
+                    if (mine + warps < pieces)
+                        ahead = look(mine + warps);
+                    if (value)
+                        fetch(mine, l, std::integral_constant<uint32_t, PIECE_KEYS> {}, std::integral_constant<uint32_t, D / 16> {}, 0);
+                    else
+                        fetch(mine, l, std::integral_constant<uint32_t, kKeyTile> {}, std::integral_constant<uint32_t, 4> {}, mine % PER_TILE * 64);
+                    ++staged;
+                    if (staged - converted > 1)
+                        ok = convert(converted++, true);
+                    if (ok && !query) { // behind the first piece, which may find room before the queries do
+                        ok = load_query();
+                        query = true;
+                    }
+                }
+                if (ok && !query) { // no piece here: one that is still staged belongs to scores that the queries wait for
+                    if (converted < staged)
+                        ok = convert(converted++, false);
+                    ok = ok && load_query();
+                }
+                before += pieces;
+                ++segments;
+                next_segment(p, seg, &at, &left);
+                continue;
+            }
             // A warp looks up the pages of its next piece before it waits for room.
             struct Ahead {
                 uint32_t key0, slot; // slot, page: of this lane's box
@@ -370,9 +598,6 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 copies.push(&full_bar[s]);
                 return true;
             };
-            const uint32_t pieces = seg.count * PER_TILE;
-            uint32_t mine = (w + warps - before % warps) % warps; // the first that goes to one of this warp's slots
-            bool query = value; // loaded, or not this warp's business
             Ahead ahead;
             if (mine < pieces)
                 ahead = look(mine);
@@ -395,11 +620,13 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
             ++segments;
             next_segment(p, seg, &at, &left);
         }
+        if (FP8 && ok && converted < staged)
+            convert(converted, false);
         copies.drain();
     } else if (warp >= Shape::kScoreWarp) {
         // ------------------------------------------------------------------------------- products --
         // The whole warp goes through the loops and one lane issues.
-        constexpr uint32_t kFormat = (1u << 4) | (1u << 7) | (1u << 10) | ((kRowTile >> 4) << 24); // bf16 x bf16 -> f32
+        constexpr uint32_t kFormat = (1u << 4) | (FP8 ? 0u : (1u << 7) | (1u << 10)) | ((kRowTile >> 4) << 24); // f16 or bf16 -> f32
         constexpr uint32_t kScores = kFormat | ((STEP >> 3) << 17);
         constexpr uint32_t kSums = kFormat | ((D >> 3) << 17) | (1u << 16);
         constexpr uint64_t kOperand = (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
@@ -442,32 +669,33 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
             ++done[q];
             return true;
         };
-        // The step's keys are PER_TILE pieces of V (one step per key tile), or a part of one piece.
-        static_assert(STEPS == 1 || PER_TILE == 1, "");
+        // A step's keys are one or more pieces of V, or a part of one.
+        constexpr bool WHOLE = PER_TILE >= STEPS;
+        constexpr uint32_t OF_STEP = WHOLE ? PER_TILE / STEPS : 1;
         const auto sums = [&](uint32_t u, uint32_t q, bool last) {
             const uint32_t half = done[q] & 1, part = u % STEPS;
             const uint32_t d = columns + q * D, a = columns + 256 + TILES * STEP + (q * 2 + half) * (STEP / 2);
             if (u == 0 && !wait(&bar.o_free[q], (segs[q] & 1) ^ 1, ERR_PF_SUM_WAIT))
                 return false;
 #pragma unroll
-            for (uint32_t i = 0; i < PER_TILE; ++i) {
-                const uint32_t piece = before + u / STEPS * PER_TILE + i, s = piece % SLOTS_V;
-                if (part == 0 && q == 0 && !wait(&bar.v_full[s], (piece / SLOTS_V) & 1, ERR_PF_FULL_WAIT))
+            for (uint32_t i = 0; i < OF_STEP; ++i) {
+                const uint32_t piece = before + (WHOLE ? u * OF_STEP + i : u / STEPS), s = piece % SLOTS_V;
+                if ((WHOLE || part == 0) && q == 0 && !wait(&bar.v_full[s], (piece / SLOTS_V) & 1, ERR_PF_FULL_WAIT))
                     return false;
                 if (i == 0) {
                     if (!wait(&bar.p_full[q][half], (done[q] >> 1) & 1, ERR_PF_WEIGHT_WAIT))
                         return false;
                     tc_fence_after();
                 }
-                const uint32_t b_lo = uniform(ring_lo + (SLOTS_K + s) * (kPiece / 16) + part * (STEP * 128 / 16));
-                constexpr uint32_t COUNT = STEP / PER_TILE / 16; // products of 16 keys: 2048 bytes of V, eight columns of P
+                const uint32_t b_lo = uniform(ring_lo + (SLOTS_K + s) * (kPiece / 16) + (WHOLE ? 0 : part * (STEP * 128 / 16)));
+                constexpr uint32_t COUNT = STEP / OF_STEP / 16; // products of 16 keys: 2048 bytes of V, eight columns of P
                 if (elect_one()) {
 #pragma unroll
                     for (uint32_t j = 0; j < COUNT; ++j)
                         mma_ts(d, a + (i * COUNT + j) * 8, kValue | (b_lo + j * (2048 >> 4)), kSums, u > 0 || i > 0 || j > 0);
-                    if (i + 1 == PER_TILE)
+                    if (i + 1 == OF_STEP)
                         tc_commit(&bar.pv_done[q][half]);
-                    if (last && part + 1 == STEPS)
+                    if (last && (WHOLE || part + 1 == STEPS))
                         tc_commit(&bar.v_empty[s]);
                 }
             }
@@ -502,7 +730,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
         // -------------------------------------------------------------------------------- weights --
         const uint32_t q = TILES == 1 ? 0 : warp / 4, half = TILES == 1 ? warp / 4 : 0;
         const uint32_t lanes = (warp & 3) << 21, tile_row = (warp & 3) * 32 + lane; // 32 lanes of tensor memory
-        uint32_t done = 0;                                                          // steps
+        uint32_t done = 0, segments = 0, tiles_before_this = 0;                     // steps; key tiles of earlier segments
         bool ok = true;
         const auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
             const bool r = __all_sync(0xffffffffu, mbar_wait(b, parity, &bar.abort, p.err, code)) != 0;
@@ -528,7 +756,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     visible_keys(p.tiling, seg.rows.fresh, seg.pages.length, token, &lo, &hi);
                     hi = min(hi, seg.pages.length);
                 }
-                float m = -INFINITY, l = 0.0f;
+                float m = -INFINITY, l = 0.0f, q_scale = 1.0f;
                 for (uint32_t u = 0; u < steps; ++u, ++done) {
                     ok = wait(&bar.s_full[q], done & 1, ERR_PF_SCORE_WAIT);
                     uint32_t x[kMine];
@@ -544,10 +772,30 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                         mbar_arrive(&bar.s_free[q]);
                     if (done >= 2)
                         ok = wait_sums(done - 2) && ok;
+                    const uint32_t in_tile = u % STEPS * STEP + half * kMine; // this thread's first key
+                    const float* scale = nullptr;
+                    if constexpr (FP8) {
+                        const uint32_t tile = tiles_before_this + u / STEPS;
+                        ok = wait(&bar.scale_full[tile % kScaleTiles], (tile / kScaleTiles) & 1, ERR_PF_SCORE_WAIT) && ok;
+                        scale = scales + tile % kScaleTiles * (kKeyTile * 3);
+                        if (u == 0)
+                            q_scale = q_scales[(segments & 1) * Shape::kRows + r];
+                    }
                     if (idle && !ok)
                         break;
                     if (!idle) {
-                        const uint32_t key0 = seg.tile0 * kKeyTile + u * STEP + half * kMine;
+                        const uint32_t key0 = (seg.tile0 + u / STEPS) * kKeyTile + in_tile;
+                        if constexpr (FP8) {
+                            const uint64_t q2 = pack2(q_scale, q_scale);
+#pragma unroll
+                            for (uint32_t j = 0; j < kMine / 2; ++j) {
+                                const float4 kv = *reinterpret_cast<const float4*>(scale + (in_tile / 2 + j) * 4);
+                                const uint64_t e = fma2(mul2(pack2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), q2),
+                                                        pack2(kv.x, kv.y), pack2(kv.z, kv.w));
+                                x[2 * j] = static_cast<uint32_t>(e);
+                                x[2 * j + 1] = static_cast<uint32_t>(e >> 32);
+                            }
+                        }
                         const bool part = __any_sync(0xffffffffu, lo > key0 || hi < key0 + kMine);
                         if (part) {
 #pragma unroll
@@ -560,8 +808,8 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                             top0 = fmaxf(top0, fmaxf(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
                             top1 = fmaxf(top1, fmaxf(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])));
                         }
-                        float top = fmaxf(top0, top1) * p.scale_log2;
-                        if (any(!ok || top > m + kGrowth)) { // (m = -inf: whenever something is seen)
+                        float top = FP8 ? fmaxf(top0, top1) : fmaxf(top0, top1) * p.scale_log2;
+                        if (any(!ok || top > m + kGrowth<FP8>)) { // (m = -inf: whenever something is seen)
                             if constexpr (TILES == 1) // the two warps of a row stop together
                                 ok = group_all(1 + (warp & 3), 64, ok);
                             if (!ok)
@@ -571,7 +819,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                                 group_all(1 + (warp & 3), 64, true);
                                 top = fmaxf(top, bar.share[half ^ 1][tile_row]);
                             }
-                            const bool grow = top > m + kGrowth;
+                            const bool grow = top > m + kGrowth<FP8>;
                             const float next = grow ? top : m;
                             const float keep = grow ? exp2_approx(m - next) : 1.0f;
                             m = next;
@@ -594,7 +842,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                                 }
                             }
                         }
-                        const float base = m == -INFINITY ? 0.0f : m;
+                        const float base = m == -INFINITY ? 0.0f : m - kTop<FP8>;
                         const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), base2 = pack2(-base, -base);
                         uint64_t sum2 = pack2(0.0f, 0.0f);
 #pragma unroll
@@ -602,10 +850,18 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                             uint32_t w[16];
 #pragma unroll
                             for (uint32_t j = 0; j < 16; ++j) {
-                                const uint64_t e = fma2(pack2(__uint_as_float(x[c * 32 + 2 * j]), __uint_as_float(x[c * 32 + 2 * j + 1])), scale2, base2);
+                                const uint32_t i = c * 32 + 2 * j;
+                                const uint64_t x2 = pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                                const uint64_t e = FP8 ? add2(x2, base2) : fma2(x2, scale2, base2);
                                 const float a = exp2_approx(low2(e)), b = exp2_approx(high2(e));
-                                sum2 = add2(sum2, pack2(a, b));
-                                w[j] = pack_bf16x2(a, b);
+                                if constexpr (FP8) {
+                                    const float2 inv = *reinterpret_cast<const float2*>(scale + kKeyTile * 2 + in_tile + i);
+                                    sum2 = fma2(pack2(a, b), pack2(inv.x, inv.y), sum2);
+                                    w[j] = pack_f16x2(a, b);
+                                } else {
+                                    sum2 = add2(sum2, pack2(a, b));
+                                    w[j] = pack_bf16x2(a, b);
+                                }
                             }
                             tc_st16(p_col(q, done) + lanes + half * (kMine / 2) + c * 16, w);
                         }
@@ -627,11 +883,14 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 if (!ok)
                     break;
                 const bool whole = seg.whole;
+                // in units of the sums: O counts 2^kSumUnit times too much
+                if (m != -INFINITY)
+                    m += kSumUnit<FP8> - kTop<FP8>;
                 const uint32_t h = at.head * p.tiling.group.d + flat - token * p.tiling.group.d;
                 const size_t part_row = static_cast<size_t>(blockIdx.x * 2 + (seg.starts ? 1 : 0)) * Shape::kRows + r;
                 uint8_t* const out = p.out + (seg.rows.row0 + token) * p.out_token + h * p.out_head;
                 float* const part_o = p.part_o + part_row * D;
-                const float inv = whole ? (m == -INFINITY ? 0.0f : 1.0f / l) : 1.0f;
+                const float inv = whole ? (m == -INFINITY ? 0.0f : kSumFactor<FP8> / l) : kSumFactor<FP8>;
                 uint32_t x[32];
 #pragma unroll 1
                 for (uint32_t i = 0; i < D / 32 / (TILES == 1 ? 2 : 1); ++i) {
@@ -652,7 +911,9 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     } else {
 #pragma unroll
                         for (uint32_t j = 0; j < 8; ++j)
-                            *reinterpret_cast<uint4*>(part_o + c * 32 + j * 4) = make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+                            *reinterpret_cast<float4*>(part_o + c * 32 + j * 4)
+                                = make_float4(__uint_as_float(x[4 * j]) * inv, __uint_as_float(x[4 * j + 1]) * inv,
+                                              __uint_as_float(x[4 * j + 2]) * inv, __uint_as_float(x[4 * j + 3]) * inv);
                     }
                 }
                 tc_fence_before();
@@ -665,6 +926,8 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 if (live && !whole && half == 0)
                     p.part_ml[part_row] = make_float2(m, l);
             }
+            tiles_before_this += seg.count;
+            ++segments;
             next_segment(p, seg, &at, &left);
         }
     }
@@ -674,10 +937,10 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
 }
 
-template <uint32_t D> cudaError_t launch_prefill_as(const AttnParams& p, cudaStream_t stream)
+template <uint32_t D, bool FP8> cudaError_t launch_prefill_as(const AttnParams& p, cudaStream_t stream)
 {
-    using Shape = PrefillShape<D>;
-    const cudaError_t err = cudaFuncSetAttribute(attn_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
+    using Shape = PrefillShape<D, FP8>;
+    const cudaError_t err = cudaFuncSetAttribute(attn_prefill_kernel<D, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
     if (err != cudaSuccess)
         return err;
     // Pages that a box fits into a whole number of times are fetched by TMA, others and the ends of sequences row by row.
@@ -687,23 +950,29 @@ template <uint32_t D> cudaError_t launch_prefill_as(const AttnParams& p, cudaStr
         const uint64_t dims[4] = { D, size, p.view.kv_heads, p.view.pages };
         const uint64_t strides[3] = { static_cast<uint64_t>(pool.slot_stride), static_cast<uint64_t>(pool.head_stride),
                                       static_cast<uint64_t>(pool.page_stride) };
-        if (rows < 8 || size % rows != 0 || most % rows != 0 || !make_page_map(map, pool.data, dims, strides, rows))
+        if (FP8 || rows < 8 || size % rows != 0 || most % rows != 0 || !make_page_map(map, pool.data, dims, strides, rows))
             return 0u;
         return rows;
     };
     CUtensorMap k_map {}, v_map {};
     const uint32_t k_box = box(&k_map, p.view.k, kKeyTile), v_box = box(&v_map, p.view.v, Shape::kPieceKeys);
-    return launch_chained(attn_prefill_kernel<D>, dim3(p.blocks), Shape::kThreads, Shape::kSmem, stream, p, k_map, v_map, k_box, v_box);
+    return launch_chained(attn_prefill_kernel<D, FP8>, dim3(p.blocks), Shape::kThreads, Shape::kSmem, stream, p, k_map, v_map, k_box, v_box);
 }
 
 } // namespace
 
 uint32_t attn_prefill_rows(uint32_t head_dim) { return head_dim == 256 ? kRowTile : 2 * kRowTile; }
 
-cudaError_t launch_attn_prefill(const AttnParams& p, cudaStream_t stream)
+cudaError_t launch_attn_prefill(const AttnParams& p, bool fp8, cudaStream_t stream)
 {
     const uint32_t d = p.view.head_dim;
-    return d == 64 ? launch_prefill_as<64>(p, stream) : d == 128 ? launch_prefill_as<128>(p, stream) : launch_prefill_as<256>(p, stream);
+    if (fp8)
+        return d == 64 ? launch_prefill_as<64, true>(p, stream)
+            : d == 128 ? launch_prefill_as<128, true>(p, stream)
+                       : launch_prefill_as<256, true>(p, stream);
+    return d == 64 ? launch_prefill_as<64, false>(p, stream)
+        : d == 128 ? launch_prefill_as<128, false>(p, stream)
+                   : launch_prefill_as<256, false>(p, stream);
 }
 
 } // namespace qs3
