@@ -959,8 +959,7 @@ qsfi_status qs3_rope(qsfi_context* ctx, const qs3_rope_desc* desc);
 
 /* A pool of pages. bf16, or e4m3 codes with one f32 scale per token and KV head:
  *   scale = max(amax / 448, 1e-30),  code = e4m3_rn_sat(x * (1 / scale)).
- * A row with an infinity or a NaN reads back as NaNs. Codes 0x7f and 0xff, which no append writes beside a finite scale, count
- * as +-480 in attention. */
+ * A row with an infinity or a NaN reads back as NaNs. Scales are positive; V's below 1e-30 count as 1e-30 in attention. */
 typedef struct {
     qsfi_tensor4 k, v;             /* bf16 or e4m3 [pages, kv_heads, page_size, head_dim] */
     qsfi_tensor3 k_scale, v_scale; /* e4m3: f32 [pages, kv_heads, page_size] */

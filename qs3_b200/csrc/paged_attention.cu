@@ -8,7 +8,11 @@
 // through its own ring in shared memory (cp.async, three stages), and the only barriers are those at an item's ends. The
 // products run on the tensor cores with the keys on the M side and the rows (at most 16: query heads that share the KV head,
 // times new tokens) on the N side of m16n8k16: S^T = K Q^T, then O^T += V^T P^T, so that no row of a tile is padding when eight
-// heads share a KV head, and the running maximum of a row sits in the lane that rescales it. 
+// heads share a KV head, and the running maximum of a row sits in the lane that rescales it.
+//
+// e4m3 caches are multiplied in f16 as in paged_prefill.cu: queries scaled by powers of two, K's scales a factor on the scores, V's
+// scales part of the weights. (With codes moved to bf16 by integer instructions, five for two codes instead of one conversion,
+// the kernel waited for those: 66 sequences of up to 16 384 tokens 335 us.)
 #include "paged_attention.cuh"
 #include "tcgen05.cuh"
 
@@ -47,12 +51,18 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v)
     return r;
 }
 
-__device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1)
+template <bool F16> __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    if constexpr (F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // 16 bytes to shared memory, zeros where `there` is 0.
@@ -77,15 +87,25 @@ __device__ __forceinline__ float exp2_fast(float x)
     return r;
 }
 
-// Two e4m3 codes, in the upper bytes of the halves of x, as bf16: the code's seven bits are an exponent and mantissa with a
-// bias of 7, moved to a bf16's place they read 2^120 times too small, subnormals included. NaN (0x7f) becomes 480.
-__device__ __forceinline__ uint32_t e4m3x2_to_bf16x2(uint32_t x)
+// Two codes in the low half of x.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t x)
 {
-    const uint32_t bits = (x & 0x80008000u) | (x >> 4 & 0x07f007f0u);
     uint32_t r;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(bits), "r"(0x7b807b80u));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(x)));
     return r;
 }
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+
+// e4m3: where the largest weight lies, in powers of two (f16 ends at 2^16 and loses bits below 2^-14), and a factor on 1 / scale
+// of V, at most 1e30, so that sums of a long row of zeros stay finite.
+template <bool FP8> constexpr float kTop = FP8 ? 14.0f : 0.0f;
+template <bool FP8> constexpr float kSumUnit = FP8 ? 20.0f : 0.0f;
+template <bool FP8> constexpr float kSumFactor = FP8 ? 1.0f / 1048576.0f : 1.0f;
 
 template <uint32_t D, uint32_t NT, bool FP8> struct StreamShape {
     static constexpr uint32_t kRows = 8 * NT;
@@ -100,7 +120,7 @@ template <uint32_t D, uint32_t NT, bool FP8> struct StreamShape {
     static constexpr uint32_t kCosts = kMaxBatch * 8;
     static constexpr uint32_t kLarger = kRing > kSums ? kRing : kSums;
     static constexpr uint32_t kUnion = kLarger > kCosts ? kLarger : kCosts;
-    static constexpr uint32_t kSmem = kUnion + kQ + kStreamWarps * kRows * 8;
+    static constexpr uint32_t kSmem = kUnion + kQ + kStreamWarps * kRows * 8 + (FP8 ? kRows * 4 : 0);
     static constexpr uint32_t kBlocks = 227 * 1024 / (kSmem + 1024); // per SM
 };
 
@@ -120,6 +140,7 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* const s_q = smem + Shape::kUnion;
     float2* const s_ml = reinterpret_cast<float2*>(s_q + Shape::kQ); // [warps][rows]
+    float* const s_q_scale = reinterpret_cast<float*>(s_ml + kStreamWarps * ROWS); // e4m3: what a row was divided by
     chain_begin();
 
     const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
@@ -146,6 +167,24 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
                 const uint32_t token = p.tiling.group.div(row0 + r), h = at.head * p.tiling.group.d + row0 + r - token * p.tiling.group.d;
                 w = *reinterpret_cast<const uint4*>(p.q + (rows.row0 + token) * p.q_token + h * p.q_head + c * 16);
             }
+            if constexpr (FP8) { // to f16, the row's largest element brought to 2^13 or just above; an infinity or NaN stays one
+                static_assert(ROWS * D / 8 % 32 == 0, "whole warps");
+                uint32_t a[4] = { w.x, w.y, w.z, w.w }, most = 0; // of the magnitudes, which are in the order of their bits
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j)
+                    most = max(most, max(a[j] & 0x7fffu, a[j] >> 16 & 0x7fffu));
+#pragma unroll
+                for (uint32_t o = 1; o < D / 8; o <<= 1)
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const int power = most >= 0x7f80u ? 0 : max(-126, min(126, 127 + 13 - static_cast<int>(most >> 7)));
+                const float up = __uint_as_float(static_cast<uint32_t>(127 + power) << 23);
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j)
+                    a[j] = pack_f16x2(bf16_bits_to_f32(a[j] & 0xffffu) * up, bf16_bits_to_f32(a[j] >> 16) * up);
+                w = make_uint4(a[0], a[1], a[2], a[3]);
+                if (c == 0)
+                    s_q_scale[r] = __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
+            }
             *reinterpret_cast<uint4*>(s_q + swizzled<D * 2>(r, c)) = w;
         }
         __syncthreads();
@@ -168,6 +207,14 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
                     hi[n][j] = min(hi[n][j], pages.length);
                 }
             }
+
+        float q_scale[NT][2];
+        if constexpr (FP8)
+#pragma unroll
+            for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+                for (uint32_t j = 0; j < 2; ++j)
+                    q_scale[n][j] = s_q_scale[n * 8 + (lane & 3) * 2 + j];
 
         // B fragments of the queries: for 8-bit keys the four consecutive elements that a lane converts from one word
         uint32_t qf[NT == 1 ? D / 16 : 1][2];
@@ -264,7 +311,7 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
                             b[0] = qf[ks][0], b[1] = qf[ks][1];
                         else
                             q_frag(n, ks, b);
-                        mma16816(s[n][ks & 1], a, b[0], b[1]);
+                        mma16816<FP8>(s[n][ks & 1], a, b[0], b[1]);
                     }
                 }
             } else {
@@ -275,10 +322,8 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
 #pragma unroll
                     for (uint32_t u = 0; u < 2; ++u) {
                         const uint32_t ks = kb * 2 + u;
-                        const uint32_t a[4] = { e4m3x2_to_bf16x2(__byte_perm(w[2 * u], 0, 0x1404)),
-                                                e4m3x2_to_bf16x2(__byte_perm(w[2 * u + 1], 0, 0x1404)),
-                                                e4m3x2_to_bf16x2(__byte_perm(w[2 * u], 0, 0x3424)),
-                                                e4m3x2_to_bf16x2(__byte_perm(w[2 * u + 1], 0, 0x3424)) };
+                        const uint32_t a[4] = { e4m3x2_to_f16x2(w[2 * u]), e4m3x2_to_f16x2(w[2 * u + 1]),
+                                                e4m3x2_to_f16x2(w[2 * u] >> 16), e4m3x2_to_f16x2(w[2 * u + 1] >> 16) };
 #pragma unroll
                         for (uint32_t n = 0; n < NT; ++n) {
                             uint32_t b[2];
@@ -286,18 +331,22 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
                                 b[0] = qf[ks][0], b[1] = qf[ks][1];
                             else
                                 q_frag(n, ks, b);
-                            mma16816(s[n][u], a, b[0], b[1]);
+                            mma16816<FP8>(s[n][u], a, b[0], b[1]);
                         }
                     }
                 }
             }
-            float ks0 = p.scale_log2, ks1 = p.scale_log2, vs0 = 1.0f, vs1 = 1.0f;
+            // factor on the scores, what is added to them, and the factor on the weights in the row's sum, of a lane's two keys
+            float ks0 = p.scale_log2, ks1 = p.scale_log2, lv0 = 0.0f, lv1 = 0.0f, unit0 = 1.0f, unit1 = 1.0f;
             if constexpr (FP8) {
                 const float* sc = reinterpret_cast<const float*>(ring + (i % kStreamStages) * Shape::kStage + 2 * Shape::kHalf);
                 ks0 *= sc[lane / 4];
                 ks1 *= sc[lane / 4 + 8];
-                vs0 = sc[16 + lane / 4];
-                vs1 = sc[16 + lane / 4 + 8];
+                const float v0 = sc[16 + lane / 4], v1 = sc[16 + lane / 4 + 8];
+                lv0 = __log2f(v0 < 1.0e-30f ? 1.0e-30f : v0); // (a NaN stays one)
+                lv1 = __log2f(v1 < 1.0e-30f ? 1.0e-30f : v1);
+                unit0 = kSumFactor<FP8> / (v0 < 1.0e-30f ? 1.0e-30f : v0);
+                unit1 = kSumFactor<FP8> / (v1 < 1.0e-30f ? 1.0e-30f : v1);
             }
 
             // P^T, a lane's keys lane / 4 and lane / 4 + 8 and rows 2 (lane % 4) and the next
@@ -305,8 +354,15 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
             const uint32_t ka = key0 + lane / 4, kb = ka + 8;
 #pragma unroll
             for (uint32_t n = 0; n < NT; ++n) {
-                float v[4] = { (s[n][0][0] + s[n][1][0]) * ks0, (s[n][0][1] + s[n][1][1]) * ks0,
-                               (s[n][0][2] + s[n][1][2]) * ks1, (s[n][0][3] + s[n][1][3]) * ks1 };
+                float v[4] = { s[n][0][0] + s[n][1][0], s[n][0][1] + s[n][1][1], s[n][0][2] + s[n][1][2], s[n][0][3] + s[n][1][3] };
+                if constexpr (FP8) {
+                    v[0] = fmaf(v[0] * q_scale[n][0], ks0, lv0);
+                    v[1] = fmaf(v[1] * q_scale[n][1], ks0, lv0);
+                    v[2] = fmaf(v[2] * q_scale[n][0], ks1, lv1);
+                    v[3] = fmaf(v[3] * q_scale[n][1], ks1, lv1);
+                } else {
+                    v[0] *= ks0, v[1] *= ks0, v[2] *= ks1, v[3] *= ks1;
+                }
                 float w[4];
 #pragma unroll
                 for (uint32_t j = 0; j < 2; ++j) {
@@ -320,9 +376,9 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
                     const float base = top == -INFINITY ? 0.0f : top; // nothing seen yet: exp2(-inf - 0) = 0
                     const float keep = exp2_fast(m[n][j] - base);
                     m[n][j] = top;
-                    w[j] = exp2_fast(v[j] - base);
-                    w[j + 2] = exp2_fast(v[j + 2] - base);
-                    l[n][j] = l[n][j] * keep + (w[j] + w[j + 2]);
+                    w[j] = exp2_fast(v[j] - (base - kTop<FP8>));
+                    w[j + 2] = exp2_fast(v[j + 2] - (base - kTop<FP8>));
+                    l[n][j] = FP8 ? fmaf(w[j], unit0, fmaf(w[j + 2], unit1, l[n][j] * keep)) : l[n][j] * keep + (w[j] + w[j + 2]);
                     if (__any_sync(0xffffffffu, keep != 1.0f)) {
 #pragma unroll
                         for (uint32_t d = 0; d < D / 16; ++d) {
@@ -331,8 +387,8 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
                         }
                     }
                 }
-                pf[n][0] = transpose8(tc::pack_bf16x2(w[0] * vs0, w[1] * vs0));
-                pf[n][1] = transpose8(tc::pack_bf16x2(w[2] * vs1, w[3] * vs1));
+                pf[n][0] = transpose8(FP8 ? pack_f16x2(w[0], w[1]) : tc::pack_bf16x2(w[0], w[1]));
+                pf[n][1] = transpose8(FP8 ? pack_f16x2(w[2], w[3]) : tc::pack_bf16x2(w[2], w[3]));
             }
 
             // O^T += V^T P^T
@@ -344,7 +400,7 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
                     ldmatrix4_trans(a, v_base + swizzled<ROW_BYTES>((lane & 7) + lane / 16 * 8, d * 2 + (lane >> 3 & 1)));
 #pragma unroll
                     for (uint32_t n = 0; n < NT; ++n)
-                        mma16816(o[d][n], a, pf[n][0], pf[n][1]);
+                        mma16816<FP8>(o[d][n], a, pf[n][0], pf[n][1]);
                 }
             } else {
 #pragma unroll
@@ -354,13 +410,12 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
 #pragma unroll
                     for (uint32_t u = 0; u < 2; ++u) {
                         // a word holds elements 2r, 2r + 1 of two keys: rows r and r + 8 of the product
-                        const uint32_t a[4] = { e4m3x2_to_bf16x2(__byte_perm(w[2 * u], 0, 0x2404)),
-                                                e4m3x2_to_bf16x2(__byte_perm(w[2 * u], 0, 0x3414)),
-                                                e4m3x2_to_bf16x2(__byte_perm(w[2 * u + 1], 0, 0x2404)),
-                                                e4m3x2_to_bf16x2(__byte_perm(w[2 * u + 1], 0, 0x3414)) };
+                        const uint32_t first = __byte_perm(w[2 * u], 0, 0x3120), second = __byte_perm(w[2 * u + 1], 0, 0x3120);
+                        const uint32_t a[4] = { e4m3x2_to_f16x2(first), e4m3x2_to_f16x2(first >> 16), e4m3x2_to_f16x2(second),
+                                                e4m3x2_to_f16x2(second >> 16) };
 #pragma unroll
                         for (uint32_t n = 0; n < NT; ++n)
-                            mma16816(o[db * 2 + u][n], a, pf[n][0], pf[n][1]);
+                            mma16816<FP8>(o[db * 2 + u][n], a, pf[n][0], pf[n][1]);
                     }
                 }
             }
@@ -399,6 +454,7 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
                 }
             }
         __syncthreads();
+        constexpr float kUnits = kSumUnit<FP8> - kTop<FP8>; // from a row's maximum to the unit of its sums
         const bool whole = seg.whole;
         const uint32_t slot = blockIdx.x * 2 + (seg.starts ? 1 : 0);
         for (uint32_t i = tid; i < nrows * (D / 4); i += kStreamThreads) {
@@ -418,16 +474,18 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
             }
             if (whole) {
                 const uint32_t token = p.tiling.group.div(row0 + r), h = at.head * p.tiling.group.d + row0 + r - token * p.tiling.group.d;
-                const float inv = top == -INFINITY ? 0.0f : 1.0f / sum;
+                const float inv = top == -INFINITY ? 0.0f : kSumFactor<FP8> / sum;
                 const uint2 w = make_uint2(tc::pack_bf16x2(acc.x * inv, acc.y * inv), tc::pack_bf16x2(acc.z * inv, acc.w * inv));
                 *reinterpret_cast<uint2*>(p.out + (rows.row0 + token) * p.out_token + h * p.out_head + e * 2) = w;
                 if (e == 0 && p.lse != nullptr)
                     p.lse[(rows.row0 + token) * p.lse_token + h * p.lse_head]
-                        = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
+                        = top == -INFINITY ? -INFINITY : (top + kUnits + log2f(sum)) * 0.693147180559945f;
             } else {
-                *reinterpret_cast<float4*>(p.part_o + (static_cast<size_t>(slot) * ROWS + r) * D + e) = acc;
+                constexpr float f = kSumFactor<FP8>;
+                *reinterpret_cast<float4*>(p.part_o + (static_cast<size_t>(slot) * ROWS + r) * D + e)
+                    = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
                 if (e == 0)
-                    p.part_ml[static_cast<size_t>(slot) * ROWS + r] = make_float2(top, sum);
+                    p.part_ml[static_cast<size_t>(slot) * ROWS + r] = make_float2(top + kUnits, sum);
             }
         }
         next_segment(p, seg, &at, &left);
