@@ -580,6 +580,15 @@ bool rows_apart(const qsfi_tensor3& t) // rows of shape[2] elements at two strid
     return true;
 }
 
+bool rows_fit(const PagedView& v)
+{
+    for (const PagedPool* p : { &v.k, &v.v })
+        if (((v.pages - 1) * static_cast<uint64_t>(p->page_stride) + (v.page_size - 1) * static_cast<uint64_t>(p->slot_stride)) >> p->unit_shift
+            >= 0xffffffffu)
+            return false;
+    return true;
+}
+
 qsfi_status paged_view(qsfi_context* ctx, const qs3_paged_kv_cache& cache, const qs3_page_table& table, const char* op,
                        PagedView* out, bool* fp8)
 {
@@ -637,6 +646,10 @@ qsfi_status paged_view(qsfi_context* ctx, const qs3_paged_kv_cache& cache, const
         p.page_stride = t.stride[0] * unit;
         p.head_stride = t.stride[1] * unit;
         p.slot_stride = t.stride[2] * unit;
+        p.unit_shift = 4; // (16-byte rows)
+        while (p.unit_shift < 20 && (p.page_stride | p.slot_stride) % (int64_t { 2 } << p.unit_shift) == 0)
+            ++p.unit_shift;
+        p.unit = 1u << p.unit_shift;
         p.scale = static_cast<float*>(scale.data);
         p.scale_page_stride = scale.stride[0];
         p.scale_head_stride = scale.stride[1];

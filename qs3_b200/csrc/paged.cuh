@@ -16,6 +16,7 @@ constexpr uint32_t kMaxBatch = 4096;
 struct PagedPool {
     uint8_t* data;
     int64_t page_stride, head_stride, slot_stride;
+    uint32_t unit, unit_shift; // power of two that divides page_stride and slot_stride
     float* scale;
     int64_t scale_page_stride, scale_head_stride, scale_slot_stride;
 };
@@ -69,6 +70,18 @@ __device__ __forceinline__ int32_t page_of(const PagedView& p, const SeqPages& s
     return -1;
 }
 
+// Where a token's row of the first head begins, in the pool's units, which 32 bits hold (rows_fit on the host). None: a token
+// that is not there, whose row counts as zeros.
+constexpr uint32_t kNoRow = 0xffffffffu;
+__device__ __forceinline__ uint32_t row_units(const PagedPool& pool, int32_t page, uint32_t slot)
+{
+    return page < 0 ? kNoRow : static_cast<uint32_t>((page * pool.page_stride + slot * pool.slot_stride) >> pool.unit_shift);
+}
+__device__ __forceinline__ uint64_t row_bytes(const PagedPool& pool, uint32_t row)
+{
+    return static_cast<uint64_t>(row == kNoRow ? 0 : row) * pool.unit;
+}
+
 // Largest i in [0, n) with table[i] <= x, for ascending table[0 .. n] with table[0] <= x; the whole warp searches, 32 places
 // at a time. Any table gives an i in range.
 __device__ __forceinline__ uint32_t warp_upper(const int32_t* table, uint32_t n, int32_t x)
@@ -90,6 +103,7 @@ __device__ __forceinline__ uint32_t warp_upper(const int32_t* table, uint32_t n,
 
 // Host side: checks and views of the descriptors (kv_cache.cu).
 bool rows_apart(const qsfi_tensor3& t);
+bool rows_fit(const PagedView& v);
 qsfi_status check_rows(qsfi_context* ctx, const qsfi_tensor3& t, const char* op, const char* name, qsfi_dtype dtype);
 qsfi_status check_index(qsfi_context* ctx, const qsfi_tensor1& t, const char* op, const char* name, int64_t length);
 qsfi_status paged_view(qsfi_context* ctx, const qs3_paged_kv_cache& cache, const qs3_page_table& table, const char* op,

@@ -121,7 +121,9 @@ template <uint32_t D, uint32_t NT, bool FP8> struct StreamShape {
     static constexpr uint32_t kLarger = kRing > kSums ? kRing : kSums;
     static constexpr uint32_t kUnion = kLarger > kCosts ? kLarger : kCosts;
     static constexpr uint32_t kSmem = kUnion + kQ + kStreamWarps * kRows * 8 + (FP8 ? kRows * 4 : 0);
-    static constexpr uint32_t kBlocks = 227 * 1024 / (kSmem + 1024); // per SM
+    // per SM, by shared memory and by 128 registers a thread where that is more than two
+    static constexpr uint32_t kFit = 227 * 1024 / (kSmem + 1024);
+    static constexpr uint32_t kBlocks = kFit < 4 ? kFit : 4;
 };
 
 // Byte offset of 16-byte unit `c` of row `r`: eight rows that one ldmatrix reads lie in different banks.
@@ -133,7 +135,8 @@ template <uint32_t ROW_BYTES> __device__ __forceinline__ uint32_t swizzled(uint3
         return r * ROW_BYTES + ((c ^ (r >> 1 & 3)) * 16);
 }
 
-template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(kStreamThreads) attn_stream_kernel(AttnParams p)
+template <uint32_t D, uint32_t NT, bool FP8> 
+__global__ void __launch_bounds__(kStreamThreads, StreamShape<D, NT, FP8>::kBlocks) attn_stream_kernel(AttnParams p)
 {
     using Shape = StreamShape<D, NT, FP8>;
     constexpr uint32_t ROWS = Shape::kRows, ROW_BYTES = Shape::kRowBytes;
@@ -256,19 +259,17 @@ template <uint32_t D, uint32_t NT, bool FP8> __global__ void __launch_bounds__(k
                 int32_t page = -1;
                 if (key >= seen_lo && key < seen_hi)
                     page = page_of(p.view, pages, key, &slot);
+                const uint32_t k_row = row_units(p.view.k, page, slot), v_row = row_units(p.view.v, page, slot);
                 constexpr uint32_t UNITS = ROW_BYTES / 16, STEP = 32 / UNITS == 0 ? 1 : 32 / UNITS; // rows per instruction
                 const uint32_t r_lane = lane / UNITS, c = lane % UNITS;
                 static_assert(UNITS <= 32, "a row is at most 512 bytes");
 #pragma unroll
                 for (uint32_t r0 = 0; r0 < kWarpKeys; r0 += STEP) {
                     const uint32_t r = r0 + r_lane;
-                    const int32_t pg = __shfl_sync(0xffffffffu, page, r & 15);
-                    const uint32_t sl = __shfl_sync(0xffffffffu, slot, r & 15);
-                    const int64_t pg0 = pg < 0 ? 0 : pg;
+                    const uint32_t k = __shfl_sync(0xffffffffu, k_row, r & 15), v = __shfl_sync(0xffffffffu, v_row, r & 15);
                     const uint32_t dst = base + swizzled<ROW_BYTES>(r, c);
-                    cp_async16(dst, k_head + pg0 * p.view.k.page_stride + sl * p.view.k.slot_stride + c * 16, pg >= 0);
-                    cp_async16(dst + Shape::kHalf, v_head + pg0 * p.view.v.page_stride + sl * p.view.v.slot_stride + c * 16,
-                               pg >= 0);
+                    cp_async16(dst, k_head + row_bytes(p.view.k, k) + c * 16, k != kNoRow);
+                    cp_async16(dst + Shape::kHalf, v_head + row_bytes(p.view.v, v) + c * 16, v != kNoRow);
                 }
                 if constexpr (FP8) {
                     const PagedPool& pool = lane < 16 ? p.view.k : p.view.v;
@@ -745,6 +746,8 @@ qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_des
         p.lse_token = d->lse.stride[0];
         p.lse_head = d->lse.stride[1];
     }
+    if (!rows_fit(p.view))
+        return set_unsupported(ctx, "paged_attention cache has more than 2^32 rows' worth of memory between its first and last");
     if (d->window != 0 && d->causal == 0)
         return set_unsupported(ctx, "paged_attention window needs causal");
     if (!std::isfinite(d->sm_scale) || d->sm_scale < 0.0f)
@@ -784,11 +787,7 @@ qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_des
     p.tiling.kv_heads = p.view.kv_heads;
     p.tiling.window = d->window;
     p.tiling.causal = d->causal;
-    // the kernel for chunks counts rows of the cache in units of 16 bytes, 32 bits of them
-    const auto reach = [&](const PagedPool& pool) {
-        return static_cast<int64_t>(p.view.pages - 1) * pool.page_stride + static_cast<int64_t>(p.view.page_size - 1) * pool.slot_stride;
-    };
-    const bool chunks = fresh * group > 16 && reach(p.view.k) < (int64_t { 1 } << 36) && reach(p.view.v) < (int64_t { 1 } << 36);
+    const bool chunks = fresh * group > 16;
     uint32_t item_rows;
     if (chunks) {
         item_rows = attn_prefill_rows(dim);

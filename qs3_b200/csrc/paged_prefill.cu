@@ -45,7 +45,6 @@ constexpr uint32_t kSoftmaxWarps = 8;
 constexpr uint32_t kMostSlots = 6;
 constexpr uint32_t kScaleTiles = 4; // key tiles whose scales are held
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kNone = 0xffffffffu;
 // Growth of a row's maximum, in powers of two, before O is rescaled, and where the largest weight lies at first: f16 weights end at
 // 2^16 and lose bits below 2^-14.
 template <bool FP8> constexpr float kGrowth = FP8 ? 7.0f : 8.0f;
@@ -467,7 +466,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 const auto fetch = [&](uint32_t piece, Places l, auto keys, auto units, uint32_t skip) {
                     constexpr uint32_t KEYS = decltype(keys)::value, UNITS = decltype(units)::value, AT_ONCE = 32 / UNITS;
                     const PagedPool& pool = value ? p.view.v : p.view.k;
-                    uint32_t row[KEYS / 32]; // in units of 16 bytes; none: zeros
+                    uint32_t row[KEYS / 32];
 #pragma unroll
                     for (uint32_t j = 0; j < KEYS / 32; ++j) {
                         const uint32_t key = key_of(piece, j);
@@ -476,7 +475,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                                 atomicCAS(p.err, 0u, static_cast<uint32_t>(ERR_PAGE_TABLE));
                             l.page[j] = -1;
                         }
-                        row[j] = l.page[j] < 0 ? kNone : static_cast<uint32_t>((l.page[j] * pool.page_stride + l.slot[j] * pool.slot_stride) >> 4);
+                        row[j] = row_units(pool, l.page[j], l.slot[j]);
                     }
                     const uint8_t* const from = pool.data + at.head * pool.head_stride + skip + (lane % UNITS) * 16;
                     const uint32_t to = smem_u32(staging) + ((warp - Shape::kLoadWarp) * 2 + (staged & 1)) * Shape::kStage;
@@ -484,7 +483,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
 #pragma unroll
                     for (uint32_t j = 0; j < KEYS / AT_ONCE; ++j) {
                         const uint32_t r = __shfl_sync(0xffffffffu, row[j * AT_ONCE / 32], (j * AT_ONCE + lane / UNITS) & 31);
-                        cp_async16z(to + (j * 32 + lane) * 16, from + static_cast<uint64_t>(r == kNone ? 0 : r) * 16, r != kNone);
+                        cp_async16z(to + (j * 32 + lane) * 16, from + row_bytes(pool, r), r != kNoRow);
                     }
                     if (!value && piece % PER_TILE == 0) // the tile's scales, of K and V
 #pragma unroll
@@ -557,19 +556,14 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 constexpr uint32_t KEYS = decltype(keys)::value, UNITS = decltype(units)::value, AT_ONCE = 32 / UNITS;
                 const uint32_t s = (before + piece) % slots;
                 const bool boxes = a.boxes && __all_sync(0xffffffffu, a.page >= 0);
-                // otherwise where the rows of keys lane + 32 j begin, in units of 16 bytes; none: zeros
+                // otherwise the rows of keys lane + 32 j
                 uint32_t row[KEYS / 32];
                 if (!boxes) {
 #pragma unroll
                     for (uint32_t j = 0; j < KEYS / 32; ++j) {
                         const uint32_t key = a.key0 + j * 32 + lane;
-                        row[j] = kNone;
-                        if (key >= seen_lo && key < seen_hi) {
-                            uint32_t slot;
-                            const int32_t page = page_of(p.view, seg.pages, key, &slot);
-                            if (page >= 0)
-                                row[j] = static_cast<uint32_t>((page * pool.page_stride + slot * pool.slot_stride) >> 4);
-                        }
+                        uint32_t slot = 0;
+                        row[j] = row_units(pool, key >= seen_lo && key < seen_hi ? page_of(p.view, seg.pages, key, &slot) : -1, slot);
                     }
                 }
                 if (!wait(&empty_bar[s], (((before + piece) / slots) & 1) ^ 1, ERR_PF_EMPTY_WAIT))
@@ -593,7 +587,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     const uint32_t key = j * AT_ONCE + lane / UNITS;
                     const uint32_t r = __shfl_sync(0xffffffffu, row[j * AT_ONCE / 32], key & 31);
                     cp_async16z(to + key * 128 + (((lane & 7) ^ (key & 7)) * 16),
-                                from + static_cast<uint64_t>(r == kNone ? 0 : r) * 16, r != kNone);
+                                from + row_bytes(pool, r), r != kNoRow);
                 }
                 copies.push(&full_bar[s]);
                 return true;
