@@ -883,17 +883,20 @@ bool make_output_map(CUtensorMap* map, bool f32, void* out, uint64_t cols, uint6
         == CUDA_SUCCESS;
 }
 
-bool make_page_map(CUtensorMap* map, const void* base, const uint64_t* dims, const uint64_t* strides, uint32_t box_rows)
+bool make_page_map(CUtensorMap* map, bool bytes_type, const void* base, const uint64_t* dims, const uint64_t* strides, uint32_t box_bytes,
+                   uint32_t box_rows)
 {
     EncodeTiledFn fn = encode_tiled_fn();
     if (fn == nullptr || !aligned16(base))
         return false;
     const cuuint64_t d[4] = { dims[0], dims[1], dims[2], dims[3] };
     const cuuint64_t st[3] = { strides[0], strides[1], strides[2] };
-    const cuuint32_t box[4] = { 64, box_rows, 1, 1 };
+    const cuuint32_t box[4] = { bytes_type ? box_bytes : box_bytes / 2, box_rows, 1, 1 };
     const cuuint32_t estr[4] = { 1, 1, 1, 1 };
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
+    const CUtensorMapDataType type = bytes_type ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return fn(map, type, 4, const_cast<void*>(base), d, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
         == CUDA_SUCCESS;
 }
 

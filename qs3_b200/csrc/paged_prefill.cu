@@ -21,11 +21,14 @@
 // divides come that way; other page sizes, the ends of sequences and windows row by row with cp.async, 16 bytes being the unit
 // in which every page size, stride and swizzled place works. Keys that no row sees are zeros then.
 //
-// e4m3 caches are multiplied in f16, which holds every code exactly: the fetching warps copy codes to a staging area of their own,
-// and from there, converted, to the ring. A row of queries is scaled by the power of two that brings its largest element to 2^13
-// or just above, so that f16 holds it to 2^-26 of that element, below the rounding of the f32 sums. K's scales are a factor on the
-// scores. V's are part of the weights, w = exp2(s + log2(scale) - m): the largest is again at a known place, and f16 keeps 11
-// bits of them where bf16 products would keep 8. The row's sum takes the scale out again.
+// e4m3 caches: K's codes are multiplied as they are. A row of queries is scaled by the power of two that brings its largest element
+// to 2^7 or just above and becomes the sum of two e4m3 numbers, the high one rounded to 4 bits and the low one the rest: bf16's 8
+// bits exactly, and no element is off by more than 2^-17 of the largest. Two products of twice the rate take the time of one.
+// K's scales are a factor on the scores. V's are part of the weights, w = exp2(s + log2(scale) - m), of which the largest is again
+// at a known place; a second e4m3 number would keep 8 bits of a weight but only 14 of the range below the largest, which many
+// small weights together need, so the weights are f16 and V is converted, by the five warps that fetch it: from memory to
+// registers, half a piece while the other half is converted, and on to the ring. The row's sum takes V's scale out again.
+// (All converted to f16, K too, by way of a staging area: 1021 tokens behind 31 111 cached ones 965 us.)
 #include "paged_attention.cuh"
 #include "tcgen05.cuh"
 
@@ -79,28 +82,29 @@ template <uint32_t D, bool FP8> struct PrefillShape {
     static constexpr uint32_t kStep = kTiles == 1 ? 128 : 64; // keys of a score tile
     static constexpr uint32_t kSteps = kKeyTile / kStep;      // of a key tile
     static constexpr uint32_t kRows = kTiles * kRowTile;
-    static constexpr uint32_t kPiece = D == 64 || FP8 ? 16384 : 32768;
-    static constexpr uint32_t kWarpsK = FP8 ? 2 : 3, kWarpsV = 2, kLoadWarps = kWarpsK + kWarpsV;
-    static constexpr uint32_t kSlotsK = FP8 ? 2 : D == 64 ? 6 : 3, kSlotsV = FP8 ? 2 : D == 64 ? 4 : 2; // of the rings
-    // e4m3: codes of two pieces for each fetching warp, K's and V's scales of a tile beside them
-    static constexpr uint32_t kCodes = kPiece / 2, kStage = kCodes + 2 * kKeyTile * 4;
-    static constexpr uint32_t kStaging = FP8 ? kLoadWarps * 2 * kStage : 0;
+    static constexpr uint32_t kWidth = FP8 && D == 64 ? 64 : 128; // bytes of a row in a panel of K, and of Q
+    static constexpr uint32_t kPieceK = FP8 ? kKeyTile * kWidth : D == 64 ? 16384 : 32768, kPieceV = D == 64 || FP8 ? 16384 : 32768;
+    static constexpr uint32_t kWarpsK = FP8 ? 1 : 3, kWarpsV = FP8 ? 5 : 2, kLoadWarps = kWarpsK + kWarpsV;
+    static constexpr uint32_t kQueryWarps = FP8 ? kWarpsV : kWarpsK; // load the queries too
+    // of the rings; e4m3: K of two tiles, which is also what the ring of scales relies on
+    static constexpr uint32_t kSlotsK = FP8 ? (D == 256 ? 4 : 2) : D == 64 ? 6 : 3, kSlotsV = FP8 ? 5 : D == 64 ? 4 : 2;
     static constexpr uint32_t kScales = FP8 ? kScaleTiles * kKeyTile * 3 * 4 : 0;
     static constexpr uint32_t kQueryScales = FP8 ? 2 * kRows * 4 : 0;
-    static constexpr uint32_t kPanels = kPiece / (kKeyTile * 128);  // panels of 64 elements in a piece of K
-    static constexpr uint32_t kPieceKeys = kPiece / (2 * D);        // keys of a piece of V
-    static constexpr uint32_t kPerTile = kKeyTile / kPieceKeys;     // pieces of a tile of K, and of V
+    static constexpr uint32_t kPanels = kPieceK / (kKeyTile * kWidth); // of a piece of K
+    static constexpr uint32_t kPieceKeys = kPieceV / (2 * D);          // of a piece of V
+    static constexpr uint32_t kPerTileK = kKeyTile * D * (FP8 ? 1 : 2) / kPieceK, kPerTileV = kKeyTile / kPieceKeys; // pieces of a tile
     static constexpr uint32_t kQ = kRows * D * 2;
-    static constexpr uint32_t kLoadWarp = kSoftmaxWarps;            // first of five
+    static constexpr uint32_t kLoadWarp = kSoftmaxWarps;            // first of those that fetch
     static constexpr uint32_t kScoreWarp = kSoftmaxWarps + kLoadWarps;
     static constexpr uint32_t kThreads = (kSoftmaxWarps + kLoadWarps + 2) * 32;
-    static constexpr uint32_t kRing = (kSlotsK + kSlotsV) * kPiece;
-    static constexpr uint32_t kSmem = 1024 + kQ + kRing + kStaging + kScales + kQueryScales + sizeof(Barriers);
+    static constexpr uint32_t kRingK = kSlotsK * kPieceK, kRing = kRingK + kSlotsV * kPieceV;
+    static constexpr uint32_t kSmem = 1024 + kQ + kRing + kScales + kQueryScales + sizeof(Barriers);
     static_assert(kSlotsK % kWarpsK == 0 && kSlotsV % kWarpsV == 0, "a slot is one warp's");
     static_assert(kSmem <= 227 * 1024, "shared memory of a block");
     static_assert(kRing >= kMaxBatch * 8, "the search for the block's range uses the ring");
     static_assert(kSlotsK <= kMostSlots && kSlotsV <= kMostSlots, "barriers of the slots");
-    static_assert(kPanels * 64 * kPerTile == D, "a tile of K has as many pieces as one of V");
+    static_assert(!FP8 || kSlotsK == 2 * kPerTileK, "K of two tiles");
+    static_assert(kThreads <= 512, "128 registers for each");
 };
 
 __device__ __forceinline__ void cp_async16z(uint32_t dst, const void* src, bool there)
@@ -166,6 +170,29 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t x)
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(x)));
     return r;
 }
+
+// Two codes in the low half, that of a in the low byte.
+__device__ __forceinline__ uint32_t pack_e4m3x2(float a, float b)
+{
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+    return r;
+}
+__device__ __forceinline__ float2 f16x2_to_f32(uint32_t x)
+{
+    float2 r;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(r.x), "=f"(r.y) : "r"(x));
+    return r;
+}
+__device__ __forceinline__ uint4 load_codes(const uint8_t* p)
+{
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+
+// What the place of a row's unit of 16 bytes is crossed with, rows being 128 or 64 bytes.
+template <uint32_t WIDTH> __device__ __forceinline__ uint32_t swizzle_of(uint32_t row) { return WIDTH == 128 ? row & 7 : row >> 1 & 3; }
 
 // Two floats in a register pair, one instruction for both.
 __device__ __forceinline__ uint64_t pack2(float a, float b)
@@ -247,14 +274,14 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
     using Shape = PrefillShape<D, FP8>;
     constexpr uint32_t kWarpsK = Shape::kWarpsK, kWarpsV = Shape::kWarpsV;
     constexpr uint32_t TILES = Shape::kTiles, STEP = Shape::kStep, STEPS = Shape::kSteps, PANELS = Shape::kPanels, PIECE_KEYS = Shape::kPieceKeys;
-    constexpr uint32_t PER_TILE = Shape::kPerTile, kPiece = Shape::kPiece, SLOTS_K = Shape::kSlotsK, SLOTS_V = Shape::kSlotsV;
+    constexpr uint32_t PER_TILE_K = Shape::kPerTileK, PER_TILE_V = Shape::kPerTileV, SLOTS_K = Shape::kSlotsK, SLOTS_V = Shape::kSlotsV;
+    constexpr uint32_t kPieceK = Shape::kPieceK, kPieceV = Shape::kPieceV, WIDTH = Shape::kWidth;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* const ring = smem + Shape::kQ;
-    uint8_t* const staging = ring + Shape::kRing;
-    float* const scales = reinterpret_cast<float*>(staging + Shape::kStaging); // of a tile's key pairs: K's, log2 of V's; then 1 / V's
+    float* const scales = reinterpret_cast<float*>(ring + Shape::kRing); // of a tile's key pairs: K's, log2 of V's; then 1 / V's
     float* const q_scales = scales + Shape::kScales / 4; // what the rows of queries were divided by, of this segment and the next
-    Barriers& bar = *reinterpret_cast<Barriers*>(staging + Shape::kStaging + Shape::kScales + Shape::kQueryScales);
+    Barriers& bar = *reinterpret_cast<Barriers*>(ring + Shape::kRing + Shape::kScales + Shape::kQueryScales);
     const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
 
     if (tid == 0) {
@@ -266,7 +293,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
         }
         for (uint32_t i = 0; i < kScaleTiles; ++i)
             mbar_init(&bar.scale_full[i], 1);
-        mbar_init(&bar.q_full, kWarpsK);
+        mbar_init(&bar.q_full, Shape::kQueryWarps);
         mbar_init(&bar.q_free, 1);
         for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(&bar.s_full[i], 1);
@@ -308,71 +335,19 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
         // ------------------------------------------------------------------------------ fetching --
         const bool value = warp - Shape::kLoadWarp >= kWarpsK; // fetches V
         const uint32_t w = value ? warp - Shape::kLoadWarp - kWarpsK : warp - Shape::kLoadWarp, warps = value ? kWarpsV : kWarpsK;
-        const uint32_t slots = value ? SLOTS_V : SLOTS_K;
+        const uint32_t slots = value ? SLOTS_V : SLOTS_K, piece_bytes = value ? kPieceV : kPieceK;
         uint64_t* const full_bar = value ? bar.v_full : bar.k_full;
         uint64_t* const empty_bar = value ? bar.v_empty : bar.k_empty;
-        const uint32_t ring_at = smem_u32(ring) + (value ? SLOTS_K * kPiece : 0);
+        const uint32_t ring_at = smem_u32(ring) + (value ? Shape::kRingK : 0);
         Copies copies;
         uint32_t before = 0, segments = 0; // pieces of earlier segments
+        uint32_t filled = 0;               // this warp's pieces so far, the n-th of them being number n * warps + w of all
         bool ok = true;
         const auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
             if (__all_sync(0xffffffffu, mbar_test_wait(b, parity)))
                 return true;
-            if constexpr (!FP8)
-                copies.drain();
+            copies.drain();
             return __all_sync(0xffffffffu, mbar_wait(b, parity, &bar.abort, p.err, code)) != 0;
-        };
-        // e4m3: pieces that this warp has fetched so far, of all segments; the last one or two wait in its staging area. Its n-th
-        // is number n * warps + w of all. `newer`: another one has been fetched since.
-        uint32_t staged = 0, converted = 0;
-        const auto convert = [&](uint32_t n, bool newer) {
-            const uint32_t piece = n * warps + w, s = piece % slots;
-            if (!wait(&empty_bar[s], ((piece / slots) & 1) ^ 1, ERR_PF_EMPTY_WAIT))
-                return false;
-            if (newer)
-                asm volatile("cp.async.wait_group 1;" ::: "memory");
-            else
-                asm volatile("cp.async.wait_all;" ::: "memory");
-            const uint8_t* const from = staging + ((warp - Shape::kLoadWarp) * 2 + (n & 1)) * Shape::kStage;
-            const uint32_t units = value ? D / 16 : 4, panel = value ? PIECE_KEYS * 128 : 0; // 16 codes each; bytes of a panel
-            uint8_t* const to = ring + (value ? SLOTS_K * kPiece : 0) + s * kPiece;
-#pragma unroll 4
-            for (uint32_t j = 0; j < Shape::kCodes / 512; ++j) {
-                const uint32_t i = j * 32 + lane, key = i / units, u = i % units;
-                const uint4 c = *reinterpret_cast<const uint4*>(from + i * 16); // (fetched by this lane)
-                const uint32_t x[4] = { c.x, c.y, c.z, c.w };
-                uint32_t y[8];
-#pragma unroll
-                for (uint32_t k = 0; k < 8; ++k)
-                    y[k] = e4m3x2_to_f16x2(x[k / 2] >> (16 * (k & 1)));
-                uint8_t* const row = to + u / 4 * panel + key * 128;
-                const uint32_t first = u % 4 * 2;
-                *reinterpret_cast<uint4*>(row + ((first ^ (key & 7)) * 16)) = make_uint4(y[0], y[1], y[2], y[3]);
-                *reinterpret_cast<uint4*>(row + (((first + 1) ^ (key & 7)) * 16)) = make_uint4(y[4], y[5], y[6], y[7]);
-            }
-            if (!value && piece % PER_TILE == 0) {
-                // These need no barrier for their way back: K of four tiles on is not fetched before the scores of two tiles on have
-                // been read.
-                const uint32_t tile = piece / PER_TILE % kScaleTiles;
-                const float* const raw = reinterpret_cast<const float*>(from + Shape::kCodes);
-                float* const out = scales + tile * (kKeyTile * 3);
-#pragma unroll
-                for (uint32_t j = 0; j < kKeyTile / 32; ++j) {
-                    const uint32_t key = j * 32 + lane;
-                    const float v = raw[kKeyTile + key];
-                    out[key / 2 * 4 + (key & 1)] = raw[key] * p.scale_log2;
-                    out[key / 2 * 4 + 2 + (key & 1)] = log2f(v < 1.0e-30f ? 1.0e-30f : v); // (a NaN stays one)
-                    out[kKeyTile * 2 + key] = kSumFactor<FP8> / (v < 1.0e-30f ? 1.0e-30f : v);
-                }
-                __syncwarp();
-                if (lane == 0)
-                    mbar_arrive(&bar.scale_full[tile]);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the tensor core reads what was written here
-            __syncwarp();
-            if (lane == 0)
-                mbar_arrive(&full_bar[s]);
-            return true;
         };
         while (ok && this_segment(p, at, left, &seg)) {
             uint32_t seen_lo, seen_hi, unused;
@@ -385,14 +360,15 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     return false;
                 static_assert(Shape::kRows % 4 == 0, "four rows of a warp at a time");
 #pragma unroll 1
-                for (uint32_t r0 = w * 4; r0 < Shape::kRows; r0 += kWarpsK * 4) {
+                for (uint32_t r0 = w * 4; r0 < Shape::kRows; r0 += Shape::kQueryWarps * 4) {
                     const uint32_t r = r0 + lane / 8, in_tile = r & (kRowTile - 1);
                     const bool there = r < seg.nrows;
                     const uint32_t flat = seg.row0 + (there ? r : 0), token = p.tiling.group.div(flat);
                     const uint8_t* src = p.q + (seg.rows.row0 + token) * p.q_token
                         + (at.head * p.tiling.group.d + flat - token * p.tiling.group.d) * p.q_head + (lane & 7) * 16;
-                    const uint32_t dst = (r / kRowTile) * (kRowTile * D * 2) + in_tile * 128 + (((lane & 7) ^ (r & 7)) * 16);
+                    const uint32_t tile_at = (r / kRowTile) * (kRowTile * D * 2);
                     if constexpr (!FP8) {
+                        const uint32_t dst = tile_at + in_tile * 128 + (((lane & 7) ^ (r & 7)) * 16);
 #pragma unroll
                         for (uint32_t panel = 0; panel < D / 64; ++panel)
                             cp_async16z(smem_u32(smem) + dst + panel * (kRowTile * 128), src + panel * 128, there);
@@ -410,18 +386,27 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
 #pragma unroll
                         for (uint32_t o = 1; o < 8; o <<= 1)
                             most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                        // the power of two and its reciprocal are both f32's; an infinity or NaN stays one
-                        const int power = most >= 0x7f80u ? 0 : max(-126, min(126, 127 + 13 - static_cast<int>(most >> 7)));
+                        // the power of two and its reciprocal are both f32's; a row with an infinity or a NaN becomes NaN
+                        const int power = most >= 0x7f80u ? 0 : max(-126, min(126, 127 + 7 - static_cast<int>(most >> 7)));
                         const float up = __uint_as_float(static_cast<uint32_t>(127 + power) << 23);
                         if ((lane & 7) == 0)
                             q_scales[(segments & 1) * Shape::kRows + r] = __uint_as_float(static_cast<uint32_t>(127 - power) << 23);
 #pragma unroll
                         for (uint32_t panel = 0; panel < D / 64; ++panel) {
-                            uint32_t a[4] = { v[panel].x, v[panel].y, v[panel].z, v[panel].w };
+                            const uint32_t a[4] = { v[panel].x, v[panel].y, v[panel].z, v[panel].w };
+                            uint32_t hi[4], lo[4];
 #pragma unroll
-                            for (uint32_t j = 0; j < 4; ++j)
-                                a[j] = pack_f16x2(bf16_bits_to_f32(a[j] & 0xffffu) * up, bf16_bits_to_f32(a[j] >> 16) * up);
-                            *reinterpret_cast<uint4*>(smem + dst + panel * (kRowTile * 128)) = make_uint4(a[0], a[1], a[2], a[3]);
+                            for (uint32_t j = 0; j < 4; ++j) {
+                                const float x = bf16_bits_to_f32(a[j] & 0xffffu) * up, y = bf16_bits_to_f32(a[j] >> 16) * up;
+                                hi[j] = most >= 0x7f80u ? 0x7f7fu : pack_e4m3x2(x, y);
+                                const float2 h = f16x2_to_f32(e4m3x2_to_f16x2(hi[j]));
+                                lo[j] = pack_e4m3x2(x - h.x, y - h.y);
+                            }
+                            const uint32_t at_byte = panel * 64 + (lane & 7) * 8, unit = at_byte % WIDTH / 16;
+                            uint8_t* const dst = smem + tile_at + at_byte / WIDTH * (kRowTile * WIDTH) + in_tile * WIDTH
+                                + ((unit ^ swizzle_of<WIDTH>(in_tile)) * 16) + at_byte % 16;
+                            *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16);
+                            *reinterpret_cast<uint2*>(dst + kRowTile * D) = make_uint2(lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
                         }
                     }
                 }
@@ -437,25 +422,24 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 return true;
             };
 
-            const uint32_t pieces = seg.count * PER_TILE;
+            const uint32_t pieces = seg.count * (value ? PER_TILE_V : PER_TILE_K);
             uint32_t mine = (w + warps - before % warps) % warps; // the first that goes to one of this warp's slots
             bool query = value; // loaded, or not this warp's business
-            if constexpr (FP8) {
+            if (FP8 && value) {
+                // ---- V: codes to registers, from there in f16 to the ring; two halves of a piece in turn
+                constexpr uint32_t UNITS = D / 16, AT_ONCE = 32 / UNITS, SETS = PIECE_KEYS / 32, LOADS = PIECE_KEYS / AT_ONCE, HALF = LOADS / 2;
                 struct Places { // of keys lane + 32 j of a piece
-                    int32_t page[kKeyTile / 32];
-                    uint32_t slot[kKeyTile / 32];
+                    int32_t page[SETS];
+                    uint32_t slot[SETS];
                 };
-                const auto key_of = [&](uint32_t piece, uint32_t j) {
-                    return seg.tile0 * kKeyTile + (value ? piece * PIECE_KEYS : piece / PER_TILE * kKeyTile) + j * 32 + lane;
-                };
-                const auto look = [&](uint32_t piece) {
+                const auto look = [&](uint32_t piece) { // (pages are not looked at yet: their loads may take their time)
                     Places l;
 #pragma unroll
-                    for (uint32_t j = 0; j < kKeyTile / 32; ++j) {
-                        const uint32_t key = key_of(piece, j);
+                    for (uint32_t j = 0; j < SETS; ++j) {
+                        const uint32_t key = seg.tile0 * kKeyTile + piece * PIECE_KEYS + j * 32 + lane;
                         l.page[j] = -1;
                         l.slot[j] = 0;
-                        if (j < (value ? PIECE_KEYS : kKeyTile) / 32 && key >= seen_lo && key < seen_hi) {
+                        if (key >= seen_lo && key < seen_hi) {
                             const uint32_t i = p.view.page_div.div(key);
                             l.slot[j] = key - i * p.view.page_size;
                             l.page[j] = __ldg(p.view.indices + seg.pages.first + i);
@@ -463,67 +447,183 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     }
                     return l;
                 };
-                const auto fetch = [&](uint32_t piece, Places l, auto keys, auto units, uint32_t skip) {
-                    constexpr uint32_t KEYS = decltype(keys)::value, UNITS = decltype(units)::value, AT_ONCE = 32 / UNITS;
-                    const PagedPool& pool = value ? p.view.v : p.view.k;
-                    uint32_t row[KEYS / 32];
+                uint32_t row[SETS];
+                const auto rows = [&](uint32_t piece, Places l) {
 #pragma unroll
-                    for (uint32_t j = 0; j < KEYS / 32; ++j) {
-                        const uint32_t key = key_of(piece, j);
-                        if (static_cast<uint32_t>(l.page[j]) >= p.view.pages) {
-                            if (key >= seen_lo && key < seen_hi)
-                                atomicCAS(p.err, 0u, static_cast<uint32_t>(ERR_PAGE_TABLE));
-                            l.page[j] = -1;
-                        }
-                        row[j] = row_units(pool, l.page[j], l.slot[j]);
+                    for (uint32_t j = 0; j < SETS; ++j) {
+                        const bool there = static_cast<uint32_t>(l.page[j]) < p.view.pages;
+                        const uint32_t key = seg.tile0 * kKeyTile + piece * PIECE_KEYS + j * 32 + lane;
+                        if (!there && key >= seen_lo && key < seen_hi)
+                            atomicCAS(p.err, 0u, static_cast<uint32_t>(ERR_PAGE_TABLE));
+                        row[j] = row_units(p.view.v, there ? l.page[j] : -1, l.slot[j]);
                     }
-                    const uint8_t* const from = pool.data + at.head * pool.head_stride + skip + (lane % UNITS) * 16;
-                    const uint32_t to = smem_u32(staging) + ((warp - Shape::kLoadWarp) * 2 + (staged & 1)) * Shape::kStage;
+                };
+                const uint8_t* const from = p.view.v.data + at.head * p.view.v.head_stride + (lane % UNITS) * 16;
+                uint4 codes[2][HALF];
+                const auto fetch = [&](auto which) {
+                    constexpr uint32_t H = decltype(which)::value;
                     __syncwarp();
 #pragma unroll
-                    for (uint32_t j = 0; j < KEYS / AT_ONCE; ++j) {
-                        const uint32_t r = __shfl_sync(0xffffffffu, row[j * AT_ONCE / 32], (j * AT_ONCE + lane / UNITS) & 31);
-                        cp_async16z(to + (j * 32 + lane) * 16, from + row_bytes(pool, r), r != kNoRow);
+                    for (uint32_t j = 0; j < HALF; ++j) {
+                        const uint32_t i = H * HALF + j;
+                        const uint32_t r = __shfl_sync(0xffffffffu, row[i * AT_ONCE / 32], (i * AT_ONCE + lane / UNITS) & 31);
+                        codes[H][j] = r == kNoRow ? make_uint4(0, 0, 0, 0) : load_codes(from + row_bytes(p.view.v, r));
                     }
-                    if (!value && piece % PER_TILE == 0) // the tile's scales, of K and V
-#pragma unroll
-                        for (uint32_t j = 0; j < KEYS / 32; ++j)
-#pragma unroll
-                            for (uint32_t v = 0; v < 2; ++v) {
-                                const PagedPool& of = v ? p.view.v : p.view.k;
-                                const bool there = l.page[j] >= 0;
-                                const float* from_scale = of.scale + at.head * of.scale_head_stride
-                                    + (there ? l.page[j] * of.scale_page_stride + l.slot[j] * of.scale_slot_stride : 0);
-                                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
-                                                 to + Shape::kCodes + (v * kKeyTile + j * 32 + lane) * 4),
-                                             "l"(from_scale), "r"(there ? 4u : 0u)
-                                             : "memory");
-                            }
-                    asm volatile("cp.async.commit_group;" ::: "memory");
                 };
-                Places ahead;
-                if (mine < pieces)
-                    ahead = look(mine);
-                for (; ok && mine < pieces; mine += warps) { // a piece's codes are fetched while the one before is converted
-                    const Places l = ahead;
-                    if (mine + warps < pieces)
-                        ahead = look(mine + warps);
-                    if (value)
-                        fetch(mine, l, std::integral_constant<uint32_t, PIECE_KEYS> {}, std::integral_constant<uint32_t, D / 16> {}, 0);
-                    else
-                        fetch(mine, l, std::integral_constant<uint32_t, kKeyTile> {}, std::integral_constant<uint32_t, 4> {}, mine % PER_TILE * 64);
-                    ++staged;
-                    if (staged - converted > 1)
-                        ok = convert(converted++, true);
-                    if (ok && !query) { // behind the first piece, which may find room before the queries do
-                        ok = load_query();
-                        query = true;
+                const auto convert = [&](auto which, uint8_t* to) {
+                    constexpr uint32_t H = decltype(which)::value;
+#pragma unroll
+                    for (uint32_t j = 0; j < HALF; ++j) {
+                        const uint32_t key = (H * HALF + j) * AT_ONCE + lane / UNITS, first = lane % 4 * 2;
+                        const uint32_t x[4] = { codes[H][j].x, codes[H][j].y, codes[H][j].z, codes[H][j].w };
+                        uint32_t y[8];
+#pragma unroll
+                        for (uint32_t k = 0; k < 8; ++k)
+                            y[k] = e4m3x2_to_f16x2(x[k / 2] >> (16 * (k & 1)));
+                        *reinterpret_cast<uint4*>(to + key * 128 + ((first ^ (key & 7)) * 16)) = make_uint4(y[0], y[1], y[2], y[3]);
+                        *reinterpret_cast<uint4*>(to + key * 128 + (((first + 1) ^ (key & 7)) * 16)) = make_uint4(y[4], y[5], y[6], y[7]);
                     }
+                };
+                constexpr std::integral_constant<uint32_t, 0> kFirst {};
+                constexpr std::integral_constant<uint32_t, 1> kSecond {};
+                if (mine < pieces) {
+                    rows(mine, look(mine));
+                    fetch(kFirst);
                 }
-                if (ok && !query) { // no piece here: one that is still staged belongs to scores that the queries wait for
-                    if (converted < staged)
-                        ok = convert(converted++, false);
-                    ok = ok && load_query();
+                ok = load_query();
+                for (; ok && mine < pieces; mine += kWarpsV) {
+                    const bool more = mine + kWarpsV < pieces;
+                    Places ahead;
+                    if (more)
+                        ahead = look(mine + kWarpsV);
+                    fetch(kSecond);
+                    const uint32_t s = (before + mine) % SLOTS_V;
+                    ok = wait(&empty_bar[s], (((before + mine) / SLOTS_V) & 1) ^ 1, ERR_PF_EMPTY_WAIT);
+                    if (!ok)
+                        break;
+                    uint8_t* const to = ring + Shape::kRingK + s * kPieceV + lane % UNITS / 4 * (PIECE_KEYS * 128);
+                    convert(kFirst, to);
+                    if (more) {
+                        rows(mine + kWarpsV, ahead);
+                        fetch(kFirst);
+                    }
+                    convert(kSecond, to);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the tensor core reads what was written here
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive(&full_bar[s]);
+                }
+                before += pieces;
+                ++segments;
+                next_segment(p, seg, &at, &left);
+                continue;
+            }
+            if constexpr (FP8) {
+                // ---- K as it is, a tile at a time, and the scales of both
+                struct Tile { // pages and slots of keys lane + 32 j; not looked at yet
+                    int32_t page[kKeyTile / 32];
+                    uint32_t slot[kKeyTile / 32];
+                    bool boxes; // whole boxes of cached tokens
+                };
+                const auto look = [&](uint32_t tile) {
+                    Tile t;
+                    const uint32_t key0 = (seg.tile0 + tile) * kKeyTile;
+                    t.boxes = k_box != 0 && key0 >= seen_lo && key0 + kKeyTile <= seg.pages.length;
+#pragma unroll
+                    for (uint32_t j = 0; j < kKeyTile / 32; ++j) {
+                        const uint32_t key = key0 + j * 32 + lane;
+                        t.page[j] = -1;
+                        t.slot[j] = 0;
+                        if (t.boxes || (key >= seen_lo && key < seen_hi)) {
+                            const uint32_t i = p.view.page_div.div(key);
+                            t.slot[j] = key - i * p.view.page_size;
+                            t.page[j] = __ldg(p.view.indices + seg.pages.first + i);
+                        }
+                    }
+                    return t;
+                };
+                Tile ahead = look(0);
+                for (uint32_t tile = 0; ok && tile < seg.count; ++tile) {
+                    Tile t = ahead;
+                    if (tile + 1 < seg.count)
+                        ahead = look(tile + 1);
+                    const uint32_t key0 = (seg.tile0 + tile) * kKeyTile;
+                    float scale[2][kKeyTile / 32];
+                    uint32_t row[kKeyTile / 32];
+                    bool bad = false;
+#pragma unroll
+                    for (uint32_t j = 0; j < kKeyTile / 32; ++j) {
+                        const uint32_t key = key0 + j * 32 + lane;
+                        const bool there = static_cast<uint32_t>(t.page[j]) < p.view.pages;
+                        bad |= !there && (t.boxes || (key >= seen_lo && key < seen_hi));
+                        t.page[j] = there ? t.page[j] : -1;
+                        row[j] = row_units(p.view.k, t.page[j], t.slot[j]);
+#pragma unroll
+                        for (uint32_t v = 0; v < 2; ++v) {
+                            const PagedPool& of = v ? p.view.v : p.view.k;
+                            scale[v][j] = there
+                                ? __ldg(of.scale + at.head * of.scale_head_stride + t.page[j] * of.scale_page_stride + t.slot[j] * of.scale_slot_stride)
+                                : 0.0f;
+                        }
+                    }
+                    if (bad)
+                        atomicCAS(p.err, 0u, static_cast<uint32_t>(ERR_PAGE_TABLE));
+                    const bool boxes = t.boxes && !__any_sync(0xffffffffu, bad);
+                    // lane i has box i, which begins with key i * k_box
+                    int32_t page = 0;
+                    uint32_t slot = 0;
+                    if (boxes)
+#pragma unroll
+                        for (uint32_t j = 0; j < kKeyTile / 32; ++j) {
+                            const int32_t box_page = __shfl_sync(0xffffffffu, t.page[j], lane * k_box & 31);
+                            const uint32_t box_slot = __shfl_sync(0xffffffffu, t.slot[j], lane * k_box & 31);
+                            if (lane * k_box / 32 == j)
+                                page = box_page, slot = box_slot;
+                        }
+#pragma unroll
+                    for (uint32_t panel = 0; panel < PER_TILE_K; ++panel) {
+                        const uint32_t piece = before + tile * PER_TILE_K + panel, s = piece % SLOTS_K;
+                        ok = wait(&empty_bar[s], ((piece / SLOTS_K) & 1) ^ 1, ERR_PF_EMPTY_WAIT);
+                        if (!ok)
+                            break;
+                        const uint32_t to = ring_at + s * kPieceK;
+                        if (boxes) {
+                            if (lane == 0)
+                                mbar_expect_tx(&full_bar[s], kPieceK);
+                            __syncwarp();
+                            if (lane * k_box < kKeyTile)
+                                tma_load_page(to + lane * k_box * WIDTH, &k_map, &full_bar[s], static_cast<int>(panel * WIDTH), static_cast<int>(slot),
+                                              static_cast<int>(at.head), page);
+                        } else {
+                            constexpr uint32_t UNITS = WIDTH / 16, AT_ONCE = 32 / UNITS;
+                            const uint8_t* const from = p.view.k.data + at.head * p.view.k.head_stride + panel * WIDTH + (lane % UNITS) * 16;
+#pragma unroll
+                            for (uint32_t j = 0; j < kKeyTile / AT_ONCE; ++j) {
+                                const uint32_t key = j * AT_ONCE + lane / UNITS;
+                                const uint32_t r = __shfl_sync(0xffffffffu, row[j * AT_ONCE / 32], key & 31);
+                                cp_async16z(to + key * WIDTH + ((lane % UNITS ^ swizzle_of<WIDTH>(key)) * 16), from + row_bytes(p.view.k, r), r != kNoRow);
+                            }
+                            copies.push(&full_bar[s]);
+                        }
+                        ++filled;
+                    }
+                    if (!ok)
+                        break;
+                    // These need no barrier for their way back: K of this tile has found room, so the scores of two tiles ago are
+                    // through, and those of three ago have been read, by warps that were done with the scales of four ago.
+                    const uint32_t place = (before / PER_TILE_K + tile) % kScaleTiles;
+                    float* const out = scales + place * (kKeyTile * 3);
+#pragma unroll
+                    for (uint32_t j = 0; j < kKeyTile / 32; ++j) {
+                        const uint32_t key = j * 32 + lane;
+                        const float v = scale[1][j] < 1.0e-30f ? 1.0e-30f : scale[1][j]; // (a NaN stays one)
+                        out[key / 2 * 4 + (key & 1)] = scale[0][j] * p.scale_log2;
+                        out[key / 2 * 4 + 2 + (key & 1)] = log2f(v);
+                        out[kKeyTile * 2 + key] = kSumFactor<FP8> / v;
+                    }
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive(&bar.scale_full[place]);
                 }
                 before += pieces;
                 ++segments;
@@ -538,7 +638,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
             };
             const auto look = [&](uint32_t piece) { // of the segment
                 Ahead a;
-                a.key0 = seg.tile0 * kKeyTile + (value ? piece * PIECE_KEYS : piece / PER_TILE * kKeyTile);
+                a.key0 = seg.tile0 * kKeyTile + (value ? piece * PIECE_KEYS : piece / PER_TILE_K * kKeyTile);
                 const uint32_t keys = value ? PIECE_KEYS : kKeyTile, box = value ? v_box : k_box;
                 a.slot = 0;
                 a.page = 0;
@@ -571,17 +671,18 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 if (boxes) {
                     const uint32_t per_panel = KEYS / box;
                     if (lane == 0)
-                        mbar_expect_tx(&full_bar[s], kPiece);
+                        mbar_expect_tx(&full_bar[s], piece_bytes);
                     __syncwarp();
                     if (lane < per_panel * (UNITS / 8)) {
                         const uint32_t panel = lane / per_panel, first = (lane - panel * per_panel) * box;
-                        tma_load_page(ring_at + s * kPiece + panel * (KEYS * 128) + first * 128, &map, &full_bar[s],
+                        tma_load_page(ring_at + s * piece_bytes + panel * (KEYS * 128) + first * 128, &map, &full_bar[s],
                                       static_cast<int>(skip / 2 + panel * 64), static_cast<int>(a.slot), static_cast<int>(at.head), a.page);
                     }
+                    ++filled;
                     return true;
                 }
                 const uint8_t* const from = pool.data + at.head * pool.head_stride + skip + (lane % UNITS) * 16;
-                const uint32_t to = ring_at + s * kPiece + (lane % UNITS / 8) * (KEYS * 128);
+                const uint32_t to = ring_at + s * piece_bytes + (lane % UNITS / 8) * (KEYS * 128);
 #pragma unroll
                 for (uint32_t j = 0; j < KEYS / AT_ONCE; ++j) {
                     const uint32_t key = j * AT_ONCE + lane / UNITS;
@@ -590,6 +691,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                                 from + row_bytes(pool, r), r != kNoRow);
                 }
                 copies.push(&full_bar[s]);
+                ++filled;
                 return true;
             };
             Ahead ahead;
@@ -602,7 +704,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 ok = value ? load(mine, a, p.view.v, v_map, v_box, std::integral_constant<uint32_t, PIECE_KEYS> {},
                                   std::integral_constant<uint32_t, D / 8> {}, 0)
                            : load(mine, a, p.view.k, k_map, k_box, std::integral_constant<uint32_t, kKeyTile> {},
-                                  std::integral_constant<uint32_t, 8 * PANELS> {}, mine % PER_TILE * (PANELS * 128));
+                                  std::integral_constant<uint32_t, 8 * PANELS> {}, mine % PER_TILE_K * (PANELS * 128));
                 if (ok && !query) { // behind the first piece, which may find room before the queries do
                     ok = load_query();
                     query = true;
@@ -614,9 +716,12 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
             ++segments;
             next_segment(p, seg, &at, &left);
         }
-        if (FP8 && ok && converted < staged)
-            convert(converted, false);
         copies.drain();
+        if (!ok) { // a wait gave up: boxes that are under way still write to this block's memory
+            volatile uint32_t never = 0;
+            for (uint32_t n = filled - min(filled, slots / warps); n < filled; ++n)
+                mbar_wait(&full_bar[(n * warps + w) % slots], (n * warps + w) / slots & 1, &never, p.err, ERR_PF_FULL_WAIT);
+        }
     } else if (warp >= Shape::kScoreWarp) {
         // ------------------------------------------------------------------------------- products --
         // The whole warp goes through the loops and one lane issues.
@@ -624,11 +729,13 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
         constexpr uint32_t kScores = kFormat | ((STEP >> 3) << 17);
         constexpr uint32_t kSums = kFormat | ((D >> 3) << 17) | (1u << 16);
         constexpr uint64_t kOperand = (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+        constexpr uint64_t kNarrow = (static_cast<uint64_t>(512 >> 4) << 32) | (1ull << 46) | (4ull << 61); // rows of 64 bytes
+        constexpr uint64_t kRow = WIDTH == 64 ? kNarrow : kOperand;
         // V as the B operand with its n side contiguous: panels of 64 elements, keys 128 bytes apart, groups of eight keys 1024
         constexpr uint64_t kValue = kOperand | (static_cast<uint64_t>(PIECE_KEYS * 128 >> 4) << 16);
         const auto uniform = [](uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); };
         const uint32_t ring_lo = uniform(smem_u32(ring) >> 4), query_lo = uniform(smem_u32(smem) >> 4), columns = uniform(tmem);
-        uint32_t before = 0, segments = 0;   // pieces of earlier segments, of K and as many of V
+        uint32_t before = 0, segments = 0;   // key tiles of earlier segments
         uint32_t done[2] = {}, segs[2] = {}; // steps and segments of a query tile
         bool ok = true;
         const auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
@@ -642,21 +749,29 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
             tc_fence_after();
             const uint32_t part = u % STEPS; // of the key tile
 #pragma unroll
-            for (uint32_t i = 0; i < PER_TILE; ++i) {
-                const uint32_t piece = before + u / STEPS * PER_TILE + i, s = piece % SLOTS_K;
+            for (uint32_t i = 0; i < PER_TILE_K; ++i) {
+                const uint32_t piece = (before + u / STEPS) * PER_TILE_K + i, s = piece % SLOTS_K;
                 if (part == 0 && q == 0 && !wait(&bar.k_full[s], (piece / SLOTS_K) & 1, ERR_PF_FULL_WAIT))
                     return false;
-                const uint32_t a_lo = query_lo + (q * (kRowTile * D * 2) + i * (PANELS * kRowTile * 128)) / 16;
-                const uint32_t b_lo = uniform(ring_lo + s * (kPiece / 16) + part * (STEP * 128 / 16));
+                const uint32_t a_lo = query_lo + (q * (kRowTile * D * 2) + i * (PANELS * kRowTile * WIDTH)) / 16;
+                const uint32_t b_lo = uniform(ring_lo + (s * kPieceK + part * (STEP * WIDTH)) / 16);
                 if (elect_one()) {
+                    if constexpr (FP8) {
 #pragma unroll
-                    for (uint32_t j = 0; j < 4 * PANELS; ++j) {
-                        const uint32_t k = j / 4 * (kKeyTile * 128 / 16) + j % 4 * 2; // (query tiles are as high as key tiles)
-                        tc_mma_bf16(d, kOperand | (a_lo + k), kOperand | (b_lo + k), kScores, i > 0 || j > 0);
+                        for (uint32_t j = 0; j < WIDTH / 16; ++j) { // 32 elements each: of the queries' high parts, of the low ones
+                            const uint32_t k = j % (WIDTH / 32) * 2, low = j / (WIDTH / 32) * (kRowTile * D / 16);
+                            tc_mma_f8(d, kRow | (a_lo + low + k), kRow | (b_lo + k), kScores, i > 0 || j > 0);
+                        }
+                    } else {
+#pragma unroll
+                        for (uint32_t j = 0; j < 4 * PANELS; ++j) {
+                            const uint32_t k = j / 4 * (kKeyTile * 128 / 16) + j % 4 * 2; // (query tiles are as high as key tiles)
+                            tc_mma_bf16(d, kOperand | (a_lo + k), kOperand | (b_lo + k), kScores, i > 0 || j > 0);
+                        }
                     }
                     if (last && part + 1 == STEPS)
                         tc_commit(&bar.k_empty[s]);
-                    if (i + 1 == PER_TILE)
+                    if (i + 1 == PER_TILE_K)
                         tc_commit(&bar.s_full[q]);
                 }
             }
@@ -664,8 +779,8 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
             return true;
         };
         // A step's keys are one or more pieces of V, or a part of one.
-        constexpr bool WHOLE = PER_TILE >= STEPS;
-        constexpr uint32_t OF_STEP = WHOLE ? PER_TILE / STEPS : 1;
+        constexpr bool WHOLE = PER_TILE_V >= STEPS;
+        constexpr uint32_t OF_STEP = WHOLE ? PER_TILE_V / STEPS : 1;
         const auto sums = [&](uint32_t u, uint32_t q, bool last) {
             const uint32_t half = done[q] & 1, part = u % STEPS;
             const uint32_t d = columns + q * D, a = columns + 256 + TILES * STEP + (q * 2 + half) * (STEP / 2);
@@ -673,7 +788,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 return false;
 #pragma unroll
             for (uint32_t i = 0; i < OF_STEP; ++i) {
-                const uint32_t piece = before + (WHOLE ? u * OF_STEP + i : u / STEPS), s = piece % SLOTS_V;
+                const uint32_t piece = before * PER_TILE_V + (WHOLE ? u * OF_STEP + i : u / STEPS), s = piece % SLOTS_V;
                 if ((WHOLE || part == 0) && q == 0 && !wait(&bar.v_full[s], (piece / SLOTS_V) & 1, ERR_PF_FULL_WAIT))
                     return false;
                 if (i == 0) {
@@ -681,7 +796,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                         return false;
                     tc_fence_after();
                 }
-                const uint32_t b_lo = uniform(ring_lo + (SLOTS_K + s) * (kPiece / 16) + (WHOLE ? 0 : part * (STEP * 128 / 16)));
+                const uint32_t b_lo = uniform(ring_lo + (Shape::kRingK + s * kPieceV) / 16 + (WHOLE ? 0 : part * (STEP * 128 / 16)));
                 constexpr uint32_t COUNT = STEP / OF_STEP / 16; // products of 16 keys: 2048 bytes of V, eight columns of P
                 if (elect_one()) {
 #pragma unroll
@@ -711,7 +826,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
             ++segs[0];
             segs[1] += second ? 1 : 0;
             ++segments;
-            before += n * PER_TILE;
+            before += n;
             next_segment(p, seg, &at, &left);
         }
         // whatever was issued is complete before the tensor memory goes back
@@ -944,12 +1059,12 @@ template <uint32_t D, bool FP8> cudaError_t launch_prefill_as(const AttnParams& 
         const uint64_t dims[4] = { D, size, p.view.kv_heads, p.view.pages };
         const uint64_t strides[3] = { static_cast<uint64_t>(pool.slot_stride), static_cast<uint64_t>(pool.head_stride),
                                       static_cast<uint64_t>(pool.page_stride) };
-        if (FP8 || rows < 8 || size % rows != 0 || most % rows != 0 || !make_page_map(map, pool.data, dims, strides, rows))
+        if (rows < 8 || size % rows != 0 || most % rows != 0 || !make_page_map(map, FP8, pool.data, dims, strides, Shape::kWidth, rows))
             return 0u;
         return rows;
     };
     CUtensorMap k_map {}, v_map {};
-    const uint32_t k_box = box(&k_map, p.view.k, kKeyTile), v_box = box(&v_map, p.view.v, Shape::kPieceKeys);
+    const uint32_t k_box = box(&k_map, p.view.k, kKeyTile), v_box = FP8 ? 0 : box(&v_map, p.view.v, Shape::kPieceKeys);
     return launch_chained(attn_prefill_kernel<D, FP8>, dim3(p.blocks), Shape::kThreads, Shape::kSmem, stream, p, k_map, v_map, k_box, v_box);
 }
 

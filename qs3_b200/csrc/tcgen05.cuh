@@ -58,9 +58,10 @@ bool make_operand_map(CUtensorMap* map, bool bytes_type, const void* base, uint6
 // Row-major output [rows, cols] written by TMA in boxes of 32 rows x 64 bytes (64-byte swizzle). False: not addressable
 // (TMA clips a row in units of 16 bytes: columns that end inside one would write past it).
 bool make_output_map(CUtensorMap* map, bool f32, void* out, uint64_t cols, uint64_t rows, uint64_t pitch_elems);
-// bf16 pool of pages: {head_dim, page_size, kv_heads, pages} elements, strides of the last three in bytes; boxes of 64 elements x
-// box_rows slots of one head and page, 128-byte swizzle.
-bool make_page_map(CUtensorMap* map, const void* base, const uint64_t* dims, const uint64_t* strides, uint32_t box_rows);
+// Pool of pages: {head_dim, page_size, kv_heads, pages} elements of bf16 or bytes, strides of the last three in bytes; boxes of
+// box_bytes (64 or 128, which is the swizzle too) x box_rows slots of one head and page.
+bool make_page_map(CUtensorMap* map, bool bytes_type, const void* base, const uint64_t* dims, const uint64_t* strides, uint32_t box_bytes,
+                   uint32_t box_rows);
 namespace tc {
 
 // ---- PTX wrappers -------------------------------------------------------------------
