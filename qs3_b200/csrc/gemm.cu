@@ -884,7 +884,7 @@ bool make_output_map(CUtensorMap* map, bool f32, void* out, uint64_t cols, uint6
 }
 
 bool make_page_map(CUtensorMap* map, bool bytes_type, const void* base, const uint64_t* dims, const uint64_t* strides, uint32_t box_bytes,
-                   uint32_t box_rows)
+                   uint32_t box_rows, bool swizzle)
 {
     EncodeTiledFn fn = encode_tiled_fn();
     if (fn == nullptr || !aligned16(base))
@@ -895,7 +895,10 @@ bool make_page_map(CUtensorMap* map, bool bytes_type, const void* base, const ui
     const cuuint32_t estr[4] = { 1, 1, 1, 1 };
     const CUtensorMapDataType type = bytes_type ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     return fn(map, type, 4, const_cast<void*>(base), d, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              !swizzle          ? CU_TENSOR_MAP_SWIZZLE_NONE
+                  : box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                    : CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
         == CUDA_SUCCESS;
 }

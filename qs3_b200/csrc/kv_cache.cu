@@ -584,7 +584,8 @@ bool rows_fit(const PagedView& v)
 {
     for (const PagedPool* p : { &v.k, &v.v })
         if (((v.pages - 1) * static_cast<uint64_t>(p->page_stride) + (v.page_size - 1) * static_cast<uint64_t>(p->slot_stride)) >> p->unit_shift
-            >= 0xffffffffu)
+                >= 0xffffffffu
+            || (v.pages > 1 && p->scale_page_stride >> 30 != 0) || (v.page_size > 1 && p->scale_slot_stride >> 30 != 0))
             return false;
     return true;
 }
@@ -650,10 +651,14 @@ qsfi_status paged_view(qsfi_context* ctx, const qs3_paged_kv_cache& cache, const
         while (p.unit_shift < 20 && (p.page_stride | p.slot_stride) % (int64_t { 2 } << p.unit_shift) == 0)
             ++p.unit_shift;
         p.unit = 1u << p.unit_shift;
+        p.page_units = static_cast<uint32_t>(p.page_stride >> p.unit_shift);
+        p.slot_units = static_cast<uint32_t>(p.slot_stride >> p.unit_shift);
         p.scale = static_cast<float*>(scale.data);
         p.scale_page_stride = scale.stride[0];
         p.scale_head_stride = scale.stride[1];
         p.scale_slot_stride = scale.stride[2];
+        p.scale_page = static_cast<uint32_t>(scale.stride[0] * 4);
+        p.scale_slot = static_cast<uint32_t>(scale.stride[2] * 4);
         return p;
     };
     v.k = pool(cache.k, cache.k_scale);

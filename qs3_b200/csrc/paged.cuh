@@ -17,8 +17,10 @@ struct PagedPool {
     uint8_t* data;
     int64_t page_stride, head_stride, slot_stride;
     uint32_t unit, unit_shift; // power of two that divides page_stride and slot_stride
+    uint32_t page_units, slot_units;
     float* scale;
     int64_t scale_page_stride, scale_head_stride, scale_slot_stride;
+    uint32_t scale_page, scale_slot; // the same in bytes, for reads (rows_fit)
 };
 
 struct PagedView {
@@ -75,11 +77,18 @@ __device__ __forceinline__ int32_t page_of(const PagedView& p, const SeqPages& s
 constexpr uint32_t kNoRow = 0xffffffffu;
 __device__ __forceinline__ uint32_t row_units(const PagedPool& pool, int32_t page, uint32_t slot)
 {
-    return page < 0 ? kNoRow : static_cast<uint32_t>((page * pool.page_stride + slot * pool.slot_stride) >> pool.unit_shift);
+    return page < 0 ? kNoRow : page * pool.page_units + slot * pool.slot_units;
 }
 __device__ __forceinline__ uint64_t row_bytes(const PagedPool& pool, uint32_t row)
 {
     return static_cast<uint64_t>(row == kNoRow ? 0 : row) * pool.unit;
+}
+
+// Scale of a token, from that of the first page's first one of the head on.
+__device__ __forceinline__ const float* scale_at(const PagedPool& pool, const uint8_t* head, int32_t page, uint32_t slot)
+{
+    return reinterpret_cast<const float*>(head + static_cast<uint64_t>(static_cast<uint32_t>(page)) * pool.scale_page
+                                          + static_cast<uint64_t>(slot) * pool.scale_slot);
 }
 
 // Largest i in [0, n) with table[i] <= x, for ascending table[0 .. n] with table[0] <= x; the whole warp searches, 32 places

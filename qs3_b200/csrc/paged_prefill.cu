@@ -26,8 +26,10 @@
 // bits exactly, and no element is off by more than 2^-17 of the largest. Two products of twice the rate take the time of one.
 // K's scales are a factor on the scores. V's are part of the weights, w = exp2(s + log2(scale) - m), of which the largest is again
 // at a known place; a second e4m3 number would keep 8 bits of a weight but only 14 of the range below the largest, which many
-// small weights together need, so the weights are f16 and V is converted, by the five warps that fetch it: from memory to
-// registers, half a piece while the other half is converted, and on to the ring. The row's sum takes V's scale out again.
+// small weights together need, so the weights are f16 and V is converted, by the four warps that fetch it: boxes to a staging
+// area, from there to registers, which makes room for the next ones, and to the ring. (Loads straight to registers filled what
+// the first-level cache has left beside so much shared memory, and everyone's loads waited: 765 us, not PLACE.) The row's sum
+// takes V's scale out again.
 // (All converted to f16, K too, by way of a staging area: 1021 tokens behind 31 111 cached ones 965 us.)
 #include "paged_attention.cuh"
 #include "tcgen05.cuh"
@@ -67,7 +69,7 @@ enum : uint32_t {
 
 struct Barriers {
     uint64_t k_full[kMostSlots], k_empty[kMostSlots], v_full[kMostSlots], v_empty[kMostSlots];
-    uint64_t scale_full[kScaleTiles];
+    uint64_t scale_full[kScaleTiles], staged[4];
     uint64_t q_full, q_free;
     uint64_t s_full[2], s_free[2], o_free[2]; // of a query tile
     uint64_t p_full[2][2], pv_done[2][2];     // of its tiles of weights
@@ -84,10 +86,12 @@ template <uint32_t D, bool FP8> struct PrefillShape {
     static constexpr uint32_t kRows = kTiles * kRowTile;
     static constexpr uint32_t kWidth = FP8 && D == 64 ? 64 : 128; // bytes of a row in a panel of K, and of Q
     static constexpr uint32_t kPieceK = FP8 ? kKeyTile * kWidth : D == 64 ? 16384 : 32768, kPieceV = D == 64 || FP8 ? 16384 : 32768;
-    static constexpr uint32_t kWarpsK = FP8 ? 1 : 3, kWarpsV = FP8 ? 5 : 2, kLoadWarps = kWarpsK + kWarpsV;
+    static constexpr uint32_t kWarpsK = FP8 ? 1 : 3, kWarpsV = FP8 ? 4 : 2, kScaleWarps = FP8 ? 1 : 0;
+    static constexpr uint32_t kLoadWarps = kWarpsK + kWarpsV + kScaleWarps;
     static constexpr uint32_t kQueryWarps = FP8 ? kWarpsV : kWarpsK; // load the queries too
-    // of the rings; e4m3: K of two tiles, which is also what the ring of scales relies on
-    static constexpr uint32_t kSlotsK = FP8 ? (D == 256 ? 4 : 2) : D == 64 ? 6 : 3, kSlotsV = FP8 ? 5 : D == 64 ? 4 : 2;
+    // of the rings
+    static constexpr uint32_t kSlotsK = FP8 ? (D == 256 ? 3 : 2) : D == 64 ? 6 : 3, kSlotsV = FP8 || D == 64 ? 4 : 2;
+    static constexpr uint32_t kStage = FP8 ? kPieceV / 2 : 0; // codes of a piece of V, for each warp that fetches them
     static constexpr uint32_t kScales = FP8 ? kScaleTiles * kKeyTile * 3 * 4 : 0;
     static constexpr uint32_t kQueryScales = FP8 ? 2 * kRows * 4 : 0;
     static constexpr uint32_t kPanels = kPieceK / (kKeyTile * kWidth); // of a piece of K
@@ -98,12 +102,11 @@ template <uint32_t D, bool FP8> struct PrefillShape {
     static constexpr uint32_t kScoreWarp = kSoftmaxWarps + kLoadWarps;
     static constexpr uint32_t kThreads = (kSoftmaxWarps + kLoadWarps + 2) * 32;
     static constexpr uint32_t kRingK = kSlotsK * kPieceK, kRing = kRingK + kSlotsV * kPieceV;
-    static constexpr uint32_t kSmem = 1024 + kQ + kRing + kScales + kQueryScales + sizeof(Barriers);
+    static constexpr uint32_t kSmem = 1024 + kQ + kRing + kWarpsV * kStage + kScales + kQueryScales + sizeof(Barriers);
     static_assert(kSlotsK % kWarpsK == 0 && kSlotsV % kWarpsV == 0, "a slot is one warp's");
     static_assert(kSmem <= 227 * 1024, "shared memory of a block");
     static_assert(kRing >= kMaxBatch * 8, "the search for the block's range uses the ring");
     static_assert(kSlotsK <= kMostSlots && kSlotsV <= kMostSlots, "barriers of the slots");
-    static_assert(!FP8 || kSlotsK == 2 * kPerTileK, "K of two tiles");
     static_assert(kThreads <= 512, "128 registers for each");
 };
 
@@ -184,10 +187,18 @@ __device__ __forceinline__ float2 f16x2_to_f32(uint32_t x)
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(r.x), "=f"(r.y) : "r"(x));
     return r;
 }
-__device__ __forceinline__ uint4 load_codes(const uint8_t* p)
+__device__ __forceinline__ float load_scale(const float* p, bool there)
 {
-    uint4 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    float r;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.f32 %0, 0f00000000;\n\t@p ld.global.nc.f32 %0, [%1];\n\t}"
+                 : "=&f"(r)
+                 : "l"(p), "r"(static_cast<uint32_t>(there)));
+    return r;
+}
+__device__ __forceinline__ float log2_approx(float x)
+{
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
@@ -279,9 +290,10 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* const ring = smem + Shape::kQ;
-    float* const scales = reinterpret_cast<float*>(ring + Shape::kRing); // of a tile's key pairs: K's, log2 of V's; then 1 / V's
+    uint8_t* const staging = ring + Shape::kRing;
+    float* const scales = reinterpret_cast<float*>(staging + kWarpsV * Shape::kStage); // of a tile's key pairs: K's, log2 of V's; then 1 / V's
     float* const q_scales = scales + Shape::kScales / 4; // what the rows of queries were divided by, of this segment and the next
-    Barriers& bar = *reinterpret_cast<Barriers*>(ring + Shape::kRing + Shape::kScales + Shape::kQueryScales);
+    Barriers& bar = *reinterpret_cast<Barriers*>(staging + kWarpsV * Shape::kStage + Shape::kScales + Shape::kQueryScales);
     const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
 
     if (tid == 0) {
@@ -293,6 +305,8 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
         }
         for (uint32_t i = 0; i < kScaleTiles; ++i)
             mbar_init(&bar.scale_full[i], 1);
+        for (uint32_t i = 0; i < 4; ++i)
+            mbar_init(&bar.staged[i], 1);
         mbar_init(&bar.q_full, Shape::kQueryWarps);
         mbar_init(&bar.q_free, 1);
         for (uint32_t i = 0; i < 2; ++i) {
@@ -333,8 +347,9 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
 
     if (warp >= Shape::kLoadWarp && warp < Shape::kScoreWarp) {
         // ------------------------------------------------------------------------------ fetching --
-        const bool value = warp - Shape::kLoadWarp >= kWarpsK; // fetches V
-        const uint32_t w = value ? warp - Shape::kLoadWarp - kWarpsK : warp - Shape::kLoadWarp, warps = value ? kWarpsV : kWarpsK;
+        const uint32_t role = warp - Shape::kLoadWarp;
+        const bool value = role >= kWarpsK && role < kWarpsK + kWarpsV, scaling = role >= kWarpsK + kWarpsV; // fetches V, the scales
+        const uint32_t w = value ? role - kWarpsK : scaling ? 0 : role, warps = value ? kWarpsV : kWarpsK;
         const uint32_t slots = value ? SLOTS_V : SLOTS_K, piece_bytes = value ? kPieceV : kPieceK;
         uint64_t* const full_bar = value ? bar.v_full : bar.k_full;
         uint64_t* const empty_bar = value ? bar.v_empty : bar.k_empty;
@@ -343,6 +358,8 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
         uint32_t before = 0, segments = 0; // pieces of earlier segments
         uint32_t filled = 0;               // this warp's pieces so far, the n-th of them being number n * warps + w of all
         bool ok = true;
+        bool boxed = false;                // e4m3: boxes are under way to this warp's staging area
+        uint32_t staged_phase = 0;
         const auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
             if (__all_sync(0xffffffffu, mbar_test_wait(b, parity)))
                 return true;
@@ -424,22 +441,26 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
 
             const uint32_t pieces = seg.count * (value ? PER_TILE_V : PER_TILE_K);
             uint32_t mine = (w + warps - before % warps) % warps; // the first that goes to one of this warp's slots
-            bool query = value; // loaded, or not this warp's business
+            bool query = FP8 || value; // loaded, or not this warp's business
             if (FP8 && value) {
-                // ---- V: codes to registers, from there in f16 to the ring; two halves of a piece in turn
-                constexpr uint32_t UNITS = D / 16, AT_ONCE = 32 / UNITS, SETS = PIECE_KEYS / 32, LOADS = PIECE_KEYS / AT_ONCE, HALF = LOADS / 2;
-                struct Places { // of keys lane + 32 j of a piece
-                    int32_t page[SETS];
+                // ---- V: codes to a staging area, from there to registers, and in f16 to the ring
+                constexpr uint32_t UNITS = D / 16, AT_ONCE = 32 / UNITS, SETS = PIECE_KEYS / 32, LOADS = PIECE_KEYS / AT_ONCE;
+                struct Places {
+                    int32_t page[SETS]; // of keys lane + 32 j, or of the lane's box; not looked at yet
                     uint32_t slot[SETS];
+                    bool boxes; // whole boxes of cached tokens
                 };
-                const auto look = [&](uint32_t piece) { // (pages are not looked at yet: their loads may take their time)
+                const auto first_key = [&](uint32_t piece) { return seg.tile0 * kKeyTile + piece * PIECE_KEYS; };
+                const auto look = [&](uint32_t piece) {
                     Places l;
+                    const uint32_t key0 = first_key(piece);
+                    l.boxes = v_box != 0 && key0 >= seen_lo && key0 + PIECE_KEYS <= seg.pages.length;
 #pragma unroll
                     for (uint32_t j = 0; j < SETS; ++j) {
-                        const uint32_t key = seg.tile0 * kKeyTile + piece * PIECE_KEYS + j * 32 + lane;
+                        const uint32_t key = key0 + (l.boxes ? lane * v_box : j * 32 + lane);
                         l.page[j] = -1;
                         l.slot[j] = 0;
-                        if (key >= seen_lo && key < seen_hi) {
+                        if (l.boxes ? j == 0 && lane * v_box < PIECE_KEYS : key >= seen_lo && key < seen_hi) {
                             const uint32_t i = p.view.page_div.div(key);
                             l.slot[j] = key - i * p.view.page_size;
                             l.page[j] = __ldg(p.view.indices + seg.pages.first + i);
@@ -447,35 +468,78 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     }
                     return l;
                 };
-                uint32_t row[SETS];
-                const auto rows = [&](uint32_t piece, Places l) {
+                uint8_t* const stage = staging + w * Shape::kStage;
+                const auto fetch = [&](uint32_t piece, Places l) {
+                    const uint32_t key0 = first_key(piece), stage_at = smem_u32(stage);
+                    if (l.boxes) {
+                        const bool mine = lane * v_box < PIECE_KEYS, bad = mine && static_cast<uint32_t>(l.page[0]) >= p.view.pages;
+                        boxed = !__any_sync(0xffffffffu, bad);
+                        if (boxed) {
+                            if (lane == 0)
+                                mbar_expect_tx(&bar.staged[w], Shape::kStage);
+                            __syncwarp();
+                            if (mine)
+                                tma_load_page(stage_at + lane * v_box * D, &v_map, &bar.staged[w], 0, static_cast<int>(l.slot[0]),
+                                              static_cast<int>(at.head), l.page[0]);
+                            return;
+                        }
+                    }
+                    uint32_t row[SETS];
 #pragma unroll
                     for (uint32_t j = 0; j < SETS; ++j) {
+                        const uint32_t key = key0 + j * 32 + lane;
+                        const bool seen = key >= seen_lo && key < seen_hi;
+                        if (l.boxes) // one of the boxes' pages is not there
+                            l.page[j] = seen ? page_of(p.view, seg.pages, key, &l.slot[j]) : -1;
                         const bool there = static_cast<uint32_t>(l.page[j]) < p.view.pages;
-                        const uint32_t key = seg.tile0 * kKeyTile + piece * PIECE_KEYS + j * 32 + lane;
-                        if (!there && key >= seen_lo && key < seen_hi)
+                        if (seen && !there)
                             atomicCAS(p.err, 0u, static_cast<uint32_t>(ERR_PAGE_TABLE));
                         row[j] = row_units(p.view.v, there ? l.page[j] : -1, l.slot[j]);
                     }
-                };
-                const uint8_t* const from = p.view.v.data + at.head * p.view.v.head_stride + (lane % UNITS) * 16;
-                uint4 codes[2][HALF];
-                const auto fetch = [&](auto which) {
-                    constexpr uint32_t H = decltype(which)::value;
-                    __syncwarp();
+                    const uint8_t* const from = p.view.v.data + at.head * p.view.v.head_stride + (lane % UNITS) * 16;
 #pragma unroll
-                    for (uint32_t j = 0; j < HALF; ++j) {
-                        const uint32_t i = H * HALF + j;
-                        const uint32_t r = __shfl_sync(0xffffffffu, row[i * AT_ONCE / 32], (i * AT_ONCE + lane / UNITS) & 31);
-                        codes[H][j] = r == kNoRow ? make_uint4(0, 0, 0, 0) : load_codes(from + row_bytes(p.view.v, r));
+                    for (uint32_t j = 0; j < LOADS; ++j) {
+                        const uint32_t r = __shfl_sync(0xffffffffu, row[j * AT_ONCE / 32], (j * AT_ONCE + lane / UNITS) & 31);
+                        cp_async16z(stage_at + (j * 32 + lane) * 16, from + row_bytes(p.view.v, r), r != kNoRow);
                     }
                 };
-                const auto convert = [&](auto which, uint8_t* to) {
-                    constexpr uint32_t H = decltype(which)::value;
+                Places ahead;
+                if (mine < pieces) {
+                    fetch(mine, look(mine));
+                    if (mine + kWarpsV < pieces)
+                        ahead = look(mine + kWarpsV);
+                }
+                ok = load_query();
+                for (; ok && mine < pieces; mine += kWarpsV) {
+                    if (boxed) {
+                        ok = wait(&bar.staged[w], staged_phase, ERR_PF_FULL_WAIT);
+                        if (!ok)
+                            break;
+                        staged_phase ^= 1;
+                        boxed = false;
+                    } else {
+                        asm volatile("cp.async.wait_all;" ::: "memory"); // (a lane reads what it copied)
+                    }
+                    uint4 codes[LOADS];
 #pragma unroll
-                    for (uint32_t j = 0; j < HALF; ++j) {
-                        const uint32_t key = (H * HALF + j) * AT_ONCE + lane / UNITS, first = lane % 4 * 2;
-                        const uint32_t x[4] = { codes[H][j].x, codes[H][j].y, codes[H][j].z, codes[H][j].w };
+                    for (uint32_t j = 0; j < LOADS; ++j)
+                        codes[j] = *reinterpret_cast<const uint4*>(stage + (j * 32 + lane) * 16);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // before boxes overwrite them
+                    __syncwarp();
+                    if (mine + kWarpsV < pieces) {
+                        fetch(mine + kWarpsV, ahead);
+                        if (mine + 2 * kWarpsV < pieces)
+                            ahead = look(mine + 2 * kWarpsV);
+                    }
+                    const uint32_t s = (before + mine) % SLOTS_V;
+                    ok = wait(&empty_bar[s], (((before + mine) / SLOTS_V) & 1) ^ 1, ERR_PF_EMPTY_WAIT);
+                    if (!ok)
+                        break;
+                    uint8_t* const to = ring + Shape::kRingK + s * kPieceV + lane % UNITS / 4 * (PIECE_KEYS * 128);
+#pragma unroll
+                    for (uint32_t j = 0; j < LOADS; ++j) {
+                        const uint32_t key = j * AT_ONCE + lane / UNITS, first = lane % 4 * 2;
+                        const uint32_t x[4] = { codes[j].x, codes[j].y, codes[j].z, codes[j].w };
                         uint32_t y[8];
 #pragma unroll
                         for (uint32_t k = 0; k < 8; ++k)
@@ -483,31 +547,6 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                         *reinterpret_cast<uint4*>(to + key * 128 + ((first ^ (key & 7)) * 16)) = make_uint4(y[0], y[1], y[2], y[3]);
                         *reinterpret_cast<uint4*>(to + key * 128 + (((first + 1) ^ (key & 7)) * 16)) = make_uint4(y[4], y[5], y[6], y[7]);
                     }
-                };
-                constexpr std::integral_constant<uint32_t, 0> kFirst {};
-                constexpr std::integral_constant<uint32_t, 1> kSecond {};
-                if (mine < pieces) {
-                    rows(mine, look(mine));
-                    fetch(kFirst);
-                }
-                ok = load_query();
-                for (; ok && mine < pieces; mine += kWarpsV) {
-                    const bool more = mine + kWarpsV < pieces;
-                    Places ahead;
-                    if (more)
-                        ahead = look(mine + kWarpsV);
-                    fetch(kSecond);
-                    const uint32_t s = (before + mine) % SLOTS_V;
-                    ok = wait(&empty_bar[s], (((before + mine) / SLOTS_V) & 1) ^ 1, ERR_PF_EMPTY_WAIT);
-                    if (!ok)
-                        break;
-                    uint8_t* const to = ring + Shape::kRingK + s * kPieceV + lane % UNITS / 4 * (PIECE_KEYS * 128);
-                    convert(kFirst, to);
-                    if (more) {
-                        rows(mine + kWarpsV, ahead);
-                        fetch(kFirst);
-                    }
-                    convert(kSecond, to);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the tensor core reads what was written here
                     __syncwarp();
                     if (lane == 0)
@@ -518,23 +557,25 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 next_segment(p, seg, &at, &left);
                 continue;
             }
-            if constexpr (FP8) {
-                // ---- K as it is, a tile at a time, and the scales of both
-                struct Tile { // pages and slots of keys lane + 32 j; not looked at yet
+            if (FP8 && scaling) {
+                // ---- scales of K and V; pages of a tile are looked up two tiles ahead, its scales one
+                struct Tile { // of keys lane + 32 j
                     int32_t page[kKeyTile / 32];
                     uint32_t slot[kKeyTile / 32];
-                    bool boxes; // whole boxes of cached tokens
+                    float k[kKeyTile / 32], v[kKeyTile / 32];
+                };
+                const auto seen = [&](uint32_t tile, uint32_t j) {
+                    const uint32_t key = (seg.tile0 + tile) * kKeyTile + j * 32 + lane;
+                    return key >= seen_lo && key < seen_hi;
                 };
                 const auto look = [&](uint32_t tile) {
                     Tile t;
-                    const uint32_t key0 = (seg.tile0 + tile) * kKeyTile;
-                    t.boxes = k_box != 0 && key0 >= seen_lo && key0 + kKeyTile <= seg.pages.length;
 #pragma unroll
                     for (uint32_t j = 0; j < kKeyTile / 32; ++j) {
-                        const uint32_t key = key0 + j * 32 + lane;
+                        const uint32_t key = (seg.tile0 + tile) * kKeyTile + j * 32 + lane;
                         t.page[j] = -1;
                         t.slot[j] = 0;
-                        if (t.boxes || (key >= seen_lo && key < seen_hi)) {
+                        if (seen(tile, j)) {
                             const uint32_t i = p.view.page_div.div(key);
                             t.slot[j] = key - i * p.view.page_size;
                             t.page[j] = __ldg(p.view.indices + seg.pages.first + i);
@@ -542,90 +583,52 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     }
                     return t;
                 };
-                Tile ahead = look(0);
-                for (uint32_t tile = 0; ok && tile < seg.count; ++tile) {
-                    Tile t = ahead;
-                    if (tile + 1 < seg.count)
-                        ahead = look(tile + 1);
-                    const uint32_t key0 = (seg.tile0 + tile) * kKeyTile;
-                    float scale[2][kKeyTile / 32];
-                    uint32_t row[kKeyTile / 32];
-                    bool bad = false;
+                const uint8_t* const k_scale = reinterpret_cast<const uint8_t*>(p.view.k.scale + at.head * p.view.k.scale_head_stride);
+                const uint8_t* const v_scale = reinterpret_cast<const uint8_t*>(p.view.v.scale + at.head * p.view.v.scale_head_stride);
+                const auto load_scales = [&](Tile& t) { // (who fetches the rows reports a page that is not there)
 #pragma unroll
                     for (uint32_t j = 0; j < kKeyTile / 32; ++j) {
-                        const uint32_t key = key0 + j * 32 + lane;
                         const bool there = static_cast<uint32_t>(t.page[j]) < p.view.pages;
-                        bad |= !there && (t.boxes || (key >= seen_lo && key < seen_hi));
-                        t.page[j] = there ? t.page[j] : -1;
-                        row[j] = row_units(p.view.k, t.page[j], t.slot[j]);
-#pragma unroll
-                        for (uint32_t v = 0; v < 2; ++v) {
-                            const PagedPool& of = v ? p.view.v : p.view.k;
-                            scale[v][j] = there
-                                ? __ldg(of.scale + at.head * of.scale_head_stride + t.page[j] * of.scale_page_stride + t.slot[j] * of.scale_slot_stride)
-                                : 0.0f;
-                        }
+                        t.k[j] = load_scale(scale_at(p.view.k, k_scale, t.page[j], t.slot[j]), there);
+                        t.v[j] = load_scale(scale_at(p.view.v, v_scale, t.page[j], t.slot[j]), there);
                     }
-                    if (bad)
-                        atomicCAS(p.err, 0u, static_cast<uint32_t>(ERR_PAGE_TABLE));
-                    const bool boxes = t.boxes && !__any_sync(0xffffffffu, bad);
-                    // lane i has box i, which begins with key i * k_box
-                    int32_t page = 0;
-                    uint32_t slot = 0;
-                    if (boxes)
-#pragma unroll
-                        for (uint32_t j = 0; j < kKeyTile / 32; ++j) {
-                            const int32_t box_page = __shfl_sync(0xffffffffu, t.page[j], lane * k_box & 31);
-                            const uint32_t box_slot = __shfl_sync(0xffffffffu, t.slot[j], lane * k_box & 31);
-                            if (lane * k_box / 32 == j)
-                                page = box_page, slot = box_slot;
-                        }
-#pragma unroll
-                    for (uint32_t panel = 0; panel < PER_TILE_K; ++panel) {
-                        const uint32_t piece = before + tile * PER_TILE_K + panel, s = piece % SLOTS_K;
-                        ok = wait(&empty_bar[s], ((piece / SLOTS_K) & 1) ^ 1, ERR_PF_EMPTY_WAIT);
+                };
+                Tile next = look(0), after = next;
+                if (seg.count > 1)
+                    after = look(1);
+                load_scales(next);
+                for (uint32_t tile = 0; ok && tile < seg.count; ++tile) {
+                    const Tile t = next;
+                    next = after;
+                    if (tile + 2 < seg.count)
+                        after = look(tile + 2);
+                    if (tile + 1 < seg.count)
+                        load_scales(next);
+                    // The place is free when the weights of four tiles ago are written. Those of the first query tile two steps
+                    // before this tile's first stand for that: the second one's scores of the step before had been asked for by
+                    // then, and its scores of the step before that one been read. The weights of this barrier's next phase need
+                    // these scales, so the parity stands for the phase that is meant.
+                    const uint32_t number = before + tile, place = number % kScaleTiles;
+                    if (number * STEPS >= 2) {
+                        const uint32_t step = number * STEPS - 2;
+                        ok = wait(&bar.p_full[0][step & 1], (step >> 1) & 1, ERR_PF_WEIGHT_WAIT);
                         if (!ok)
                             break;
-                        const uint32_t to = ring_at + s * kPieceK;
-                        if (boxes) {
-                            if (lane == 0)
-                                mbar_expect_tx(&full_bar[s], kPieceK);
-                            __syncwarp();
-                            if (lane * k_box < kKeyTile)
-                                tma_load_page(to + lane * k_box * WIDTH, &k_map, &full_bar[s], static_cast<int>(panel * WIDTH), static_cast<int>(slot),
-                                              static_cast<int>(at.head), page);
-                        } else {
-                            constexpr uint32_t UNITS = WIDTH / 16, AT_ONCE = 32 / UNITS;
-                            const uint8_t* const from = p.view.k.data + at.head * p.view.k.head_stride + panel * WIDTH + (lane % UNITS) * 16;
-#pragma unroll
-                            for (uint32_t j = 0; j < kKeyTile / AT_ONCE; ++j) {
-                                const uint32_t key = j * AT_ONCE + lane / UNITS;
-                                const uint32_t r = __shfl_sync(0xffffffffu, row[j * AT_ONCE / 32], key & 31);
-                                cp_async16z(to + key * WIDTH + ((lane % UNITS ^ swizzle_of<WIDTH>(key)) * 16), from + row_bytes(p.view.k, r), r != kNoRow);
-                            }
-                            copies.push(&full_bar[s]);
-                        }
-                        ++filled;
                     }
-                    if (!ok)
-                        break;
-                    // These need no barrier for their way back: K of this tile has found room, so the scores of two tiles ago are
-                    // through, and those of three ago have been read, by warps that were done with the scales of four ago.
-                    const uint32_t place = (before / PER_TILE_K + tile) % kScaleTiles;
                     float* const out = scales + place * (kKeyTile * 3);
 #pragma unroll
                     for (uint32_t j = 0; j < kKeyTile / 32; ++j) {
                         const uint32_t key = j * 32 + lane;
-                        const float v = scale[1][j] < 1.0e-30f ? 1.0e-30f : scale[1][j]; // (a NaN stays one)
-                        out[key / 2 * 4 + (key & 1)] = scale[0][j] * p.scale_log2;
-                        out[key / 2 * 4 + 2 + (key & 1)] = log2f(v);
-                        out[kKeyTile * 2 + key] = kSumFactor<FP8> / v;
+                        const float v = t.v[j] < 1.0e-30f ? 1.0e-30f : t.v[j]; // (a NaN stays one)
+                        out[key / 2 * 4 + (key & 1)] = t.k[j] * p.scale_log2;
+                        out[key / 2 * 4 + 2 + (key & 1)] = log2_approx(v);
+                        out[kKeyTile * 2 + key] = __fdividef(kSumFactor<FP8>, v);
                     }
                     __syncwarp();
                     if (lane == 0)
                         mbar_arrive(&bar.scale_full[place]);
                 }
-                before += pieces;
+                before += seg.count;
                 ++segments;
                 next_segment(p, seg, &at, &left);
                 continue;
@@ -673,10 +676,10 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     if (lane == 0)
                         mbar_expect_tx(&full_bar[s], piece_bytes);
                     __syncwarp();
-                    if (lane < per_panel * (UNITS / 8)) {
+                    if (lane < per_panel * ((UNITS + 7) / 8)) {
                         const uint32_t panel = lane / per_panel, first = (lane - panel * per_panel) * box;
-                        tma_load_page(ring_at + s * piece_bytes + panel * (KEYS * 128) + first * 128, &map, &full_bar[s],
-                                      static_cast<int>(skip / 2 + panel * 64), static_cast<int>(a.slot), static_cast<int>(at.head), a.page);
+                        tma_load_page(ring_at + s * piece_bytes + panel * (KEYS * 128) + first * WIDTH, &map, &full_bar[s],
+                                      static_cast<int>(skip / (FP8 ? 1 : 2) + panel * 64), static_cast<int>(a.slot), static_cast<int>(at.head), a.page);
                     }
                     ++filled;
                     return true;
@@ -687,7 +690,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 for (uint32_t j = 0; j < KEYS / AT_ONCE; ++j) {
                     const uint32_t key = j * AT_ONCE + lane / UNITS;
                     const uint32_t r = __shfl_sync(0xffffffffu, row[j * AT_ONCE / 32], key & 31);
-                    cp_async16z(to + key * 128 + (((lane & 7) ^ (key & 7)) * 16),
+                    cp_async16z(to + key * WIDTH + ((lane % (WIDTH / 16) ^ swizzle_of<WIDTH>(key)) * 16),
                                 from + row_bytes(pool, r), r != kNoRow);
                 }
                 copies.push(&full_bar[s]);
@@ -701,10 +704,10 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 const Ahead a = ahead;
                 if (mine + warps < pieces)
                     ahead = look(mine + warps);
-                ok = value ? load(mine, a, p.view.v, v_map, v_box, std::integral_constant<uint32_t, PIECE_KEYS> {},
+                ok = !FP8 && value ? load(mine, a, p.view.v, v_map, v_box, std::integral_constant<uint32_t, PIECE_KEYS> {},
                                   std::integral_constant<uint32_t, D / 8> {}, 0)
                            : load(mine, a, p.view.k, k_map, k_box, std::integral_constant<uint32_t, kKeyTile> {},
-                                  std::integral_constant<uint32_t, 8 * PANELS> {}, mine % PER_TILE_K * (PANELS * 128));
+                                  std::integral_constant<uint32_t, WIDTH / 16 * PANELS> {}, mine % PER_TILE_K * (PANELS * WIDTH));
                 if (ok && !query) { // behind the first piece, which may find room before the queries do
                     ok = load_query();
                     query = true;
@@ -719,6 +722,8 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
         copies.drain();
         if (!ok) { // a wait gave up: boxes that are under way still write to this block's memory
             volatile uint32_t never = 0;
+            if (boxed)
+                mbar_wait(&bar.staged[w], staged_phase, &never, p.err, ERR_PF_FULL_WAIT);
             for (uint32_t n = filled - min(filled, slots / warps); n < filled; ++n)
                 mbar_wait(&full_bar[(n * warps + w) % slots], (n * warps + w) / slots & 1, &never, p.err, ERR_PF_FULL_WAIT);
         }
@@ -1053,18 +1058,19 @@ template <uint32_t D, bool FP8> cudaError_t launch_prefill_as(const AttnParams& 
     if (err != cudaSuccess)
         return err;
     // Pages that a box fits into a whole number of times are fetched by TMA, others and the ends of sequences row by row.
-    const auto box = [&](CUtensorMap* map, const PagedPool& pool, uint32_t most) {
+    const auto box = [&](CUtensorMap* map, const PagedPool& pool, uint32_t most, uint32_t bytes, bool swizzle) {
         const uint32_t size = p.view.page_size;
         const uint32_t rows = size < most ? size : most;
         const uint64_t dims[4] = { D, size, p.view.kv_heads, p.view.pages };
         const uint64_t strides[3] = { static_cast<uint64_t>(pool.slot_stride), static_cast<uint64_t>(pool.head_stride),
                                       static_cast<uint64_t>(pool.page_stride) };
-        if (rows < 8 || size % rows != 0 || most % rows != 0 || !make_page_map(map, FP8, pool.data, dims, strides, Shape::kWidth, rows))
+        if (rows < 8 || size % rows != 0 || most % rows != 0 || !make_page_map(map, FP8, pool.data, dims, strides, bytes, rows, swizzle))
             return 0u;
         return rows;
     };
     CUtensorMap k_map {}, v_map {};
-    const uint32_t k_box = box(&k_map, p.view.k, kKeyTile), v_box = FP8 ? 0 : box(&v_map, p.view.v, Shape::kPieceKeys);
+    const uint32_t k_box = box(&k_map, p.view.k, kKeyTile, Shape::kWidth, true);
+    const uint32_t v_box = box(&v_map, p.view.v, Shape::kPieceKeys, FP8 ? D : 128, !FP8);
     return launch_chained(attn_prefill_kernel<D, FP8>, dim3(p.blocks), Shape::kThreads, Shape::kSmem, stream, p, k_map, v_map, k_box, v_box);
 }
 

@@ -59,9 +59,9 @@ bool make_operand_map(CUtensorMap* map, bool bytes_type, const void* base, uint6
 // (TMA clips a row in units of 16 bytes: columns that end inside one would write past it).
 bool make_output_map(CUtensorMap* map, bool f32, void* out, uint64_t cols, uint64_t rows, uint64_t pitch_elems);
 // Pool of pages: {head_dim, page_size, kv_heads, pages} elements of bf16 or bytes, strides of the last three in bytes; boxes of
-// box_bytes (64 or 128, which is the swizzle too) x box_rows slots of one head and page.
+// box_bytes x box_rows slots of one head and page, as they lie or with a swizzle of box_bytes, then 64 or 128.
 bool make_page_map(CUtensorMap* map, bool bytes_type, const void* base, const uint64_t* dims, const uint64_t* strides, uint32_t box_bytes,
-                   uint32_t box_rows);
+                   uint32_t box_rows, bool swizzle);
 namespace tc {
 
 // ---- PTX wrappers -------------------------------------------------------------------
