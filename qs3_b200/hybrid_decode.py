@@ -11,12 +11,16 @@ This is that loop. What runs through the C ABI of this library, per layer:
     residual add + the next layer's input norm                  qs3_moe_layer_execute
 
 and once per step the first norm (``qsfi_rmsnorm``) and the LM head (``qscb_gemm_bf16``).
-The token mixers (gated attention over a KV cache, GatedDeltaNet recurrence) are NOT part of
-this library: they are stand-ins written with torch operators, with the tensor shapes, state
+The token mixers (gated attention over a KV cache, GatedDeltaNet recurrence) are by default NOT
+part of this library: they are stand-ins written with torch operators, with the tensor shapes, state
 sizes and memory traffic of the real layers, so that the step time the MoE share is quoted
 against is a realistic one. The KV cache is paged: fixed-size pages in a pool, addressed through a
 CSR page table as upstream's runtime builds it (src/runtime.rs:99-181). One step is captured in a
 CUDA graph and replayed.
+
+With ``attention="paged"`` (``--attention paged``) the attention layers' rotary positions, cache writes and
+attention are this library's too (``qs3_kv_append``, ``qs3_paged_attention``), over a bf16 or an e4m3 cache
+(``--kv-cache fp8``); their projections, norms and gate stay torch operators.
 
 ``python -m qs3_b200.hybrid_decode`` prints one JSON line: decode tokens/s and the share of the
 step spent in the calls of this library.
@@ -59,6 +63,8 @@ class HybridConfig:
     context: int = 4096
     new_tokens: int = 256
     page_size: int = 16              # tokens per KV-cache page
+    attention: str = "torch"         # "paged": the library's attention over the cache
+    kv_fp8: bool = False             # paged: an e4m3 cache with a scale for every row
     eps: float = 1e-6
     seed: int = 0
 
@@ -173,6 +179,58 @@ class _Attention:
         return out.reshape(b, qh * d) @ self.w_o.t()
 
 
+class _PagedAttention(_Attention):
+    """The same layer with this library's operators from the norms to the gate: q and k are rotated and k and v
+    written to the cache in one pass, and attention reads the pages where they lie. `kv_len` (i32 [batch]) counts the
+    cached tokens, the new one included; it is the caller's, one for all layers."""
+
+    def __init__(self, cfg: HybridConfig, gen, dev, max_len, ctx: ops.Context, kv_len: torch.Tensor):
+        super().__init__(cfg, gen, dev, max_len)
+        self.ctx, self.kv_len = ctx, kv_len
+        self.freq = ops.rope_frequencies(cfg.rotary_dim, 10000.0, device=dev)
+        self.k_scale = self.v_scale = None
+        if cfg.kv_fp8:
+            self._quantise_context(dev)
+        b, d = cfg.batch, cfg.head_dim
+        self.workspace = torch.empty(ops.paged_attention_workspace_size(
+            ctx, torch.empty((b, cfg.q_heads, d), dtype=torch.bfloat16, device="meta"), self._cache(), batch=b),
+            dtype=torch.uint8, device=dev)
+
+    def _cache(self):
+        return ops.PagedKvCache(self.k_pool, self.v_pool, self.k_scale, self.v_scale)
+
+    def _quantise_context(self, dev):
+        """The prefilled bf16 context becomes an e4m3 one, a sequence at a time."""
+        cfg, n = self.cfg, self.cfg.context
+        bf16 = self._cache()
+        codes = lambda pool: torch.zeros(pool.shape, dtype=torch.uint8, device=dev)
+        scales = lambda pool: torch.ones(pool.shape[:3], dtype=torch.float32, device=dev)
+        quantised = ops.PagedKvCache(codes(self.k_pool), codes(self.v_pool), scales(self.k_pool), scales(self.v_pool))
+        rows = torch.tensor([0, n], dtype=torch.int32, device=dev)
+        length = rows[1:].contiguous()
+        k, v = (torch.empty((n, cfg.kv_heads, cfg.head_dim), dtype=torch.bfloat16, device=dev) for _ in range(2))
+        for i in range(cfg.batch if n else 0):
+            table = ops.PageTable(self.kv_indptr[i: i + 2].contiguous(), self.kv_indices, length)
+            ops.kv_gather(self.ctx, bf16, table, rows, k, v)
+            ops.kv_append(self.ctx, quantised, table, k, v, q_indptr=rows)
+        self.k_pool, self.v_pool, self.k_scale, self.v_scale = quantised.k, quantised.v, quantised.k_scale, quantised.v_scale
+
+    def __call__(self, x, pos, mask):
+        cfg = self.cfg
+        b, qh, kvh, d = x.shape[0], cfg.q_heads, cfg.kv_heads, cfg.head_dim
+        qg = (x @ self.w_qg.t()).view(b, qh, 2, d)
+        q, gate = qg[:, :, 0], qg[:, :, 1]
+        kv = (x @ self.w_kv.t()).view(b, 2, kvh, d)
+        norm = lambda t: (t.float() * torch.rsqrt(t.float().pow(2).mean(-1, keepdim=True) + cfg.eps)).to(t.dtype)
+        q, k, v = norm(q), norm(kv[:, 0]), kv[:, 1]
+        table = ops.PageTable(self.kv_indptr, self.kv_indices, self.kv_len)
+        ops.kv_append(self.ctx, self._cache(), table, k, v, q=q, inv_freq=self.freq.inv_freq, rope_scale=self.freq.scale)
+        out = torch.empty_like(q)
+        ops.paged_attention(self.ctx, q, self._cache(), table, out, self.workspace)
+        out = out * torch.sigmoid(gate.float()).to(x.dtype)
+        return out.reshape(b, qh * d) @ self.w_o.t()
+
+
 class _GatedDeltaNet:
     """Stand-in for a GatedDeltaNet layer (torch operators): input projection, causal depth-wise
     convolution over the last `conv_kernel` tokens, gated delta-rule update of a per-head
@@ -222,6 +280,8 @@ class HybridDecoder:
     the batch by one token; `capture()` records one step in a CUDA graph."""
 
     def __init__(self, cfg: HybridConfig, device: int = 0, keep_linear_scales: bool = False):
+        if cfg.attention not in ("torch", "paged") or (cfg.kv_fp8 and cfg.attention != "paged"):
+            raise ValueError("attention is 'torch' or 'paged', and only 'paged' has an e4m3 cache")
         self.cfg = cfg
         dev = torch.device("cuda", device)
         self.dev = dev
@@ -235,10 +295,15 @@ class HybridDecoder:
             self.embed = _normal((cfg.vocab, h), 0.02, gen, dev)
             self.lm_head = _normal((cfg.vocab, h), 0.02, gen, dev)
             self.input_norm = [torch.ones(h, dtype=torch.bfloat16, device=dev) for _ in range(cfg.layers + 1)]
+            self.kv_len = torch.full((b,), cfg.context, dtype=torch.int32, device=dev)   # paged attention: cached tokens
             self.mixers, self.blocks = [], []
             for layer in range(cfg.layers):
-                self.mixers.append(_Attention(cfg, gen, dev, self.max_len) if cfg.is_attention(layer)
-                                   else _GatedDeltaNet(cfg, gen, dev))
+                if not cfg.is_attention(layer):
+                    self.mixers.append(_GatedDeltaNet(cfg, gen, dev))
+                elif cfg.attention == "paged":
+                    self.mixers.append(_PagedAttention(cfg, gen, dev, self.max_len, self.ctx, self.kv_len))
+                else:
+                    self.mixers.append(_Attention(cfg, gen, dev, self.max_len))
                 self.blocks.append(_MoeBlock(self.ctx, cfg, gen, dev, keep_linear_scales))
             self.plan = ops.MoePlan(self.ctx, ops.MoePlanConfig(
                 max_num_tokens=b, hidden_size=h, intermediate_size=cfg.inter, num_experts=cfg.experts,
@@ -275,6 +340,7 @@ class HybridDecoder:
         # the device-side position is clamped as well, so that no replay can index past the cache
         pos = self.pos.clamp(max=self.max_len - 1)
         self.mask.index_fill_(2, pos, 0.0)               # the new token attends to itself
+        self.kv_len.copy_((pos + 1).expand(cfg.batch))
         self.residual.copy_(self.embed.index_select(0, self.tokens))
         ops.rmsnorm(ctx, self.residual, self.input_norm[0], self.x, cfg.eps)
         for layer, (mixer, blk) in enumerate(zip(self.mixers, self.blocks)):
@@ -345,6 +411,8 @@ class HybridDecoder:
         for m in self.mixers:
             if isinstance(m, _Attention):
                 out += [(m.k_pool, m.decode_pages), (m.v_pool, m.decode_pages)]
+                if self.cfg.kv_fp8:
+                    out += [(m.k_scale, m.decode_pages), (m.v_scale, m.decode_pages)]
             else:
                 out += [(m.conv_state, None), (m.state, None)]
         return out
@@ -409,7 +477,9 @@ def measure(steps: int | None = None, cfg: HybridConfig | None = None) -> dict:
         "library_calls": "rmsnorm, fused add+rmsnorm+NVFP4, MoE layer (+ residual add + next norm), LM head",
         "moe_weight_bytes_per_step": moe_bytes, "moe_weight_stream_gbs": moe_bytes / (lib * 1e-3) / 1e9,
         "mixers": f"torch stand-ins (gated attention over a paged KV cache, {cfg.page_size}-token pages behind a CSR "
-                  "page table; GatedDeltaNet recurrence)",
+                  "page table; GatedDeltaNet recurrence)"
+                  + (f"; rotary positions, cache and attention by this library, {'e4m3' if cfg.kv_fp8 else 'bf16'} cache"
+                     if cfg.attention == "paged" else ""),
         "config": {k: getattr(cfg, k) for k in ("layers", "hidden", "experts", "top_k", "inter", "shared_inter",
                                                  "batch", "context", "vocab", "page_size")},
         "steps": timed, "device_error": err, "data": "synthetic"}
@@ -421,8 +491,13 @@ def main():
     ap.add_argument("--layers", type=int, default=HybridConfig.layers)
     ap.add_argument("--batch", type=int, default=HybridConfig.batch)
     ap.add_argument("--context", type=int, default=HybridConfig.context)
+    ap.add_argument("--attention", choices=("torch", "paged"), default=HybridConfig.attention)
+    ap.add_argument("--kv-cache", choices=("bf16", "fp8"), default="bf16", help="of --attention paged")
     args = ap.parse_args()
-    cfg = HybridConfig(layers=args.layers, batch=args.batch, context=args.context)
+    if args.kv_cache == "fp8" and args.attention != "paged":
+        ap.error("--kv-cache fp8 needs --attention paged")
+    cfg = HybridConfig(layers=args.layers, batch=args.batch, context=args.context, attention=args.attention,
+                       kv_fp8=args.kv_cache == "fp8")
     print(json.dumps(measure(args.steps, cfg)))
 
 
