@@ -967,7 +967,7 @@ typedef struct {
 
 /* Token p of sequence b lies in slot p % page_size of page kv_indices[kv_indptr[b] + p / page_size]. At most 4096 sequences.
  * The tables are read on the device. A page id outside the pool and a length beyond a sequence's pages are not followed:
- * such tokens count as zeros, or as absent, and qs3_moe_check_device_error reports 0x5b000001. */
+ * such tokens count as zeros, or as absent, and qs3_moe_check_device_error reports 0x5d000001. */
 typedef struct {
     qsfi_tensor1 kv_indptr;  /* i32 [batch + 1], ascending */
     qsfi_tensor1 kv_indices; /* i32 */
@@ -1006,8 +1006,10 @@ qsfi_status qs3_kv_gather(qsfi_context* ctx, const qs3_kv_gather_desc* desc);
  * over the tokens j that row i of n of sequence b sees: with p = kv_len[b] - n + i all j <= p (causal; else all
  * j < kv_len[b]), and j > p - window where there is one. A row that sees none gets 0 and -infinity. Query heads
  * h * group .. h * group + group - 1 share KV head h. Head sizes 64, 128 and 256. Sums, maxima and the exponents are in
- * 32 bits; the weights exp(s_j - max) are rounded to bf16 for the product with v. Values of v at tokens that only some rows
- * of a tile see have to be finite, as 0 * inf is NaN; what lies in the pages behind a sequence's end does not matter. */
+ * 32 bits; the weights exp(s_j - max), times v's scales, are rounded to bf16 (bf16 caches) or f16 (e4m3 ones) for the product
+ * with v, and with e4m3 caches an element of q may be off by 2^-17 of the largest of its row. v has to be finite at every
+ * token of a sequence, also at those that a row does not see, as 0 * inf is NaN; a row of q with an infinity or a NaN gets
+ * NaN. What k holds where a row does not see it, and what lies in the pages behind a sequence's end, does not matter. */
 typedef struct {
     qsfi_tensor3 q; /* bf16 [rows, heads, head_dim], heads a multiple of kv_heads */
     qs3_paged_kv_cache cache;

@@ -11,6 +11,7 @@
 //   * qs3_debug_bounded_wait_probe: a one-CTA kernel that waits on an mbarrier nobody
 //     completes, with a caller-chosen short limit, for testing the expiry path without
 //     faulting, trapping or hanging anything.
+#include "paged.cuh"
 #include "tcgen05.cuh"
 
 namespace qs3 {
@@ -128,6 +129,11 @@ extern "C" qsfi_status qs3_moe_check_device_error(qsfi_context* ctx)
     qsfi_status status = qs3_moe_read_device_error(ctx, &code);
     if (status != QSFI_STATUS_OK)
         return status;
+    if (code == ERR_PAGE_TABLE)
+        return set_error(ctx, QSFI_STATUS_BACKEND_ERROR, QSFI_ERROR_SOURCE_QSFI, static_cast<int32_t>(code),
+                         "a page table (code 0x%08x) names a page outside its pool, or a sequence is longer than its pages; "
+                         "such tokens counted as zeros or as absent",
+                         code);
     if (code != 0)
         return set_error(ctx, QSFI_STATUS_BACKEND_ERROR, QSFI_ERROR_SOURCE_QSFI, static_cast<int32_t>(code),
                          "a bounded device-side wait expired (code 0x%08x): a load, a tensor-core commit or a peer "

@@ -7,7 +7,7 @@
 namespace qs3 {
 
 // Codes in the device error word: a page id outside the pool, or a sequence longer than its pages.
-enum : uint32_t { ERR_PAGE_TABLE = 0x5b000001u };
+enum : uint32_t { ERR_PAGE_TABLE = 0x5d000001u };
 
 constexpr uint32_t kMaxHeadDim = 256;
 constexpr uint32_t kMaxBatch = 4096;

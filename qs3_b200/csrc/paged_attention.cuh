@@ -253,7 +253,7 @@ cudaError_t launch_attn_stream(const AttnParams& p, bool fp8, cudaStream_t strea
 cudaError_t launch_attn_prefill(const AttnParams& p, bool fp8, cudaStream_t stream);
 cudaError_t launch_attn_join(const AttnParams& p, cudaStream_t stream);
 // Rows of an item of the streaming kernel: 8 or 16; blocks that fit the device at once.
-uint32_t attn_stream_rows(uint32_t rows_per_seq, uint32_t head_dim);
+uint32_t attn_stream_rows(uint32_t rows_per_seq);
 uint32_t attn_prefill_rows(uint32_t head_dim); // and of the kernel for chunks; keys of its key tile: 128
 uint32_t attn_stream_blocks(uint32_t tile_rows, uint32_t head_dim, bool fp8);
 

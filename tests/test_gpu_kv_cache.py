@@ -246,7 +246,7 @@ def test_bad_pages_are_left_alone(ops, ctx):
     before = cache.k.clone()
     ops.kv_append(ctx, cache, table, k, k)
     torch.cuda.synchronize()
-    assert ctx.read_device_error() == 0x5b000001
+    assert ctx.read_device_error() == 0x5d000001
     page0 = int(table.kv_indices[1])
     assert torch.equal(cache.k[page0, :, 3], k[0])
     changed = (cache.k != before).flatten(1).any(1).nonzero().flatten().tolist()
@@ -254,7 +254,7 @@ def test_bad_pages_are_left_alone(ops, ctx):
     out = torch.full((100, 2, 64), 7.0, dtype=torch.bfloat16, device="cuda")
     ops.kv_gather(ctx, cache, table, ints([0, 20, 60, 100]), out, out.clone())
     torch.cuda.synchronize()
-    assert ctx.read_device_error() == 0x5b000001
+    assert ctx.read_device_error() == 0x5d000001
     assert torch.equal(out[19], k[0]) and bool((out[52:60] == 7.0).all())
 
 
