@@ -747,7 +747,7 @@ qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_des
         p.lse_head = d->lse.stride[1];
     }
     if (!rows_fit(p.view))
-        return set_unsupported(ctx, "paged_attention cache strides are too large: 2^32 steps of a row's alignment, or scales 2^30 elements apart");
+        return set_unsupported(ctx, "paged_attention cache has more than 2^32 rows' worth of memory between its first and last, or scales 2^30 apart");
     if (d->window != 0 && d->causal == 0)
         return set_unsupported(ctx, "paged_attention window needs causal");
     if (!std::isfinite(d->sm_scale) || d->sm_scale < 0.0f)

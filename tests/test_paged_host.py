@@ -281,6 +281,8 @@ def attention_desc(**kw):
     (dict(q_indptr=t(I32, 3)), INVALID, "q_indptr"),
     (dict(lse=t(F32, 3, 3)), INVALID, "lse"),
     (dict(window=4, causal=0), UNSUPPORTED, "window needs causal"),
+    (dict(cache=cache(k=t(E4M3, 4, 2, 16, 64), v=t(E4M3, 4, 2, 16, 64), k_scale=t(F32, 4, 2, 16, stride=(1 << 30, 16, 1)),
+                      v_scale=t(F32, 4, 2, 16))), UNSUPPORTED, "scales 2^30 apart"),
     (dict(cache=cache(k=t(BF16, 1 << 30, 2, 16, 64, stride=(2056, 1024, 64, 1)), v=t(BF16, 1 << 30, 2, 16, 64))), UNSUPPORTED, "2^32 rows"),
     (dict(sm_scale=float("inf")), INVALID, "sm_scale"),
     (dict(sm_scale=-1.0), INVALID, "sm_scale"),
