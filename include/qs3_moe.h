@@ -1015,7 +1015,8 @@ typedef struct {
     qs3_paged_kv_cache cache;
     qs3_page_table table;
     qsfi_tensor1 q_indptr;  /* optional i32 [batch + 1], ascending from 0; absent: row b belongs to sequence b */
-    qsfi_tensor3 out;       /* bf16 [rows, heads, head_dim]; rows behind the last sequence are left as they are */
+    qsfi_tensor3 out;       /* bf16 [rows, heads, head_dim], may be q but not overlap it otherwise; rows behind the last sequence
+                               are left as they are */
     qsfi_tensor2 lse;       /* optional f32 [rows, heads] */
     qsfi_tensor1 workspace; /* u8, qs3_paged_attention_workspace_size bytes, 256-byte aligned; calls that may overlap on
                                the device need one each */

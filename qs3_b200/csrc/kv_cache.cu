@@ -499,39 +499,6 @@ void fill_rows(Rows* r, const qsfi_tensor3& src, const qsfi_tensor3& dst, int64_
     r->heads = static_cast<uint32_t>(src.shape[1]);
 }
 
-// Where `out` is absent the rows are turned in place. The two may be the same rows or apart, nothing between.
-qsfi_status check_out(qsfi_context* ctx, const qsfi_tensor3& x, const qsfi_tensor3& out, const char* op, const char* name,
-                      qsfi_tensor3* dst, int* in_place)
-{
-    *dst = out.data != nullptr ? out : x;
-    if (out.data != nullptr) {
-        if (const qsfi_status s = check_rows(ctx, out, op, name, x.dtype); s != QSFI_STATUS_OK)
-            return s;
-        for (int i = 0; i < 3; ++i)
-            if (out.shape[i] != x.shape[i])
-                return set_invalid_arg(ctx, "%s %s shape must match its input", op, name);
-    }
-    if (!rows_apart(*dst))
-        return set_invalid_arg(ctx, "%s %s rows must not overlap", op, name);
-    *in_place = dst->data == x.data && dst->stride[0] == x.stride[0] && dst->stride[1] == x.stride[1];
-    const int64_t size = x.dtype == QSFI_DTYPE_F32 ? 4 : 2;
-    const auto span = [&](const qsfi_tensor3& t) {
-        return ((t.shape[0] - 1) * t.stride[0] + (t.shape[1] - 1) * t.stride[1] + t.shape[2]) * size;
-    };
-    const uint8_t *a = static_cast<const uint8_t*>(x.data), *b = static_cast<const uint8_t*>(dst->data);
-    if (!*in_place && a < b + span(*dst) && b < a + span(x)) {
-        // views of one buffer (the heads of a fused projection) lie between each other without sharing an element when
-        // their token strides are the same and their rows fall into different parts of it
-        const int64_t pitch = x.stride[0] * size;
-        const int64_t wide_a = ((x.shape[1] - 1) * x.stride[1] + x.shape[2]) * size;
-        const int64_t wide_b = ((dst->shape[1] - 1) * dst->stride[1] + dst->shape[2]) * size;
-        const int64_t shift = pitch > 0 ? ((b - a) % pitch + pitch) % pitch : 0;
-        if (x.stride[0] != dst->stride[0] || shift < wide_a || shift + wide_b > pitch)
-            return set_invalid_arg(ctx, "%s %s overlaps its input without being the same rows", op, name);
-    }
-    return QSFI_STATUS_OK;
-}
-
 template <typename T, int TARGET> cudaError_t launch_turn(const TurnParams& p, bool interleaved, cudaStream_t stream)
 {
     const dim3 grid((p.tokens + p.block_tokens - 1) / p.block_tokens);
@@ -615,6 +582,39 @@ bool rows_apart(const qsfi_tensor3& t) // rows of shape[2] elements at two strid
     if (t.shape[0] > 1 && t.shape[1] > 1)
         return a0 >= (t.shape[1] - 1) * a1 + t.shape[2] || a1 >= (t.shape[0] - 1) * a0 + t.shape[2];
     return true;
+}
+
+// `out`, or where it is absent x itself, becomes `dst`. The two may be the same rows or apart, nothing between.
+qsfi_status check_out(qsfi_context* ctx, const qsfi_tensor3& x, const qsfi_tensor3& out, const char* op, const char* name,
+                      qsfi_tensor3* dst, int* in_place)
+{
+    *dst = out.data != nullptr ? out : x;
+    if (out.data != nullptr) {
+        if (const qsfi_status s = check_rows(ctx, out, op, name, x.dtype); s != QSFI_STATUS_OK)
+            return s;
+        for (int i = 0; i < 3; ++i)
+            if (out.shape[i] != x.shape[i])
+                return set_invalid_arg(ctx, "%s %s shape must match its input", op, name);
+    }
+    if (!rows_apart(*dst))
+        return set_invalid_arg(ctx, "%s %s rows must not overlap", op, name);
+    *in_place = dst->data == x.data && dst->stride[0] == x.stride[0] && dst->stride[1] == x.stride[1];
+    const int64_t size = x.dtype == QSFI_DTYPE_F32 ? 4 : 2;
+    const auto span = [&](const qsfi_tensor3& t) {
+        return ((t.shape[0] - 1) * t.stride[0] + (t.shape[1] - 1) * t.stride[1] + t.shape[2]) * size;
+    };
+    const uint8_t *a = static_cast<const uint8_t*>(x.data), *b = static_cast<const uint8_t*>(dst->data);
+    if (!*in_place && a < b + span(*dst) && b < a + span(x)) {
+        // views of one buffer (the heads of a fused projection) lie between each other without sharing an element when
+        // their token strides are the same and their rows fall into different parts of it
+        const int64_t pitch = x.stride[0] * size;
+        const int64_t wide_a = ((x.shape[1] - 1) * x.stride[1] + x.shape[2]) * size;
+        const int64_t wide_b = ((dst->shape[1] - 1) * dst->stride[1] + dst->shape[2]) * size;
+        const int64_t shift = pitch > 0 ? ((b - a) % pitch + pitch) % pitch : 0;
+        if (x.stride[0] != dst->stride[0] || shift < wide_a || shift + wide_b > pitch)
+            return set_invalid_arg(ctx, "%s %s overlaps its input without being the same rows", op, name);
+    }
+    return QSFI_STATUS_OK;
 }
 
 bool rows_fit(const PagedView& v)

@@ -66,7 +66,7 @@ __device__ __forceinline__ uint64_t warp_tiles_cost(const AttnTiling& a, uint32_
     uint64_t sum = 0;
     for (uint32_t t = threadIdx.x & 31; t < tiles; t += 32) {
         const KeyTiles k = key_tiles(a, fresh, length, t);
-        sum += k.end - k.first + a.item_cost;
+        sum += cost_of(a, k.end - k.first);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
@@ -89,7 +89,7 @@ __device__ BlockRange find_range(const AttnParams& p, uint64_t* cost, uint32_t b
             const uint32_t length = seq_pages(p.view, b).length;
             for (uint32_t t = 0; t < tiles; ++t) {
                 const KeyTiles k = key_tiles(p.tiling, fresh, length, t);
-                sum += k.end - k.first + p.tiling.item_cost;
+                sum += cost_of(p.tiling, k.end - k.first);
             }
         } else {
             sum = kUnknown;
@@ -155,7 +155,7 @@ __device__ BlockRange find_range(const AttnParams& p, uint64_t* cost, uint32_t b
         uint32_t mine = 0;
         if (t0 + lane < tiles) {
             const KeyTiles k = key_tiles(p.tiling, fresh, length, t0 + lane);
-            mine = k.end - k.first + p.tiling.item_cost;
+            mine = cost_of(p.tiling, k.end - k.first);
         }
         uint64_t run = mine;
 #pragma unroll
@@ -195,7 +195,7 @@ __device__ __forceinline__ void next_item(const AttnParams& p, AttnPlace* at, ui
 __device__ __forceinline__ void note_split(const AttnParams& p, const BlockRange& r)
 {
     SplitNote n { r.place.seq, r.place.head, r.place.tile, 0 };
-    if (r.begin < r.end && r.place.offset > p.tiling.item_cost) {
+    if (r.begin < r.end && r.place.offset > p.tiling.item_cost) { // (never with even items, which have an offset of 0)
         const uint64_t item = r.begin - r.place.offset;
         const KeyTiles k = key_tiles(p.tiling, seq_rows(p, n.seq).fresh, seq_pages(p.view, n.seq).length, n.tile);
         if (block_begin(r.total, r.active, blockIdx.x - 1) <= item + p.tiling.item_cost) // (block 0 begins with an item)
@@ -242,7 +242,7 @@ __device__ __forceinline__ bool this_segment(const AttnParams& p, const AttnPlac
 
 __device__ __forceinline__ void next_segment(const AttnParams& p, const Segment& s, AttnPlace* at, uint64_t* left)
 {
-    const uint64_t rest = static_cast<uint64_t>(p.tiling.item_cost) + s.tiles - at->offset;
+    const uint64_t rest = cost_of(p.tiling, s.tiles) - at->offset;
     *left = *left > rest ? *left - rest : 0;
     next_item(p, at, row_tiles(p.tiling, s.rows.fresh));
 }

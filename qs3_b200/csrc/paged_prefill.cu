@@ -1036,7 +1036,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     mbar_arrive(&bar.o_free[q]);
                 if (live && whole && half == 0 && p.lse != nullptr)
                     p.lse[(seg.rows.row0 + token) * p.lse_token + h * p.lse_head]
-                        = m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
+                        = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
                 if (live && !whole && half == 0)
                     p.part_ml[part_row] = make_float2(m, l);
             }

@@ -6,7 +6,8 @@
 // more for its start and end. Items follow each other by sequence, KV head, tile; their costs, laid end to end, are cut into
 // equal ranges, one per block of the launch. A range ends where it ends, inside an item as well, so that lengths which differ
 // leave no block idle and a single long context is spread over all SMs; an item whose key tiles are cut this way leaves
-// partial results that a second launch joins.
+// partial results that a second launch joins. Short contexts are not worth that launch: `even` items cost 1 each, whatever their
+// length, and no range ends inside one.
 #pragma once
 
 #include <cstdint>
@@ -46,6 +47,7 @@ struct AttnTiling {
     uint32_t window;    // 0: none
     uint32_t causal;
     uint32_t item_cost; // in key tiles
+    uint32_t even = 0;
 };
 
 struct KeyTiles {
@@ -83,6 +85,8 @@ QS3_HD KeyTiles key_tiles(const AttnTiling& a, uint32_t fresh, uint32_t length, 
     return k;
 }
 
+QS3_HD uint32_t cost_of(const AttnTiling& a, uint32_t tiles) { return a.even ? 1 : a.item_cost + tiles; }
+
 // Blocks that get work: every one at least `least` key tiles, as far as there are any.
 QS3_HD uint32_t active_blocks(uint64_t total, uint32_t blocks, uint32_t least)
 {
@@ -103,6 +107,8 @@ QS3_HD uint32_t block_of_end(uint64_t total, uint32_t blocks, uint64_t end)
 // Key tiles of an item that lie before a position `offset` from its beginning.
 QS3_HD uint32_t tiles_before(const AttnTiling& a, uint64_t offset, uint32_t tiles)
 {
+    if (a.even)
+        return offset > 0 ? tiles : 0;
     const uint64_t t = offset > a.item_cost ? offset - a.item_cost : 0;
     return t < tiles ? static_cast<uint32_t>(t) : tiles;
 }

@@ -79,12 +79,12 @@ def make_case(ops, q_len, kv_len, *, heads, kv_heads, dim, page=16, fp8=False, s
                 ops.PagedKvCache(*pools, *scales), ints(running(q_len)), truth[0], truth[1], q, sum(q_len))
 
 
-def attention_reference(c: Case, *, causal=True, window=0, scale=None):
+def attention_reference(c: Case, *, causal=True, window=0, scale=None, q_off=0.0):
     """out, lse in 64 bits, and the most that each may be off.
 
     A kernel computes scores in 32 bits (each product's sum off by at most (D + 8) 2^-24 of the sum of the magnitudes, the
     weights by e to that, and by a few units of 2^-22 for the exponential), rounds the weights to bf16 (2^-8 of each, half a
-    step) and the result once more."""
+    step) and the result once more. `q_off`: what an element of q may be off besides, of the largest of its row."""
     scale = c.dim ** -0.5 if scale is None else scale
     group = c.heads // c.kv_heads
     out = torch.zeros((c.rows, c.heads, c.dim), dtype=torch.float64, device="cuda")
@@ -104,6 +104,7 @@ def attention_reference(c: Case, *, causal=True, window=0, scale=None):
             q, k, v = c.q[row: row + n, h].double(), c.keys[b][:, h // group], c.values[b][:, h // group]
             s = torch.where(seen, q @ k.T * scale, -math.inf)
             off = ((c.dim + 8) * 2.0 ** -24 * scale * (q.abs() @ k.abs().T).masked_fill(~seen, 0)).amax(1, keepdim=True) + 2.0 ** -20
+            off = off + q_off * scale * q.abs().amax(1, keepdim=True) * torch.where(seen, k.abs().sum(1)[None], 0.0).amax(1, keepdim=True)
             some = seen.any(1, keepdim=True)
             w = torch.where(some, torch.softmax(torch.where(some, s, 0.0), dim=1), 0.0)
             o = w @ v

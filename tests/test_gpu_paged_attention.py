@@ -165,3 +165,80 @@ def test_results_do_not_depend_on_the_run(ops, ctx):
     for _ in range(3):
         again = run_attention(ops, ctx, c)
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dim,heads", [(64, 6), (128, 4), (256, 10)])
+@pytest.mark.parametrize("page,slots_first", [(8, False), (32, True), (48, False), (64, False), (128, True), (256, False)])
+def test_chunks_over_page_sizes_and_windows(ops, ctx, page, slots_first, dim, heads, fp8):
+    """Whole boxes of a page, ends of sequences inside one, and windows that begin inside one, in both row tiles of a chunk."""
+    c = make_case(ops, [200, 1, 37], [900, 300, 37], heads=heads, kv_heads=2, dim=dim, page=page, fp8=fp8, seed=page + dim,
+                  slots_first=slots_first, tail=1)
+    check_attention(*run_attention(ops, ctx, c), c)
+    check_attention(*run_attention(ops, ctx, c, window=333), c, window=333)
+    assert ctx.read_device_error() == 0
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("q_len", [[1, 1], [3, 150]])
+def test_in_place_and_on_another_stream(ops, q_len, fp8):
+    """`out` may be q; contexts on streams of their own, each with its workspace, may run at the same time."""
+    cases = [make_case(ops, q_len, [2000, 700], heads=8, kv_heads=2, dim=128, fp8=fp8, seed=20 + i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in cases], []
+    kept = []
+    for c, stream in zip(cases, streams):
+        with torch.cuda.stream(stream):
+            ctx = ops.Context()
+            ws = torch.empty(ops.paged_attention_workspace_size(ctx, c.q, c.cache, batch=2), dtype=torch.uint8, device="cuda")
+            x = c.q.clone()
+            for _ in range(5):
+                x.copy_(c.q)
+                ops.paged_attention(ctx, x, c.cache, c.table, x, ws, q_indptr=c.q_indptr)
+            outs.append(x)
+            kept += [ctx, ws]
+    torch.cuda.synchronize()
+    for c, x in zip(cases, outs):
+        check_attention(x, None, c)
+
+
+def test_queries_with_an_outlier_over_an_8_bit_cache(ops, ctx):
+    """An element of q is off by 2^-17 of the largest of its row at most."""
+    c = make_case(ops, [100], [400], heads=16, kv_heads=2, dim=256, fp8=True, seed=30)
+    c.q[..., 7] *= 64.0
+    check_attention(*run_attention(ops, ctx, c, sm_scale=0.02), c, scale=0.02, q_off=2.0 ** -17)
+
+
+def test_a_query_that_is_not_finite(ops, ctx):
+    """Its row becomes NaN, the others do not."""
+    for fp8 in (False, True):
+        for q_len in ([1, 1], [1, 40]):
+            c = make_case(ops, q_len, [50, 300], heads=4, kv_heads=2, dim=64, fp8=fp8, seed=31)
+            good, _ = run_attention(ops, ctx, c)
+            c.q[0, 1, 3] = math.nan
+            c.q[1, 2, 5] = math.inf
+            out, lse = run_attention(ops, ctx, c)
+            assert bool(out[0, 1].isnan().all()) and bool(out[1, 2].isnan().all())
+            assert bool(lse[0, 1].isnan()) and bool(lse[1, 2].isnan()) and int(lse[: c.rows].isnan().sum()) == 2
+            out[0, 1], out[1, 2] = good[0, 1], good[1, 2]
+            assert torch.equal(out, good)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("q_len", [[1] * 9, [5, 0, 130, 1, 2, 64, 3, 1, 9]])
+@pytest.mark.parametrize("said", [384, 100])
+def test_short_contexts_are_not_cut(ops, ctx, said, q_len, fp8):
+    """Contexts that the caller calls short, whether they are or not."""
+    kv = [0, 1, 384, 383, 65, 64, 3, 200, 385]
+    c = make_case(ops, q_len, [max(a, b) for a, b in zip(q_len, kv)] if max(q_len) > 1 else kv, heads=8, kv_heads=2, dim=128,
+                  fp8=fp8, seed=40)
+    check_attention(*run_attention(ops, ctx, c, max_kv_len=said), c)
+    check_attention(*run_attention(ops, ctx, c), c)
+
+
+def test_many_sequences_in_one_call(ops, ctx):
+    """As many sequences as a call takes, several items to a block."""
+    kv = [(41 * i) % 70 for i in range(4096)]
+    c = make_case(ops, [1] * len(kv), kv, heads=2, kv_heads=1, dim=64, page=64, seed=41)
+    check_attention(*run_attention(ops, ctx, c, decode=True, max_kv_len=70), c)
+    check_attention(*run_attention(ops, ctx, c, decode=True), c)

@@ -69,6 +69,12 @@ int main()
         for (uint64_t offset = 0; offset < 20; ++offset)
             CHECK(tiles_before(a, offset, 10) == (offset <= cost ? 0 : offset - cost < 10 ? offset - cost : 10));
     }
+    // even items are never cut
+    {
+        AttnTiling a { FastDiv(1), 3, 6, 1, 0, 1, 3 };
+        a.even = 1;
+        CHECK(cost_of(a, 1) == 1 && cost_of(a, 9) == 1 && tiles_before(a, 0, 9) == 0 && tiles_before(a, 1, 9) == 9 && tiles_before(a, 7, 9) == 9);
+    }
     // ranges follow each other, hold everything and differ by one at most
     for (uint64_t total : { 1ull, 2ull, 147ull, 148ull, 149ull, 12345ull, 1ull << 52 })
         for (uint32_t blocks : { 1u, 148u, 1184u })
@@ -275,6 +281,7 @@ def attention_desc(**kw):
     (dict(q=t(F32, 3, 4, 64)), INVALID, "q dtype"),
     (dict(out=t(BF16, 3, 2, 64)), INVALID, "out shape"),
     (dict(out=t(BF16, 3, 4, 64, stride=(64, 64, 1))), INVALID, "must not overlap"),
+    (dict(out=t(BF16, 3, 4, 64, ptr=0x10000 + 128)), INVALID, "overlaps its input"),
     (dict(q=t(BF16, 3, 3, 64), out=t(BF16, 3, 3, 64)), INVALID, "multiple of kv_heads"),
     (dict(q=t(BF16, 2, 4, 64), out=t(BF16, 2, 4, 64)), INVALID, "a row per sequence"),
     (dict(q=t(BF16, 1 << 25, 4, 64), out=t(BF16, 1 << 25, 4, 64)), UNSUPPORTED, "2^24 rows"),
