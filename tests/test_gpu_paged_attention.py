@@ -242,3 +242,49 @@ def test_many_sequences_in_one_call(ops, ctx):
     c = make_case(ops, [1] * len(kv), kv, heads=2, kv_heads=1, dim=64, page=64, seed=41)
     check_attention(*run_attention(ops, ctx, c, decode=True, max_kv_len=70), c)
     check_attention(*run_attention(ops, ctx, c, decode=True), c)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_pages_more_than_32_bits_apart(ops, ctx, fp8):
+    """Pages 3 GiB apart, scales 1 GiB: written, attended over by both kernels, and read back."""
+    q_len, kv_len, heads, kv_heads, dim, page = [70, 1], [300, 64], 8, 2, 128, 128
+    c = make_case(ops, q_len, kv_len, heads=heads, kv_heads=kv_heads, dim=dim, page=page, fp8=fp8, seed=50)
+    pages = c.cache.k.shape[0]
+    room = torch.empty(pages * (3 << 30), dtype=torch.uint8, device="cuda")
+    room_scales = torch.empty(pages * (1 << 28), dtype=torch.float32, device="cuda") if fp8 else None
+
+    def far(pool, at):
+        size = pool.element_size()
+        flat = room.view(pool.dtype) if size == 1 else room.view(torch.bfloat16)
+        return flat.as_strided(pool.shape, ((3 << 30) // size, page * dim, dim, 1), at * kv_heads * page * dim)
+
+    def far_scales(at):
+        return room_scales.as_strided((pages, kv_heads, page), (1 << 28, page, 1), at * kv_heads * page)
+
+    near = c.cache
+    c.cache = ops.PagedKvCache(far(near.k, 0), far(near.v, 1), *([far_scales(0), far_scales(1)] if fp8 else ()))
+    for a, b in ((c.cache.k, near.k), (c.cache.v, near.v)):
+        a.view(torch.uint8).copy_(b.view(torch.uint8)) if fp8 else a.copy_(b)
+    if fp8:
+        c.cache.k_scale.copy_(near.k_scale), c.cache.v_scale.copy_(near.v_scale)
+    check_attention(*run_attention(ops, ctx, c), c)
+    rows = sum(kv_len)
+    out = [torch.zeros((rows, kv_heads, dim), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    indptr = ints([0, kv_len[0], rows])
+    ops.kv_gather(ctx, c.cache, c.table, indptr, *out)
+    for got, want in zip(out, (c.keys, c.values)):
+        assert torch.equal(got, torch.cat(want).to(torch.bfloat16))
+    c.cache.k.view(torch.uint8).zero_(), c.cache.v.view(torch.uint8).zero_()
+    ops.kv_append(ctx, c.cache, c.table, *out, q_indptr=indptr)
+    again = [torch.zeros_like(x) for x in out]
+    ops.kv_gather(ctx, c.cache, c.table, indptr, *again)
+    for got, want in zip(again, out):   # (e4m3: once more rounded, by half a step of 2^-3 and of the bf16 result)
+        assert bool(((got.float() - want.float()).abs() <= (want.float().abs() * (2.0 ** -4 + 2.0 ** -8)
+                                                             + want.float().abs().amax(-1, keepdim=True) * 2.0 ** -18
+                                                             if fp8 else 0)).all())
+    small = make_case(ops, [1, 1], kv_len, heads=heads, kv_heads=kv_heads, dim=dim, page=page, seed=51)
+    c.q, c.q_len, c.rows, c.q_indptr = small.q, [1, 1], 2, small.q_indptr
+    c.keys, c.values = ([torch.split(x.double(), kv_len) for x in again][i] for i in range(2))
+    if not fp8:
+        check_attention(*run_attention(ops, ctx, c, decode=True), c)
+    assert ctx.read_device_error() == 0
