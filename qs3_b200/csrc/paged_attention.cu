@@ -135,7 +135,7 @@ template <uint32_t ROW_BYTES> __device__ __forceinline__ uint32_t swizzled(uint3
         return r * ROW_BYTES + ((c ^ (r >> 1 & 3)) * 16);
 }
 
-template <uint32_t D, uint32_t NT, bool FP8> 
+template <uint32_t D, uint32_t NT, bool FP8>
 __global__ void __launch_bounds__(kStreamThreads, StreamShape<D, NT, FP8>::kBlocks) attn_stream_kernel(AttnParams p)
 {
     using Shape = StreamShape<D, NT, FP8>;
@@ -747,7 +747,8 @@ qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_des
         p.lse_head = d->lse.stride[1];
     }
     if (!rows_fit(p.view))
-        return set_unsupported(ctx, "paged_attention cache has more than 2^32 rows' worth of memory between its first and last, or scales 2^30 apart");
+        return set_unsupported(ctx, "paged_attention cache has more than 2^32 rows' worth of memory between its first and last, "
+                                    "or scales 2^30 apart");
     if (d->window != 0 && d->causal == 0)
         return set_unsupported(ctx, "paged_attention window needs causal");
     if (!std::isfinite(d->sm_scale) || d->sm_scale < 0.0f)

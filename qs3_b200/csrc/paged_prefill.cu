@@ -16,21 +16,22 @@
 // m follows the row's maximum only when that has grown by 2^8 (the weights stay below 256, the sums take the difference):
 // steps that rescale O in tensor memory are then few.
 //
-// Five warps fetch, three K in panels of 64 elements and two V in groups of keys, in pieces of 32 KB, each warp its own slots of
-// K's or V's ring: a slot's barriers then pass their phases in one order for all, which parities need. Pages that a box of TMA
-// divides come that way; other page sizes, the ends of sequences and windows row by row with cp.async, 16 bytes being the unit
-// in which every page size, stride and swizzled place works. Keys that no row sees are zeros then.
+// bf16 caches: five warps fetch, three K in panels of 64 elements and two V in groups of keys, in pieces of 32 KB, each warp its
+// own slots of K's or V's ring: a slot's barriers then pass their phases in one order for all, which parities need. Pages that a
+// box of TMA divides come that way; other page sizes, the ends of sequences and windows row by row with cp.async, 16 bytes being
+// the unit in which every page size, stride and swizzled place works. Keys that no row sees are zeros then.
 //
 // e4m3 caches: K's codes are multiplied as they are. A row of queries is scaled by the power of two that brings its largest element
 // to 2^7 or just above and becomes the sum of two e4m3 numbers, the high one rounded to 4 bits and the low one the rest: bf16's 8
 // bits exactly, and no element is off by more than 2^-17 of the largest. Two products of twice the rate take the time of one.
 // K's scales are a factor on the scores. V's are part of the weights, w = exp2(s + log2(scale) - m), of which the largest is again
 // at a known place; a second e4m3 number would keep 8 bits of a weight but only 14 of the range below the largest, which many
-// small weights together need, so the weights are f16 and V is converted, by the four warps that fetch it: boxes to a staging
-// area, from there to registers, which makes room for the next ones, and to the ring. (Loads straight to registers filled what
-// the first-level cache has left beside so much shared memory, and everyone's loads waited.) The row's sum takes
-// V's scale out again. 1021 tokens behind 31 111 cached ones: 670 us; with loads straight to registers 765, and with all
-// converted to f16, K too, 965. Shared memory is the bound: codes in and out, V in f16, the products' operands and the scales.
+// small weights together need. So the weights are f16 and V is converted, by the four warps that fetch it: boxes to a staging
+// area, from there to registers, which makes room for the next ones, and to the ring. A fifth warp fetches K and a sixth the
+// scales. The row's sum takes V's scale out again.
+// 1021 tokens behind 31 111 cached ones take 670 us; with V's loads straight to registers, which fill what the first-level cache
+// has left beside so much shared memory, 765; with everything converted to f16, K too, 965. Shared memory is the bound: codes in
+// and out, V in f16, the products' operands and the scales.
 #include "paged_attention.cuh"
 #include "tcgen05.cuh"
 
@@ -679,7 +680,8 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     if (lane < per_panel * ((UNITS + 7) / 8)) {
                         const uint32_t panel = lane / per_panel, first = (lane - panel * per_panel) * box;
                         tma_load_page(ring_at + s * piece_bytes + panel * (KEYS * 128) + first * WIDTH, &map, &full_bar[s],
-                                      static_cast<int>(skip / (FP8 ? 1 : 2) + panel * 64), static_cast<int>(a.slot), static_cast<int>(at.head), a.page);
+                                      static_cast<int>(skip / (FP8 ? 1 : 2) + panel * 64), static_cast<int>(a.slot), static_cast<int>(at.head),
+                                      a.page);
                     }
                     ++filled;
                     return true;
