@@ -288,3 +288,33 @@ def test_pages_more_than_32_bits_apart(ops, ctx, fp8):
     if not fp8:
         check_attention(*run_attention(ops, ctx, c, decode=True), c)
     assert ctx.read_device_error() == 0
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dim,heads", [(64, 8), (256, 4)])
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("said", [1, 384, 3000])
+def test_bounds_that_the_caller_says_too_small(ops, ctx, said, window, dim, heads, fp8):
+    """`max_kv_len` and `max_q_len` below the lengths there are: other kernels, the same results up to rounding."""
+    for q_len in ([1, 1, 1], [300, 1, 20]):
+        c = make_case(ops, q_len, [4000, 200, 20], heads=heads, kv_heads=2, dim=dim, fp8=fp8, seed=80)
+        for most in (1, 4, 1000):
+            check_attention(*run_attention(ops, ctx, c, max_kv_len=said, max_q_len=most, window=window), c, window=window)
+
+
+def test_single_tokens_over_far_8_bit_pages(ops, ctx):
+    """The streaming kernel over e4m3 pages 3 GiB apart with scales 1 GiB apart, against the codes and scales that lie there."""
+    kv_len, heads, kv_heads, dim, page = [300, 64, 1], 8, 2, 128, 128
+    c = make_case(ops, [1, 1, 1], kv_len, heads=heads, kv_heads=kv_heads, dim=dim, page=page, fp8=True, seed=52)
+    near, pages = c.cache, c.cache.k.shape[0]
+    room = torch.empty(pages * (3 << 30), dtype=torch.uint8, device="cuda")
+    room_scales = torch.empty(pages * (1 << 28), dtype=torch.float32, device="cuda")
+    far = lambda at: room.view(near.k.dtype).as_strided(near.k.shape, (3 << 30, page * dim, dim, 1), at * kv_heads * page * dim)
+    far_scales = lambda at: room_scales.as_strided((pages, kv_heads, page), (1 << 28, page, 1), at * kv_heads * page)
+    c.cache = ops.PagedKvCache(far(0), far(1), far_scales(0), far_scales(1))
+    for a, b in ((c.cache.k, near.k), (c.cache.v, near.v)):
+        a.view(torch.uint8).copy_(b.view(torch.uint8))
+    c.cache.k_scale.copy_(near.k_scale), c.cache.v_scale.copy_(near.v_scale)
+    for attempt in (dict(decode=True), dict()):
+        check_attention(*run_attention(ops, ctx, c, max_q_len=1, **attempt), c)
+    assert ctx.read_device_error() == 0
