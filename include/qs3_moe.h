@@ -966,8 +966,9 @@ typedef struct {
 } qs3_paged_kv_cache;
 
 /* Token p of sequence b lies in slot p % page_size of page kv_indices[kv_indptr[b] + p / page_size]. At most 4096 sequences.
- * The tables are read on the device. A page id outside the pool and a length beyond a sequence's pages are not followed:
- * such tokens count as zeros, or as absent, and qs3_moe_check_device_error reports 0x5d000001. */
+ * The tables are read on the device. A page id outside the pool is not followed: its tokens count as zeros. Neither is a length
+ * beyond a sequence's pages: tokens without a place are absent (neither written nor seen nor read back), the others and the new
+ * ones keep the positions that the length gives them. qs3_moe_check_device_error reports either as 0x5d000001. */
 typedef struct {
     qsfi_tensor1 kv_indptr;  /* i32 [batch + 1], ascending */
     qsfi_tensor1 kv_indices; /* i32 */
@@ -975,8 +976,8 @@ typedef struct {
 } qs3_page_table;
 
 /* Writes k and v of the new tokens into the cache. Rows q_indptr[b] .. q_indptr[b + 1] belong to sequence b (absent: row b
- * does), the i-th of n of them is token kv_len[b] - n + i; a row without one (n > kv_len[b], or behind the last sequence)
- * is left out. With inv_freq, k is turned on the way (before it is quantised) and, where given, q as well. */
+ * does), the i-th of n of them is token kv_len[b] - n + i; a row without one (n > kv_len[b], behind the last sequence, or
+ * beyond the sequence's pages) is left out. With inv_freq, k is turned on the way (before it is quantised) and, where given, q as well. */
 typedef struct {
     qs3_paged_kv_cache cache;
     qs3_page_table table;

@@ -181,7 +181,7 @@ __device__ __forceinline__ TokenPlace place_in_cache(const TurnParams& p, uint32
         return r;
     const SeqPages s = seq_pages(p.view, seq);
     const int64_t pos = static_cast<int64_t>(s.length) - fresh + within;
-    if (pos < 0)
+    if (pos < 0 || pos >= s.room)
         return r;
     uint32_t slot;
     const int64_t page = page_of(p.view, s, static_cast<uint32_t>(pos), &slot);
@@ -456,7 +456,7 @@ template <bool FP8> __global__ void __launch_bounds__(kRowThreads, 6) kv_gather_
             const int64_t pos = static_cast<int64_t>(row) - a + (p.start != nullptr ? p.start[seq] : 0);
             if (a <= row && b > row && pos >= 0) {
                 const SeqPages s = seq_pages(p.view, seq);
-                if (pos < s.length)
+                if (pos < s.room)
                     page = page_of(p.view, s, static_cast<uint32_t>(pos), &slot);
             }
         }

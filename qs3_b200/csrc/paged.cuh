@@ -36,31 +36,34 @@ struct PagedView {
 
 #ifdef __CUDACC__
 
-// Cached tokens of a sequence and where its page ids begin. Whatever the tables hold, the ids read for positions below the
-// returned length lie inside `indices`.
+// Tokens of a sequence, and where its page ids begin. Positions, masks and angles go by `length`, as the table says it; what may be
+// read or written by `room`, the tokens that its pages hold of them: whatever the tables hold, the ids of positions below it lie
+// inside `indices`.
 struct SeqPages {
     uint32_t first;  // index of the first page id
     uint32_t length; // tokens
+    uint32_t room;   // of them with a place, the first ones
 };
 
 __device__ __forceinline__ SeqPages seq_pages(const PagedView& p, uint32_t seq)
 {
     const int32_t a = p.indptr[seq], b = p.indptr[seq + 1], n = p.length[seq];
-    SeqPages s { 0, 0 };
+    SeqPages s { 0, 0, 0 };
     if (n <= 0)
         return s;
+    s.length = static_cast<uint32_t>(n);
     if (a >= 0 && b > a && static_cast<uint32_t>(a) < p.num_indices) {
         const uint32_t end = min(static_cast<uint32_t>(b), p.num_indices);
         const uint64_t room = static_cast<uint64_t>(end - a) * p.page_size;
         s.first = static_cast<uint32_t>(a);
-        s.length = static_cast<uint32_t>(min(room, static_cast<uint64_t>(n)));
+        s.room = static_cast<uint32_t>(min(room, static_cast<uint64_t>(n)));
     }
-    if (s.length != static_cast<uint32_t>(n))
+    if (s.room != s.length)
         atomicCAS(p.err, 0u, ERR_PAGE_TABLE);
     return s;
 }
 
-// Page of position `pos` < length, and the slot in it; -1: the table names a page that is not there.
+// Page of position `pos` < room, and the slot in it; -1: the table names a page that is not there.
 __device__ __forceinline__ int32_t page_of(const PagedView& p, const SeqPages& s, uint32_t pos, uint32_t* slot)
 {
     const uint32_t i = p.page_div.div(pos);

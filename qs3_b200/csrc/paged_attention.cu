@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kStreamThreads, StreamShape<D, NT, FP8>::kBloc
         uint32_t seen_lo, seen_hi, unused;
         visible_keys(p.tiling, rows.fresh, pages.length, p.tiling.group.div(row0), &seen_lo, &unused);
         visible_keys(p.tiling, rows.fresh, pages.length, p.tiling.group.div(row0 + nrows - 1), &unused, &seen_hi);
-        seen_hi = min(seen_hi, pages.length);
+        seen_hi = min(seen_hi, pages.room);
         // keys that the rows of this lane's columns see
         uint32_t lo[NT][2], hi[NT][2];
 #pragma unroll
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kStreamThreads, StreamShape<D, NT, FP8>::kBloc
                 lo[n][j] = hi[n][j] = 0;
                 if (r < nrows) {
                     visible_keys(p.tiling, rows.fresh, pages.length, p.tiling.group.div(row0 + r), &lo[n][j], &hi[n][j]);
-                    hi[n][j] = min(hi[n][j], pages.length);
+                    hi[n][j] = min(hi[n][j], pages.room);
                 }
             }
 

@@ -61,11 +61,11 @@ struct BlockRange {
 };
 
 // Cost of the items of a (sequence, KV head), by one warp.
-__device__ __forceinline__ uint64_t warp_tiles_cost(const AttnTiling& a, uint32_t fresh, uint32_t length, uint32_t tiles)
+__device__ __forceinline__ uint64_t warp_tiles_cost(const AttnTiling& a, uint32_t fresh, const SeqPages& s, uint32_t tiles)
 {
     uint64_t sum = 0;
     for (uint32_t t = threadIdx.x & 31; t < tiles; t += 32) {
-        const KeyTiles k = key_tiles(a, fresh, length, t);
+        const KeyTiles k = key_tiles(a, fresh, s.length, t, s.room);
         sum += cost_of(a, k.end - k.first);
     }
 #pragma unroll
@@ -86,9 +86,9 @@ __device__ BlockRange find_range(const AttnParams& p, uint64_t* cost, uint32_t b
         const uint32_t fresh = seq_rows(p, b).fresh, tiles = row_tiles(p.tiling, fresh);
         uint64_t sum = 0;
         if (tiles <= kSerialTiles) {
-            const uint32_t length = seq_pages(p.view, b).length;
+            const SeqPages s = seq_pages(p.view, b);
             for (uint32_t t = 0; t < tiles; ++t) {
-                const KeyTiles k = key_tiles(p.tiling, fresh, length, t);
+                const KeyTiles k = key_tiles(p.tiling, fresh, s.length, t, s.room);
                 sum += cost_of(p.tiling, k.end - k.first);
             }
         } else {
@@ -100,7 +100,7 @@ __device__ BlockRange find_range(const AttnParams& p, uint64_t* cost, uint32_t b
     for (uint32_t b = warp; b < batch; b += THREADS / 32) {
         if (cost[b] == kUnknown) {
             const uint32_t fresh = seq_rows(p, b).fresh;
-            const uint64_t sum = warp_tiles_cost(p.tiling, fresh, seq_pages(p.view, b).length, row_tiles(p.tiling, fresh));
+            const uint64_t sum = warp_tiles_cost(p.tiling, fresh, seq_pages(p.view, b), row_tiles(p.tiling, fresh));
             __syncwarp();
             if (lane == 0)
                 cost[b] = sum;
@@ -149,12 +149,13 @@ __device__ BlockRange find_range(const AttnParams& p, uint64_t* cost, uint32_t b
     r.place.seq = seq;
     r.place.head = static_cast<uint32_t>(inside / per_head);
     uint64_t rest = inside - r.place.head * per_head;
-    const uint32_t fresh = seq_rows(p, seq).fresh, length = seq_pages(p.view, seq).length;
+    const uint32_t fresh = seq_rows(p, seq).fresh;
+    const SeqPages pages = seq_pages(p.view, seq);
     const uint32_t tiles = row_tiles(p.tiling, fresh);
     for (uint32_t t0 = 0; t0 < tiles; t0 += 32) {
         uint32_t mine = 0;
         if (t0 + lane < tiles) {
-            const KeyTiles k = key_tiles(p.tiling, fresh, length, t0 + lane);
+            const KeyTiles k = key_tiles(p.tiling, fresh, pages.length, t0 + lane, pages.room);
             mine = cost_of(p.tiling, k.end - k.first);
         }
         uint64_t run = mine;
@@ -197,7 +198,8 @@ __device__ __forceinline__ void note_split(const AttnParams& p, const BlockRange
     SplitNote n { r.place.seq, r.place.head, r.place.tile, 0 };
     if (r.begin < r.end && r.place.offset > p.tiling.item_cost) { // (never with even items, which have an offset of 0)
         const uint64_t item = r.begin - r.place.offset;
-        const KeyTiles k = key_tiles(p.tiling, seq_rows(p, n.seq).fresh, seq_pages(p.view, n.seq).length, n.tile);
+        const SeqPages s = seq_pages(p.view, n.seq);
+        const KeyTiles k = key_tiles(p.tiling, seq_rows(p, n.seq).fresh, s.length, n.tile, s.room);
         if (block_begin(r.total, r.active, blockIdx.x - 1) <= item + p.tiling.item_cost) // (block 0 begins with an item)
             n.parts = block_of_end(r.total, r.active, item + p.tiling.item_cost + (k.end - k.first)) - blockIdx.x + 1;
     }
@@ -226,7 +228,7 @@ __device__ __forceinline__ bool this_segment(const AttnParams& p, const AttnPlac
     }
     if (s->rows.fresh == 0)
         return false;
-    const KeyTiles keys = key_tiles(p.tiling, s->rows.fresh, s->pages.length, at.tile);
+    const KeyTiles keys = key_tiles(p.tiling, s->rows.fresh, s->pages.length, at.tile, s->pages.room);
     const uint32_t tiles = s->tiles = keys.end - keys.first;
     const uint32_t from = tiles_before(p.tiling, at.offset, tiles), to = tiles_before(p.tiling, at.offset + left, tiles);
     if (from >= to)

@@ -371,7 +371,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
             uint32_t seen_lo, seen_hi, unused;
             visible_keys(p.tiling, seg.rows.fresh, seg.pages.length, p.tiling.group.div(seg.row0), &seen_lo, &unused);
             visible_keys(p.tiling, seg.rows.fresh, seg.pages.length, p.tiling.group.div(seg.row0 + seg.nrows - 1), &unused, &seen_hi);
-            seen_hi = min(seen_hi, seg.pages.length);
+            seen_hi = min(seen_hi, seg.pages.room);
 
             const auto load_query = [&] {
                 if (!wait(&bar.q_free, (segments & 1) ^ 1, ERR_PF_QUERY_WAIT))
@@ -455,7 +455,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 const auto look = [&](uint32_t piece) {
                     Places l;
                     const uint32_t key0 = first_key(piece);
-                    l.boxes = v_box != 0 && key0 >= seen_lo && key0 + PIECE_KEYS <= seg.pages.length;
+                    l.boxes = v_box != 0 && key0 >= seen_lo && key0 + PIECE_KEYS <= seg.pages.room;
 #pragma unroll
                     for (uint32_t j = 0; j < SETS; ++j) {
                         const uint32_t key = key0 + (l.boxes ? lane * v_box : j * 32 + lane);
@@ -646,7 +646,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 const uint32_t keys = value ? PIECE_KEYS : kKeyTile, box = value ? v_box : k_box;
                 a.slot = 0;
                 a.page = 0;
-                a.boxes = box != 0 && a.key0 >= seen_lo && a.key0 + keys <= seg.pages.length;
+                a.boxes = box != 0 && a.key0 >= seen_lo && a.key0 + keys <= seg.pages.room;
                 if (a.boxes) {
                     const uint32_t per_panel = keys / box, panels = value ? D / 64 : PANELS;
                     if (lane < per_panel * panels)
@@ -870,7 +870,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 uint32_t lo = 0, hi = 0xffffffffu; // (rows past the last one need no mask)
                 if (live) {
                     visible_keys(p.tiling, seg.rows.fresh, seg.pages.length, token, &lo, &hi);
-                    hi = min(hi, seg.pages.length);
+                    hi = min(hi, seg.pages.room);
                 }
                 float m = -INFINITY, l = 0.0f, q_scale = 1.0f;
                 for (uint32_t u = 0; u < steps; ++u, ++done) {

@@ -70,13 +70,16 @@ QS3_HD void visible_keys(const AttnTiling& a, uint32_t fresh, uint32_t length, u
     *lo = l <= 0 ? 0 : l < h ? static_cast<uint32_t>(l) : *hi;
 }
 
-QS3_HD KeyTiles key_tiles(const AttnTiling& a, uint32_t fresh, uint32_t length, uint32_t tile)
+// `room`: the first keys of the sequence, which are there to be seen.
+QS3_HD KeyTiles key_tiles(const AttnTiling& a, uint32_t fresh, uint32_t length, uint32_t tile, uint32_t room = 0xffffffffu)
 {
     const uint32_t rows = fresh * a.group.d, r0 = tile << a.row_shift, next = r0 + (1u << a.row_shift);
     const uint32_t r1 = (next < rows ? next : rows) - 1;
     uint32_t lo, hi, unused;
     visible_keys(a, fresh, length, a.group.div(r0), &lo, &unused);
     visible_keys(a, fresh, length, a.group.div(r1), &unused, &hi);
+    hi = hi < room ? hi : room;
+    lo = lo < room ? lo : room;
     KeyTiles k;
     k.first = lo >> a.key_shift;
     k.end = (hi + (1u << a.key_shift) - 1) >> a.key_shift;

@@ -79,8 +79,9 @@ def make_case(ops, q_len, kv_len, *, heads, kv_heads, dim, page=16, fp8=False, s
                 ops.PagedKvCache(*pools, *scales), ints(running(q_len)), truth[0], truth[1], q, sum(q_len))
 
 
-def attention_reference(c: Case, *, causal=True, window=0, scale=None, q_off=0.0):
-    """out, lse in 64 bits, and the most that each may be off.
+def attention_reference(c: Case, *, causal=True, window=0, scale=None, q_off=0.0, said=None):
+    """out, lse in 64 bits, and the most that each may be off. `said`: the lengths that the page table gives, where they are more
+    than the pages hold; kv_len counts the tokens there are.
 
     A kernel computes scores in 32 bits (each product's sum off by at most (D + 8) 2^-24 of the sum of the magnitudes, the
     weights by e to that, and by a few units of 2^-22 for the exponential), rounds the weights to bf16 (2^-8 of each, half a
@@ -93,7 +94,8 @@ def attention_reference(c: Case, *, causal=True, window=0, scale=None, q_off=0.0
     lse_bound = torch.zeros_like(lse)
     row = 0
     for b, (n, length) in enumerate(zip(c.q_len, c.kv_len)):
-        pos = torch.arange(length - n, length, device="cuda")[:, None]
+        last = length if said is None else said[b]
+        pos = torch.arange(last - n, last, device="cuda")[:, None]
         j = torch.arange(length, device="cuda")[None]
         seen = (j <= pos) if causal else (j >= 0).expand(n, length)
         if window:

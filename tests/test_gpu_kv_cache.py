@@ -295,3 +295,41 @@ def test_steps_of_a_serving_loop(ops, ctx, dim, heads, kv_heads, fp8):
         c = Case(q_len, lengths, page, heads, kv_heads, dim, table, cache, indptr, truth[0], truth[1], q, sum(q_len))
         check_attention(*run_attention(ops, ctx, c), c)
     assert ctx.read_device_error() == 0
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("q_len", [[1, 1, 1], [2, 30, 40]])
+def test_tokens_beyond_the_pages_have_no_place(ops, ctx, q_len, fp8):
+    """New tokens keep their positions where a length says more than the pages hold: those beyond drop out, and nothing else moves."""
+    said, rooms, kv_heads, heads, dim, page = [20, 60, 500], [32, 48, 48], 2, 4, 64, 16
+    cache, table, indptr = empty_cache(ops, q_len, rooms, kv_heads=kv_heads, dim=dim, page=page, fp8=fp8, seed=3)
+    table.kv_len.copy_(ints(said))
+    roomy, wide, wide_indptr = empty_cache(ops, q_len, said, kv_heads=kv_heads, dim=dim, page=page, fp8=fp8, seed=4)
+    before = [x.clone() for x in raw(cache)]
+    rows = sum(q_len)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    q, k, v = (torch.randn((rows, h, dim), generator=gen, device="cuda").to(torch.bfloat16) for h in (heads, kv_heads, kv_heads))
+    f = ops.rope_frequencies(16)
+    outs = [torch.full_like(q, 7.0) for _ in range(2)]
+    for c, t, out in ((roomy, wide, outs[0]), (cache, table, outs[1])):
+        assert ctx.read_device_error() == 0
+        ops.kv_append(ctx, c, t, k, v, q_indptr=None if max(q_len) == 1 else ints(running(q_len)), q=q, q_out=out, inv_freq=f.inv_freq)
+    torch.cuda.synchronize()
+    assert ctx.read_device_error() == 0x5d000001
+    touched = torch.zeros((before[0].shape[0], kv_heads, page), dtype=torch.bool, device="cuda")
+    row = 0
+    for b, n in enumerate(q_len):
+        for i in range(n):
+            pos, r = said[b] - n + i, row + i
+            if pos >= rooms[b]:
+                assert bool((outs[1][r] == 7.0).all())
+                continue
+            assert torch.equal(outs[1][r], outs[0][r])
+            at = (int(table.kv_indices[indptr[b] + pos // page]), slice(None), pos % page)
+            there = (int(wide.kv_indices[wide_indptr[b] + pos // page]), slice(None), pos % page)
+            touched[at] = True
+            for x, y in zip(raw(cache), raw(roomy)):
+                assert torch.equal(x[at], y[there])
+        row += n
+    for a, b in zip(before, raw(cache)):
+        assert torch.equal(a[~touched], b[~touched])

@@ -318,3 +318,20 @@ def test_single_tokens_over_far_8_bit_pages(ops, ctx):
     for attempt in (dict(decode=True), dict()):
         check_attention(*run_attention(ops, ctx, c, max_q_len=1, **attempt), c)
     assert ctx.read_device_error() == 0
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 8, 2), (128, 8, 2), (256, 4, 1)])
+@pytest.mark.parametrize("q_len,rooms,said", [
+    ([400, 3, 2], [304, 64, 48], [500, 64, 1000000]),
+    ([1, 1, 1], [9008, 64, 48], [9500, 70, (1 << 31) - 1]),
+])
+@pytest.mark.parametrize("kw", [dict(), dict(window=250), dict(causal=False)])
+def test_lengths_beyond_the_pages(ops, ctx, kw, q_len, rooms, said, dim, heads, kv_heads, fp8):
+    """Rows stay at the positions that the length gives them, and see of the keys before them those that are there."""
+    c = make_case(ops, q_len, rooms, heads=heads, kv_heads=kv_heads, dim=dim, fp8=fp8, seed=60 + dim, tail=1)
+    c.table.kv_len.copy_(ints(said))
+    check_attention(*run_attention(ops, ctx, c, **kw), c, said=said, **kw)
+    if max(q_len) == 1:
+        check_attention(*run_attention(ops, ctx, c, decode=True, **kw), c, said=said, **kw)
+    assert ctx.read_device_error() == 0x5d000001

@@ -308,3 +308,47 @@ def test_workspace_size(lib, ctx):
         assert lib.qs3_paged_attention_workspace_size(ctx, *args, C.byref(n)) == INVALID
     assert lib.qs3_paged_attention_workspace_size(ctx, 8, 8, 16, 2, 80, C.byref(n)) == UNSUPPORTED
     assert lib.qs3_paged_attention_workspace_size(ctx, 8, 8, 16, 2, 64, None) == INVALID
+
+
+ROOM_PROGRAM = r"""
+#include "paged_schedule.h"
+#include <cstdio>
+#include <initializer_list>
+using namespace qs3;
+#define CHECK(x) do { if (!(x)) { std::printf("line %d: %s\n", __LINE__, #x); return 1; } } while (0)
+int main()
+{
+    // an item's key tiles hold every key that is there and that a row sees by the stated length, and none that lies behind them
+    for (uint32_t key_shift : { 6u, 7u })
+    for (uint32_t window : { 0u, 1u, 200u })
+    for (uint32_t causal : { 0u, 1u })
+    for (uint32_t fresh : { 1u, 3u, 70u, 257u })
+    for (uint32_t length : { 1u, 64u, 300u, 1000u, 0x7fffffffu })
+    for (uint32_t room : { 0u, 1u, 63u, 64u, 65u, 128u, 290u, 300u }) {
+        if ((window != 0 && causal == 0) || room > length)
+            continue;
+        const AttnTiling a { FastDiv(4), 7, key_shift, 2, window, causal, 0 };
+        for (uint32_t t = 0; t < row_tiles(a, fresh); ++t) {
+            const KeyTiles k = key_tiles(a, fresh, length, t, room);
+            CHECK(k.end > k.first);
+            CHECK(k.end == k.first + 1 || (uint64_t(k.end - 1) << key_shift) < room);
+            CHECK((uint64_t(k.first) << key_shift) <= room);
+            for (uint32_t r = t * 128; r < (t + 1) * 128 && r < fresh * 4; ++r) {
+                const int64_t pos = int64_t(length) - fresh + r / 4;
+                for (int64_t j = 0; j < room; ++j)
+                    if ((!causal || j <= pos) && (!window || j > pos - int64_t(window)))
+                        CHECK((uint32_t(j) >> key_shift) >= k.first && (uint32_t(j) >> key_shift) < k.end);
+            }
+        }
+    }
+    return 0;
+}
+"""
+
+
+def test_key_tiles_stay_inside_the_pages(tmp_path):
+    src, exe = tmp_path / "room.cpp", tmp_path / "room"
+    src.write_text(ROOM_PROGRAM)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-Werror", f"-I{CSRC}", str(src), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout
