@@ -1005,9 +1005,9 @@ qsfi_status qs3_kv_gather(qsfi_context* ctx, const qs3_kv_gather_desc* desc);
 /* Attention of new tokens over the cache, which holds them already:
  *   s_j = sm_scale * q . k_j,  out = sum_j softmax(s)_j v_j,  lse = log sum_j exp(s_j)
  * over the tokens j that row i of n of sequence b sees: with p = kv_len[b] - n + i all j <= p (causal; else all
- * j < kv_len[b]), and j > p - window where there is one. A row that sees none gets 0 and -infinity. Query heads
- * h * group .. h * group + group - 1 share KV head h. Head sizes 64, 128 and 256. Sums, maxima and the exponents are in
- * 32 bits; the weights exp(s_j - max), times v's scales, are rounded to bf16 (bf16 caches) or f16 (e4m3 ones) for the product
+ * j < kv_len[b]), and j > p - window where there is one. A row that sees none gets 0 and -infinity, one whose
+ * scores are all -infinity NaN. Query heads h * group .. h * group + group - 1 share KV head h. Head sizes 64, 128 and 256. Sums,
+ * maxima and the exponents are in 32 bits; the weights exp(s_j - max), times v's scales, are rounded to bf16 (bf16 caches) or f16 (e4m3 ones) for the product
  * with v, and with e4m3 caches an element of q may be off by 2^-17 of the largest of its row. v has to be finite at every
  * token of a sequence, also at those that a row does not see, as 0 * inf is NaN; a row of q with an infinity or a NaN gets
  * NaN. What k holds where a row does not see it, and what lies in the pages behind a sequence's end, does not matter. */

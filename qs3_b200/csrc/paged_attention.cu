@@ -475,12 +475,13 @@ __global__ void __launch_bounds__(kStreamThreads, StreamShape<D, NT, FP8>::kBloc
             }
             if (whole) {
                 const uint32_t token = p.tiling.group.div(row0 + r), h = at.head * p.tiling.group.d + row0 + r - token * p.tiling.group.d;
-                const float inv = top == -INFINITY ? 0.0f : kSumFactor<FP8> / sum;
+                const bool scored = top != -INFINITY;
+                const float inv = scored ? kSumFactor<FP8> / sum : without_scores(p, rows.fresh, pages, row0 + r);
                 const uint2 w = make_uint2(tc::pack_bf16x2(acc.x * inv, acc.y * inv), tc::pack_bf16x2(acc.z * inv, acc.w * inv));
                 *reinterpret_cast<uint2*>(p.out + (rows.row0 + token) * p.out_token + h * p.out_head + e * 2) = w;
                 if (e == 0 && p.lse != nullptr)
                     p.lse[(rows.row0 + token) * p.lse_token + h * p.lse_head]
-                        = sum == 0.0f ? -INFINITY : (top + kUnits + log2f(sum)) * 0.693147180559945f;
+                        = scored ? (top + kUnits + log2f(sum)) * 0.693147180559945f : inv == 0.0f ? -INFINITY : inv;
             } else {
                 constexpr float f = kSumFactor<FP8>;
                 *reinterpret_cast<float4*>(p.part_o + (static_cast<size_t>(slot) * ROWS + r) * D + e)
@@ -565,7 +566,8 @@ template <uint32_t D, bool SHARED> __global__ void __launch_bounds__(kJoinWarps 
                 for (uint32_t w = 1; w < kJoinWarps; ++w)
                     acc[j] += s_acc[w * D + lane * E + j];
         }
-        const float inv = top == -INFINITY ? 0.0f : 1.0f / sum;
+        const bool scored = top != -INFINITY;
+        const float inv = scored ? 1.0f / sum : without_scores(p, rows.fresh, seq_pages(p.view, n.seq), row0 + r);
         const uint32_t token = p.tiling.group.div(row0 + r), h = n.head * p.tiling.group.d + row0 + r - token * p.tiling.group.d;
         uint8_t* out = p.out + (rows.row0 + token) * p.out_token + h * p.out_head + lane * E * 2;
         uint32_t w[E / 2];
@@ -580,7 +582,7 @@ template <uint32_t D, bool SHARED> __global__ void __launch_bounds__(kJoinWarps 
             *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
         if (lane == 0 && p.lse != nullptr)
             p.lse[(rows.row0 + token) * p.lse_token + h * p.lse_head]
-                = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
+                = scored ? (top + log2f(sum)) * 0.693147180559945f : inv == 0.0f ? -INFINITY : inv;
     }
 }
 

@@ -177,6 +177,15 @@ __device__ BlockRange find_range(const AttnParams& p, uint64_t* cost, uint32_t b
     return r;
 }
 
+// What becomes of a row without a score above -infinity: zeros (and a log-sum-exp of -infinity) where it sees no key, NaN where it
+// sees some, of which no softmax exists.
+__device__ __forceinline__ float without_scores(const AttnParams& p, uint32_t fresh, const SeqPages& s, uint32_t row)
+{
+    uint32_t lo, hi;
+    visible_keys(p.tiling, fresh, s.length, p.tiling.group.div(row), &lo, &hi);
+    return lo < min(hi, s.room) ? __int_as_float(0x7fffffff) : 0.0f;
+}
+
 // The item after the one at `at`; sequences without new tokens have none.
 __device__ __forceinline__ void next_item(const AttnParams& p, AttnPlace* at, uint32_t tiles)
 {

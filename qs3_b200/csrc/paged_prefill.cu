@@ -999,14 +999,16 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 if (!ok)
                     break;
                 const bool whole = seg.whole;
+                const bool scored = m != -INFINITY;
+                const float none = lo < hi ? __int_as_float(0x7fffffff) : 0.0f; // without a score: as in without_scores
                 // in units of the sums: O counts 2^kSumUnit times too much
-                if (m != -INFINITY)
+                if (scored)
                     m += kSumUnit<FP8> - kTop<FP8>;
                 const uint32_t h = at.head * p.tiling.group.d + flat - token * p.tiling.group.d;
                 const size_t part_row = static_cast<size_t>(blockIdx.x * 2 + (seg.starts ? 1 : 0)) * Shape::kRows + r;
                 uint8_t* const out = p.out + (seg.rows.row0 + token) * p.out_token + h * p.out_head;
                 float* const part_o = p.part_o + part_row * D;
-                const float inv = whole ? (m == -INFINITY ? 0.0f : kSumFactor<FP8> / l) : kSumFactor<FP8>;
+                const float inv = whole ? (scored ? kSumFactor<FP8> / l : none) : kSumFactor<FP8>;
                 uint32_t x[32];
 #pragma unroll 1
                 for (uint32_t i = 0; i < D / 32 / (TILES == 1 ? 2 : 1); ++i) {
@@ -1038,7 +1040,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     mbar_arrive(&bar.o_free[q]);
                 if (live && whole && half == 0 && p.lse != nullptr)
                     p.lse[(seg.rows.row0 + token) * p.lse_token + h * p.lse_head]
-                        = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
+                        = scored ? (m + log2f(l)) * 0.693147180559945f : none == 0.0f ? -INFINITY : none;
                 if (live && !whole && half == 0)
                     p.part_ml[part_row] = make_float2(m, l);
             }

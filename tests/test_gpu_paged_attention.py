@@ -335,3 +335,53 @@ def test_lengths_beyond_the_pages(ops, ctx, kw, q_len, rooms, said, dim, heads, 
     if max(q_len) == 1:
         check_attention(*run_attention(ops, ctx, c, decode=True, **kw), c, said=said, **kw)
     assert ctx.read_device_error() == 0x5d000001
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+@pytest.mark.parametrize("q_len,kv_len", [([1, 1], [1, 90]), ([40, 1], [40, 2]), ([1, 1], [9000, 3]), ([30, 1], [6000, 3])])
+def test_scores_that_are_all_infinite(ops, ctx, q_len, kv_len, sign, dim, fp8):
+    """A query element of infinity over keys of one sign there: every score is an infinity of that sign, and no softmax exists."""
+    c = make_case(ops, q_len, kv_len, heads=4, kv_heads=2, dim=dim, fp8=fp8, seed=70)
+    good, good_lse = run_attention(ops, ctx, c)
+    pages = c.table.kv_indices.long()
+    if fp8:
+        c.cache.k.view(torch.uint8)[pages, ..., 5] = 0xb8 if sign < 0 else 0x38
+    else:
+        c.cache.k[pages, ..., 5] = sign
+    c.q[..., 5] = 0.0
+    good, good_lse = run_attention(ops, ctx, c)
+    assert bool(torch.isfinite(good).all()) and bool(torch.isfinite(good_lse).all())
+    row = q_len[0] - 1
+    c.q[row, 1, 5] = math.inf
+    out, lse = run_attention(ops, ctx, c)
+    assert bool(out[row, 1].isnan().all()) and bool(lse[row, 1].isnan())
+    out[row, 1], lse[row, 1] = good[row, 1], good_lse[row, 1]
+    assert torch.equal(out, good) and torch.equal(lse, good_lse)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_keys_of_minus_infinity_alone(ops, ctx, fp8):
+    """Rows that see keys but no finite score are NaN, rows that see no key 0 and -infinity, in one call."""
+    for q_len, kv_len in (([1, 1, 1], [3, 70, 0]), ([2, 40, 20], [3, 70, 9])):
+        c = make_case(ops, q_len, kv_len, heads=4, kv_heads=2, dim=64, fp8=fp8, seed=71)
+        c.q.abs_()
+        page = int(c.table.kv_indices[0])
+        if fp8:
+            c.cache.k.view(torch.uint8)[page] = 0xb8
+            c.cache.k_scale[page] = math.inf
+        else:
+            c.cache.k[page] = -math.inf
+        out, lse = run_attention(ops, ctx, c)
+        row = 0
+        for b, n in enumerate(q_len):
+            for i in range(n):
+                o, l = out[row + i].float(), lse[row + i]
+                if b == 0:
+                    assert bool(o.isnan().all()) and bool(l.isnan().all())
+                elif kv_len[b] - n + i < 0:
+                    assert bool((o == 0).all()) and bool((l == -math.inf).all())
+                else:
+                    assert bool(torch.isfinite(o).all()) and bool(torch.isfinite(l).all())
+            row += n
