@@ -759,9 +759,13 @@ class PageTable:
     kv_len: torch.Tensor
 
 
+_CODES = (torch.float8_e4m3fn, torch.uint8)
+
+
 def _fill_paged(d, layouts, cache: PagedKvCache, table: PageTable, *tensors):
-    if cache.fp8 and not (cache.k.element_size() == cache.v.element_size() == 1):
-        raise Qs3Error(capi.STATUS_INVALID_ARGUMENT, "a cache with scales holds 8-bit codes")
+    if cache.fp8 and not (cache.k.dtype in _CODES and cache.v.dtype in _CODES):
+        raise Qs3Error(capi.STATUS_INVALID_ARGUMENT,
+                       f"a cache with scales holds e4m3 codes (float8_e4m3fn or u8), not {cache.k.dtype} and {cache.v.dtype}")
     _fill(d, layouts[1 if cache.fp8 else 0], cache.k, cache.v, cache.k_scale, cache.v_scale, table.kv_indptr,
           table.kv_indices, table.kv_len, *tensors)
 

@@ -352,3 +352,33 @@ def test_key_tiles_stay_inside_the_pages(tmp_path):
     subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-Werror", f"-I{CSRC}", str(src), "-o", str(exe)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout
+
+
+def paged_call(name, pool_dtype, scales=True):
+    """A call of ops.<name> on small CPU tensors, by a context without a device: what is refused is refused before any of them is read."""
+    import torch
+
+    from qs3_b200 import ops
+    new = lambda *shape, dtype=torch.bfloat16: torch.zeros(shape, dtype=dtype)
+    i32 = lambda n: new(n, dtype=torch.int32)
+    scale = lambda: new(4, 2, 16, dtype=torch.float32) if scales else None
+    pool = lambda: new(4, 2, 16, 64, dtype=torch.uint8).view(pool_dtype) if pool_dtype.itemsize == 1 else new(4, 2, 16, 64, dtype=pool_dtype)
+    c = ops.PagedKvCache(pool(), pool(), scale(), scale())
+    p, ctx = ops.PageTable(i32(4), i32(8), i32(3)), ops.Context(device=-1)
+    if name == "kv_append":
+        ops.kv_append(ctx, c, p, new(3, 2, 64), new(3, 2, 64))
+    elif name == "kv_gather":
+        ops.kv_gather(ctx, c, p, i32(4), new(3, 2, 64), new(3, 2, 64))
+    else:
+        ops.paged_attention(ctx, new(3, 4, 64), c, p, new(3, 4, 64), new(1 << 16, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("name", ["kv_append", "kv_gather", "paged_attention"])
+@pytest.mark.parametrize("dtype", ["float8_e5m2", "int8", "bool", "float8_e4m3fnuz", "bfloat16"])
+def test_codes_of_another_kind_are_refused(name, dtype):
+    import torch
+
+    from qs3_b200 import ops
+    with pytest.raises(ops.Qs3Error, match="e4m3 codes") as e:
+        paged_call(name, getattr(torch, dtype))
+    assert e.value.status == INVALID
