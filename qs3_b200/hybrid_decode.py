@@ -295,7 +295,9 @@ class HybridDecoder:
             self.embed = _normal((cfg.vocab, h), 0.02, gen, dev)
             self.lm_head = _normal((cfg.vocab, h), 0.02, gen, dev)
             self.input_norm = [torch.ones(h, dtype=torch.bfloat16, device=dev) for _ in range(cfg.layers + 1)]
-            self.kv_len = torch.full((b,), cfg.context, dtype=torch.int32, device=dev)   # paged attention: cached tokens
+            self.kv_len = None   # paged attention: cached tokens, the new one included
+            if cfg.attention == "paged":
+                self.kv_len = torch.full((b,), cfg.context, dtype=torch.int32, device=dev)
             self.mixers, self.blocks = [], []
             for layer in range(cfg.layers):
                 if not cfg.is_attention(layer):
@@ -340,7 +342,8 @@ class HybridDecoder:
         # the device-side position is clamped as well, so that no replay can index past the cache
         pos = self.pos.clamp(max=self.max_len - 1)
         self.mask.index_fill_(2, pos, 0.0)               # the new token attends to itself
-        self.kv_len.copy_((pos + 1).expand(cfg.batch))
+        if self.kv_len is not None:
+            self.kv_len.copy_((pos + 1).expand(cfg.batch))
         self.residual.copy_(self.embed.index_select(0, self.tokens))
         ops.rmsnorm(ctx, self.residual, self.input_norm[0], self.x, cfg.eps)
         for layer, (mixer, blk) in enumerate(zip(self.mixers, self.blocks)):

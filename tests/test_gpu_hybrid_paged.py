@@ -107,3 +107,15 @@ def test_an_unknown_attention_is_refused():
     for kw in (dict(attention="flat"), dict(kv_fp8=True)):
         with pytest.raises(ValueError, match="attention"):
             HybridDecoder(tiny_config(**kw))
+
+
+def test_lengths_are_kept_for_paged_attention_only():
+    """The torch stand-in reads no lengths, and its step writes none."""
+    from qs3_b200.hybrid_decode import HybridDecoder, tiny_config
+    assert HybridDecoder(tiny_config()).kv_len is None
+    model = HybridDecoder(tiny_config(attention="paged"))
+    with torch.cuda.stream(model.stream):
+        model.ctx.use_current_stream()
+        model.step()
+        model.stream.synchronize()
+    assert bool((model.kv_len == model.cfg.context + 1).all())
