@@ -182,9 +182,10 @@ class _Attention:
 class _PagedAttention(_Attention):
     """The same layer with this library's operators from the norms to the gate: q and k are rotated and k and v
     written to the cache in one pass, and attention reads the pages where they lie. `kv_len` (i32 [batch]) counts the
-    cached tokens, the new one included; it is the caller's, one for all layers."""
+    cached tokens, the new one included; it is the caller's, one for all layers, and so may be the workspace of layers that
+    run one after another."""
 
-    def __init__(self, cfg: HybridConfig, gen, dev, max_len, ctx: ops.Context, kv_len: torch.Tensor):
+    def __init__(self, cfg: HybridConfig, gen, dev, max_len, ctx: ops.Context, kv_len: torch.Tensor, workspace=None):
         super().__init__(cfg, gen, dev, max_len)
         self.ctx, self.kv_len = ctx, kv_len
         self.freq = ops.rope_frequencies(cfg.rotary_dim, 10000.0, device=dev)
@@ -194,7 +195,7 @@ class _PagedAttention(_Attention):
         b, d = cfg.batch, cfg.head_dim
         self.workspace = torch.empty(ops.paged_attention_workspace_size(
             ctx, torch.empty((b, cfg.q_heads, d), dtype=torch.bfloat16, device="meta"), self._cache(), batch=b),
-            dtype=torch.uint8, device=dev)
+            dtype=torch.uint8, device=dev) if workspace is None else workspace
 
     def _cache(self):
         return ops.PagedKvCache(self.k_pool, self.v_pool, self.k_scale, self.v_scale)
@@ -299,11 +300,13 @@ class HybridDecoder:
             if cfg.attention == "paged":
                 self.kv_len = torch.full((b,), cfg.context, dtype=torch.int32, device=dev)
             self.mixers, self.blocks = [], []
+            attention_ws = None      # of the first paged attention layer, for all of them: they run on one stream
             for layer in range(cfg.layers):
                 if not cfg.is_attention(layer):
                     self.mixers.append(_GatedDeltaNet(cfg, gen, dev))
                 elif cfg.attention == "paged":
-                    self.mixers.append(_PagedAttention(cfg, gen, dev, self.max_len, self.ctx, self.kv_len))
+                    self.mixers.append(_PagedAttention(cfg, gen, dev, self.max_len, self.ctx, self.kv_len, attention_ws))
+                    attention_ws = self.mixers[-1].workspace
                 else:
                     self.mixers.append(_Attention(cfg, gen, dev, self.max_len))
                 self.blocks.append(_MoeBlock(self.ctx, cfg, gen, dev, keep_linear_scales))

@@ -119,3 +119,10 @@ def test_lengths_are_kept_for_paged_attention_only():
         model.step()
         model.stream.synchronize()
     assert bool((model.kv_len == model.cfg.context + 1).all())
+
+
+def test_attention_layers_share_one_workspace():
+    from qs3_b200.hybrid_decode import HybridDecoder, _PagedAttention, tiny_config
+    model = HybridDecoder(tiny_config(layers=8, attention="paged"))
+    layers = [m for m in model.mixers if isinstance(m, _PagedAttention)]
+    assert len(layers) == 2 and len({m.workspace.data_ptr() for m in layers}) == 1
