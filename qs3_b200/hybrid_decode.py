@@ -224,12 +224,16 @@ class _PagedAttention(_Attention):
         kv = (x @ self.w_kv.t()).view(b, 2, kvh, d)
         norm = lambda t: (t.float() * torch.rsqrt(t.float().pow(2).mean(-1, keepdim=True) + cfg.eps)).to(t.dtype)
         q, k, v = norm(q), norm(kv[:, 0]), kv[:, 1]
-        table = ops.PageTable(self.kv_indptr, self.kv_indices, self.kv_len)
-        ops.kv_append(self.ctx, self._cache(), table, k, v, q=q, inv_freq=self.freq.inv_freq, rope_scale=self.freq.scale)
-        out = torch.empty_like(q)
-        ops.paged_attention(self.ctx, q, self._cache(), table, out, self.workspace)
-        out = out * torch.sigmoid(gate.float()).to(x.dtype)
+        out = self.attend(q, k, v, q) * torch.sigmoid(gate.float()).to(x.dtype)
         return out.reshape(b, qh * d) @ self.w_o.t()
+
+    def attend(self, q, k, v, q_out):
+        """The library's part of the layer: k (rotated) and v into the cache, q rotated to `q_out`, and attention."""
+        table = ops.PageTable(self.kv_indptr, self.kv_indices, self.kv_len)
+        ops.kv_append(self.ctx, self._cache(), table, k, v, q=q, q_out=q_out, inv_freq=self.freq.inv_freq, rope_scale=self.freq.scale)
+        out = torch.empty_like(q_out)
+        ops.paged_attention(self.ctx, q_out, self._cache(), table, out, self.workspace)
+        return out
 
 
 class _GatedDeltaNet:
@@ -327,6 +331,10 @@ class HybridDecoder:
             self.tiled = torch.zeros(ops.nvfp4_tiled_scale_bytes(b, h), dtype=torch.uint8, device=dev)
             self.logits = torch.empty((b, cfg.vocab), dtype=torch.bfloat16, device=dev)
             self.stale_mix = _normal((b, h), 0.1, gen, dev)
+            self.stale_qkv = None    # what paged attention is given in a step without the mixers' torch operators
+            if cfg.attention == "paged":
+                self.stale_qkv = _normal((b, cfg.q_heads + 2 * cfg.kv_heads, cfg.head_dim), 1.0, gen, dev).split(
+                    [cfg.q_heads, cfg.kv_heads, cfg.kv_heads], dim=1)
             self.ids = torch.empty((b, cfg.top_k), dtype=torch.int32, device=dev)
             self.weights = torch.empty((b, cfg.top_k), dtype=torch.float32, device=dev)
         self.stream.synchronize()
@@ -338,8 +346,9 @@ class HybridDecoder:
 
     def step(self, mixers: bool = True):
         """One token for every sequence, enqueued on `self.stream` (must be current).
-        mixers=False skips the torch stand-ins (each layer then consumes a fixed tensor in
-        place of its mixer output): what remains are the calls into this library."""
+        mixers=False skips the mixers' torch operators (each layer then consumes a fixed tensor in
+        place of its mixer output): what remains are the calls into this library, those of paged
+        attention on fixed q, k and v included."""
         cfg, ctx = self.cfg, self.ctx
         self._advance()
         # the device-side position is clamped as well, so that no replay can index past the cache
@@ -352,6 +361,8 @@ class HybridDecoder:
         for layer, (mixer, blk) in enumerate(zip(self.mixers, self.blocks)):
             if not mixers:
                 mix = self.stale_mix.clone()
+                if isinstance(mixer, _PagedAttention):
+                    mixer.attend(*self.stale_qkv, q_out=torch.empty_like(self.stale_qkv[0]))
             elif cfg.is_attention(layer):
                 mix = mixer(self.x, pos, self.mask)
             else:
@@ -468,7 +479,7 @@ class HybridDecoder:
 
 def measure(steps: int | None = None, cfg: HybridConfig | None = None) -> dict:
     """Build the decoder, time `steps` decoded tokens per sequence (default: the configuration's 256)
-    as CUDA-graph replays with and without the mixers, and return the record `main` prints."""
+    as CUDA-graph replays, whole and of this library's calls alone, and return the record `main` prints."""
     cfg = cfg or HybridConfig()
     steps = cfg.new_tokens if steps is None else steps
     model = HybridDecoder(cfg)
@@ -477,15 +488,18 @@ def measure(steps: int | None = None, cfg: HybridConfig | None = None) -> dict:
     lib = model.time_steps(steps, mixers=False)
     err = model.ctx.read_device_error()
     moe_bytes = cfg.moe_weight_bytes_per_layer() * cfg.layers
+    paged = cfg.attention == "paged"
     return {
         "metric": "hybrid decode tokens/s (batch x steps / time), CUDA graph replay", "value": cfg.batch / (full * 1e-3),
         "unit": "tokens/s", "ms_per_step": full, "library_ms_per_step": lib, "library_share": lib / full,
-        "library_calls": "rmsnorm, fused add+rmsnorm+NVFP4, MoE layer (+ residual add + next norm), LM head",
-        "moe_weight_bytes_per_step": moe_bytes, "moe_weight_stream_gbs": moe_bytes / (lib * 1e-3) / 1e9,
+        "library_calls": "rmsnorm, fused add+rmsnorm+NVFP4, MoE layer (+ residual add + next norm), LM head"
+                         + (", rotary positions + cache write, paged attention" if paged else ""),
+        # (the library's time takes in paged attention, where it is this library's)
+        "moe_weight_bytes_per_step": moe_bytes, "moe_weight_stream_gbs": None if paged else moe_bytes / (lib * 1e-3) / 1e9,
         "mixers": f"torch stand-ins (gated attention over a paged KV cache, {cfg.page_size}-token pages behind a CSR "
                   "page table; GatedDeltaNet recurrence)"
                   + (f"; rotary positions, cache and attention by this library, {'e4m3' if cfg.kv_fp8 else 'bf16'} cache"
-                     if cfg.attention == "paged" else ""),
+                     if paged else ""),
         "config": {k: getattr(cfg, k) for k in ("layers", "hidden", "experts", "top_k", "inter", "shared_inter",
                                                  "batch", "context", "vocab", "page_size")},
         "steps": timed, "device_error": err, "data": "synthetic"}

@@ -126,3 +126,28 @@ def test_attention_layers_share_one_workspace():
     model = HybridDecoder(tiny_config(layers=8, attention="paged"))
     layers = [m for m in model.mixers if isinstance(m, _PagedAttention)]
     assert len(layers) == 2 and len({m.workspace.data_ptr() for m in layers}) == 1
+
+
+@pytest.mark.parametrize("attention", ["torch", "paged"])
+def test_library_share_counts_the_attention_calls(attention, monkeypatch):
+    """A step without the stand-ins still makes every call of this library that a whole step makes."""
+    from qs3_b200 import hybrid_decode as m
+    cfg = m.tiny_config(layers=8, new_tokens=12, attention=attention)
+    model, calls = m.HybridDecoder(cfg), {}
+    for name in ("kv_append", "paged_attention", "moe_layer_execute", "rmsnorm", "fused_add_rmsnorm_nvfp4"):
+        def counted(*a, _name=name, _real=getattr(m.ops, name), **kw):
+            calls[_name] = calls.get(_name, 0) + 1
+            return _real(*a, **kw)
+        monkeypatch.setattr(m.ops, name, counted)
+    made = []
+    with torch.cuda.stream(model.stream):
+        model.ctx.use_current_stream()
+        for mixers in (True, False):
+            calls.clear()
+            model.step(mixers)
+            made.append(dict(calls))
+        model.stream.synchronize()
+    assert made[0] == made[1] and made[0].get("paged_attention", 0) == (2 if attention == "paged" else 0)
+    record = m.measure(2, cfg)
+    assert ("attention" in record["library_calls"]) == (attention == "paged")
+    assert record["device_error"] == 0
