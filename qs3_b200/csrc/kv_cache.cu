@@ -9,6 +9,7 @@
 #include "fp8.cuh"
 #include "paged.cuh"
 
+#include <algorithm>
 #include <cmath>
 #include <limits>
 
@@ -591,6 +592,33 @@ template <typename Pool> bool pool_strides_ok(const Pool& t, int64_t unit)
         && t.stride[0] >= 0 && t.stride[1] >= 0 && t.stride[2] >= t.shape[3];
 }
 
+// Slots of a pool that is written, `width` elements each, share no memory. (Enough, and true of every order of the dimensions.)
+bool slots_apart(const int64_t* shape, const int64_t* stride, int64_t width)
+{
+    int order[3] = { 0, 1, 2 };
+    std::sort(order, order + 3, [&](int a, int b) { return stride[a] < stride[b]; });
+    for (const int i : order) {
+        if (shape[i] == 1)
+            continue;
+        if (stride[i] < width)
+            return false;
+        width += (shape[i] - 1) * stride[i];
+    }
+    return true;
+}
+
+qsfi_status check_written_cache(qsfi_context* ctx, const qs3_paged_kv_cache& c, bool fp8, const char* op)
+{
+    if (c.k.data == c.v.data || (fp8 && c.k_scale.data == c.v_scale.data))
+        return set_invalid_arg(ctx, "%s cache k and v must be apart", op);
+    bool apart = slots_apart(c.k.shape, c.k.stride, c.k.shape[3]) && slots_apart(c.v.shape, c.v.stride, c.v.shape[3]);
+    if (fp8)
+        apart = apart && slots_apart(c.k_scale.shape, c.k_scale.stride, 1) && slots_apart(c.v_scale.shape, c.v_scale.stride, 1);
+    if (!apart)
+        return set_invalid_arg(ctx, "%s slots of the cache must not overlap", op);
+    return QSFI_STATUS_OK;
+}
+
 } // namespace
 
 // A tensor of rows of one head: positive extents, contiguous and 16-byte aligned rows.
@@ -621,17 +649,18 @@ qsfi_status check_index(qsfi_context* ctx, const qsfi_tensor1& t, const char* op
     return QSFI_STATUS_OK;
 }
 
-// Written rows must not overlap one another.
-bool rows_apart(const qsfi_tensor3& t) // rows of shape[2] elements at two strides
+RowSet row_set(const qsfi_tensor3& t)
 {
-    const int64_t a0 = t.shape[0] > 1 ? t.stride[0] : 0, a1 = t.shape[1] > 1 ? t.stride[1] : 0;
-    if (t.shape[1] > 1 && a1 < t.shape[2])
-        return false;
-    if (t.shape[0] > 1 && a0 < t.shape[2])
-        return false;
-    if (t.shape[0] > 1 && t.shape[1] > 1)
-        return a0 >= (t.shape[1] - 1) * a1 + t.shape[2] || a1 >= (t.shape[0] - 1) * a0 + t.shape[2];
-    return true;
+    const int64_t size = t.dtype == QSFI_DTYPE_F32 ? 4 : 2;
+    return RowSet { t.data, t.shape[0], t.shape[1], t.stride[0] * size, t.stride[1] * size, t.shape[2] * size };
+}
+
+// What is written may not lie over another operand.
+qsfi_status check_apart(qsfi_context* ctx, const char* op, const char* written, const RowSet& a, const char* other, const RowSet& b)
+{
+    if (a.data != nullptr && b.data != nullptr && rows_meet(a, b))
+        return set_invalid_arg(ctx, "%s %s overlaps %s", op, written, other);
+    return QSFI_STATUS_OK;
 }
 
 // `out`, or where it is absent x itself, becomes `dst`. The two may be the same rows or apart, nothing between.
@@ -646,24 +675,12 @@ qsfi_status check_out(qsfi_context* ctx, const qsfi_tensor3& x, const qsfi_tenso
             if (out.shape[i] != x.shape[i])
                 return set_invalid_arg(ctx, "%s %s shape must match its input", op, name);
     }
-    if (!rows_apart(*dst))
+    const RowSet from = row_set(x), to = row_set(*dst);
+    if (!rows_apart(to))
         return set_invalid_arg(ctx, "%s %s rows must not overlap", op, name);
-    *in_place = dst->data == x.data && dst->stride[0] == x.stride[0] && dst->stride[1] == x.stride[1];
-    const int64_t size = x.dtype == QSFI_DTYPE_F32 ? 4 : 2;
-    const auto span = [&](const qsfi_tensor3& t) {
-        return ((t.shape[0] - 1) * t.stride[0] + (t.shape[1] - 1) * t.stride[1] + t.shape[2]) * size;
-    };
-    const uint8_t *a = static_cast<const uint8_t*>(x.data), *b = static_cast<const uint8_t*>(dst->data);
-    if (!*in_place && a < b + span(*dst) && b < a + span(x)) {
-        // views of one buffer (the heads of a fused projection) lie between each other without sharing an element when
-        // their token strides are the same and their rows fall into different parts of it
-        const int64_t pitch = x.stride[0] * size;
-        const int64_t wide_a = ((x.shape[1] - 1) * x.stride[1] + x.shape[2]) * size;
-        const int64_t wide_b = ((dst->shape[1] - 1) * dst->stride[1] + dst->shape[2]) * size;
-        const int64_t shift = pitch > 0 ? ((b - a) % pitch + pitch) % pitch : 0;
-        if (x.stride[0] != dst->stride[0] || shift < wide_a || shift + wide_b > pitch)
-            return set_invalid_arg(ctx, "%s %s overlaps its input without being the same rows", op, name);
-    }
+    *in_place = same_rows(from, to);
+    if (!*in_place && rows_meet(from, to))
+        return set_invalid_arg(ctx, "%s %s overlaps its input without being the same rows", op, name);
     return QSFI_STATUS_OK;
 }
 
@@ -783,7 +800,7 @@ qsfi_status qs3_rope(qsfi_context* ctx, const qs3_rope_desc* d)
     if (d->q.data != nullptr && d->q.dtype != QSFI_DTYPE_BF16 && d->q.dtype != QSFI_DTYPE_F32)
         return set_unsupported(ctx, "rope supports only bf16/f32 tensors");
     TurnParams p {};
-    qsfi_tensor3 dst;
+    qsfi_tensor3 dst, k_dst {};
     s = check_rows(ctx, d->q, "rope", "q", d->q.dtype);
     if (s == QSFI_STATUS_OK)
         s = check_dim(ctx, d->q.shape[2], "rope");
@@ -799,10 +816,10 @@ qsfi_status qs3_rope(qsfi_context* ctx, const qs3_rope_desc* d)
             return s;
         if (d->k.shape[0] != d->q.shape[0] || d->k.shape[2] != d->q.shape[2])
             return set_invalid_arg(ctx, "rope q and k must have the same tokens and head_dim");
-        s = check_out(ctx, d->k, d->k_out, "rope", "k_out", &dst, &p.in_place_k);
+        s = check_out(ctx, d->k, d->k_out, "rope", "k_out", &k_dst, &p.in_place_k);
         if (s != QSFI_STATUS_OK)
             return s;
-        fill_rows(&p.k, d->k, dst, size);
+        fill_rows(&p.k, d->k, k_dst, size);
     } else if (d->k_out.data != nullptr) {
         return set_invalid_arg(ctx, "rope k_out needs k");
     }
@@ -815,6 +832,15 @@ qsfi_status qs3_rope(qsfi_context* ctx, const qs3_rope_desc* d)
         return s;
     if (d->q.shape[1] + d->k.shape[1] > 65536)
         return set_unsupported(ctx, "rope takes at most 65536 heads");
+    if (d->k.data != nullptr) {
+        s = check_apart(ctx, "rope", "q_out", row_set(dst), "k", row_set(d->k));
+        if (s == QSFI_STATUS_OK)
+            s = check_apart(ctx, "rope", "k_out", row_set(k_dst), "q", row_set(d->q));
+        if (s == QSFI_STATUS_OK)
+            s = check_apart(ctx, "rope", "q_out", row_set(dst), "k_out", row_set(k_dst));
+        if (s != QSFI_STATUS_OK)
+            return s;
+    }
     p.tokens = static_cast<uint32_t>(d->q.shape[0]);
     p.dim = static_cast<uint32_t>(d->q.shape[2]);
     p.half = static_cast<uint32_t>(d->inv_freq.shape[0]);
@@ -879,8 +905,8 @@ qsfi_status qs3_kv_append(qsfi_context* ctx, const qs3_kv_append_desc* d)
     } else if (d->q.data != nullptr || d->positions.data != nullptr) {
         return set_invalid_arg(ctx, "kv_append q and positions need inv_freq");
     }
+    qsfi_tensor3 dst {};
     if (d->q.data != nullptr) {
-        qsfi_tensor3 dst;
         s = check_rows(ctx, d->q, "kv_append", "q", QSFI_DTYPE_BF16);
         if (s == QSFI_STATUS_OK)
             s = check_out(ctx, d->q, d->q_out, "kv_append", "q_out", &dst, &p.in_place_q);
@@ -896,6 +922,15 @@ qsfi_status qs3_kv_append(qsfi_context* ctx, const qs3_kv_append_desc* d)
     }
     if (p.view.kv_heads > 65536)
         return set_unsupported(ctx, "kv_append takes at most 65536 heads");
+    if (d->q.data != nullptr) {
+        s = check_apart(ctx, "kv_append", "q_out", row_set(dst), "k", row_set(d->k));
+        if (s == QSFI_STATUS_OK)
+            s = check_apart(ctx, "kv_append", "q_out", row_set(dst), "v", row_set(d->v));
+    }
+    if (s == QSFI_STATUS_OK)
+        s = check_written_cache(ctx, d->cache, fp8, "kv_append");
+    if (s != QSFI_STATUS_OK)
+        return s;
     p.view.err = device_error_word();
     if (p.view.err == nullptr)
         return set_cuda_error(ctx, cudaErrorUnknown, "device error word");
@@ -934,10 +969,13 @@ qsfi_status qs3_kv_gather(qsfi_context* ctx, const qs3_kv_gather_desc* d)
         return s;
     for (const qsfi_tensor3* t : { &d->k_out, &d->v_out })
         if (t->shape[0] != d->k_out.shape[0] || t->shape[1] != static_cast<int64_t>(p.view.kv_heads)
-            || t->shape[2] != static_cast<int64_t>(p.view.head_dim) || !rows_apart(*t))
+            || t->shape[2] != static_cast<int64_t>(p.view.head_dim) || !rows_apart(row_set(*t)))
             return set_invalid_arg(ctx, "kv_gather k_out and v_out must be [rows, kv_heads, head_dim] of the cache");
     if (p.view.kv_heads > 65536)
         return set_unsupported(ctx, "kv_gather takes at most 65536 heads");
+    s = check_apart(ctx, "kv_gather", "k_out", row_set(d->k_out), "v_out", row_set(d->v_out));
+    if (s != QSFI_STATUS_OK)
+        return s;
     p.view.err = device_error_word();
     if (p.view.err == nullptr)
         return set_cuda_error(ctx, cudaErrorUnknown, "device error word");

@@ -3,6 +3,7 @@
 
 #include "common.cuh"
 #include "paged_schedule.h"
+#include "row_sets.h"
 
 namespace qs3 {
 
@@ -114,11 +115,12 @@ __device__ __forceinline__ uint32_t warp_upper(const int32_t* table, uint32_t n,
 #endif
 
 // Host side: checks and views of the descriptors (kv_cache.cu).
-bool rows_apart(const qsfi_tensor3& t);
+RowSet row_set(const qsfi_tensor3& t);
 bool rows_fit(const PagedView& v);
 qsfi_status check_rows(qsfi_context* ctx, const qsfi_tensor3& t, const char* op, const char* name, qsfi_dtype dtype);
 qsfi_status check_out(qsfi_context* ctx, const qsfi_tensor3& x, const qsfi_tensor3& out, const char* op, const char* name,
                       qsfi_tensor3* dst, int* in_place);
+qsfi_status check_apart(qsfi_context* ctx, const char* op, const char* written, const RowSet& a, const char* other, const RowSet& b);
 qsfi_status check_index(qsfi_context* ctx, const qsfi_tensor1& t, const char* op, const char* name, int64_t length);
 qsfi_status paged_view(qsfi_context* ctx, const qs3_paged_kv_cache& cache, const qs3_page_table& table, const char* op,
                        PagedView* out, bool* fp8);

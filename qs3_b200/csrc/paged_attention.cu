@@ -766,6 +766,21 @@ qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_des
     if (static_cast<uint64_t>(d->workspace.shape[0]) < need)
         return set_invalid_arg(ctx, "paged_attention workspace has %lld bytes, needs %llu",
                                static_cast<long long>(d->workspace.shape[0]), static_cast<unsigned long long>(need));
+    const RowSet read = row_set(d->q), written = row_set(dst), scratch { d->workspace.data, 1, 1, 0, 0, static_cast<int64_t>(need) };
+    const RowSet lse { d->lse.data, rows, heads, p.lse_token * 4, p.lse_head * 4, 4 };
+    if (p.lse != nullptr && !rows_apart(lse))
+        return set_invalid_arg(ctx, "paged_attention lse rows must not overlap");
+    s = check_apart(ctx, "paged_attention", "workspace", scratch, "out", written);
+    if (s == QSFI_STATUS_OK)
+        s = check_apart(ctx, "paged_attention", "workspace", scratch, "q", read);
+    if (s == QSFI_STATUS_OK)
+        s = check_apart(ctx, "paged_attention", "workspace", scratch, "lse", lse);
+    if (s == QSFI_STATUS_OK)
+        s = check_apart(ctx, "paged_attention", "lse", lse, "q", read);
+    if (s == QSFI_STATUS_OK)
+        s = check_apart(ctx, "paged_attention", "lse", lse, "out", written);
+    if (s != QSFI_STATUS_OK)
+        return s;
 
     p.q = static_cast<const uint8_t*>(d->q.data);
     p.q_token = d->q.stride[0] * 2;

@@ -333,3 +333,32 @@ def test_tokens_beyond_the_pages_have_no_place(ops, ctx, q_len, fp8):
         row += n
     for a, b in zip(before, raw(cache)):
         assert torch.equal(a[~touched], b[~touched])
+
+
+@pytest.mark.parametrize("tokens", [1, 7, 300])
+def test_parts_between_each_other(ops, ctx, tokens):
+    """Outputs that lie between other operands without sharing memory, and one token's rows in place under another token stride."""
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    wide = torch.randn((tokens, 2, 6, 64), generator=gen, device="cuda").to(torch.bfloat16)
+    before, f = wide.clone(), ops.rope_frequencies(64)
+    positions = torch.arange(tokens, device="cuda")
+    # q, q_out, k and k_out: heads of one buffer in turn
+    q, q_out, k, k_out = wide[:, 0, 0::2], wide[:, 0, 1::2], wide[:, 1, 0::2], wide[:, 1, 1::2]
+    ops.rope(ctx, positions, f.inv_freq, q, k, q_out=q_out, k_out=k_out)
+    torch.cuda.synchronize()
+    assert torch.equal(wide[:, :, 0::2], before[:, :, 0::2])
+    for x, got in ((before[:, 0, 0::2], q_out), (before[:, 1, 0::2], k_out)):
+        want = turn(x, positions, f.inv_freq, 1.0, False)
+        assert bool(((got.double() - want).abs() <= turn_bound(x, want, 64, 1.0, 2.0 ** -8)).all())
+    # K and V of a token side by side in every head
+    c = make_case(ops, [0], [tokens], heads=2, kv_heads=2, dim=64, seed=tokens, tail=1)
+    both = torch.zeros((tokens, 2, 2, 64), dtype=torch.bfloat16, device="cuda")
+    ops.kv_gather(ctx, c.cache, c.table, ints([0, tokens]), both[:, :, 0], both[:, :, 1])
+    torch.cuda.synchronize()
+    assert torch.equal(both[:, :, 0].double(), c.keys[0]) and torch.equal(both[:, :, 1].double(), c.values[0])
+    if tokens == 1:
+        x = before[:, 0, :2].clone()
+        want = turn(x, positions + 5, f.inv_freq, 1.0, False)
+        ops.rope(ctx, positions + 5, f.inv_freq, x, q_out=x.as_strided(x.shape, (1024, 64, 1)))
+        torch.cuda.synchronize()
+        assert bool(((x.double() - want).abs() <= turn_bound(before[:, 0, :2], want, 64, 1.0, 2.0 ** -8)).all())

@@ -382,3 +382,89 @@ def test_codes_of_another_kind_are_refused(name, dtype):
     with pytest.raises(ops.Qs3Error, match="e4m3 codes") as e:
         paged_call(name, getattr(torch, dtype))
     assert e.value.status == INVALID
+
+
+ROWS_PROGRAM = r"""
+#include "row_sets.h"
+#include <cstdio>
+#include <random>
+#include <vector>
+using namespace qs3;
+int main()
+{
+    static uint8_t memory[1];
+    std::mt19937 rng(1);
+    const auto pick = [&](int n) { return static_cast<int64_t>(rng() % n); };
+    long met = 0, exact = 0, wrong = 0;
+    for (int n = 0; n < 400000; ++n) {
+        RowSet s[2];
+        for (RowSet& x : s) {
+            x = RowSet { memory + pick(80), 1 + pick(5), 1 + pick(5), pick(24), pick(24), 1 + pick(4) };
+            if (&x == s + 1 && pick(3) != 0)
+                x.s0 = s[0].s0, x.s1 = pick(2) ? s[0].s1 : x.s1;
+        }
+        std::vector<int> used(800);
+        bool apart = true, meet = false;
+        for (int64_t i = 0; i < s[0].n0; ++i)
+            for (int64_t j = 0; j < s[0].n1; ++j)
+                for (int64_t k = 0; k < s[0].width; ++k)
+                    apart = used[(const uint8_t*)s[0].data - memory + i * s[0].s0 + j * s[0].s1 + k]++ == 0 && apart;
+        for (int64_t i = 0; i < s[1].n0; ++i)
+            for (int64_t j = 0; j < s[1].n1; ++j)
+                for (int64_t k = 0; k < s[1].width; ++k)
+                    meet = used[(const uint8_t*)s[1].data - memory + i * s[1].s0 + j * s[1].s1 + k] != 0 || meet;
+        if (rows_apart(s[0]) && !apart) { std::printf("rows share memory\n"); return 1; }
+        const bool same = (s[0].n0 == 1 || s[1].n0 == 1 || s[0].s0 == s[1].s0) && (s[0].n1 == 1 || s[1].n1 == 1 || s[0].s1 == s[1].s1);
+        const bool said = rows_meet(s[0], s[1]);
+        if (said != rows_meet(s[1], s[0])) { std::printf("not symmetric\n"); return 1; }
+        if (meet && !said) { std::printf("an overlap was missed\n"); return 1; }
+        if (same && said && !meet) { std::printf("rows that are apart were taken to meet\n"); return 1; }
+        met += meet, exact += same, wrong += said != meet;
+    }
+    std::printf("%ld %ld %ld\n", met, exact, wrong);
+    return met > 10000 && exact > 10000 ? 0 : 1;
+}
+"""
+
+
+def test_rows_that_share_memory(tmp_path):
+    """Against every byte of small sets."""
+    src, exe = tmp_path / "rows.cpp", tmp_path / "rows"
+    src.write_text(ROWS_PROGRAM)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-Werror", f"-I{CSRC}", str(src), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout
+
+
+ROPE_Q = dict(q=t(BF16, 4, 2, 64, ptr=0x100000))
+KV_PARTS = dict(k=t(BF16, 3, 2, 64, ptr=0x200000), v=t(BF16, 3, 2, 64, ptr=0x300000), inv_freq=t(F64, 8))
+
+
+@pytest.mark.parametrize("fn,make,kw,fragment", [
+    ("qs3_rope", "rope_desc", dict(ROPE_Q, k=t(BF16, 4, 2, 64, ptr=0x100000)), "q_out overlaps k"),
+    ("qs3_rope", "rope_desc", dict(ROPE_Q, k=t(BF16, 4, 2, 64, ptr=0x100080)), "q_out overlaps k"),
+    ("qs3_rope", "rope_desc", dict(ROPE_Q, q_out=t(BF16, 4, 2, 64, ptr=0x200000), k=t(BF16, 4, 1, 64, ptr=0x200200)), "q_out overlaps k"),
+    ("qs3_rope", "rope_desc", dict(ROPE_Q, k=t(BF16, 4, 2, 64, ptr=0x300000), k_out=t(BF16, 4, 2, 64, ptr=0x100000)), "k_out overlaps q"),
+    ("qs3_rope", "rope_desc", dict(ROPE_Q, q_out=t(BF16, 4, 2, 64, ptr=0x200000), k=t(BF16, 4, 2, 64, ptr=0x300000),
+                                   k_out=t(BF16, 4, 2, 64, ptr=0x200000)), "q_out overlaps k_out"),
+    ("qs3_kv_append", "append_desc", dict(KV_PARTS, q=t(BF16, 3, 2, 64, ptr=0x400000), q_out=t(BF16, 3, 2, 64, ptr=0x200000)), "q_out overlaps k"),
+    ("qs3_kv_append", "append_desc", dict(KV_PARTS, q=t(BF16, 3, 2, 64, ptr=0x300080)), "q_out overlaps v"),
+    ("qs3_kv_append", "append_desc", dict(k=t(BF16, 3, 2, 64, ptr=0x200000)), "cache k and v"),
+    ("qs3_kv_append", "append_desc", dict(cache=cache(v=t(BF16, 10, 2, 16, 64, ptr=0x400000, stride=(1024, 0, 64, 1)))), "slots of the cache"),
+    ("qs3_kv_append", "append_desc", dict(cache=cache(k=t(BF16, 10, 2, 16, 64, ptr=0x400000, stride=(1024, 1024, 64, 1)))), "slots of the cache"),
+    ("qs3_kv_append", "append_desc", dict(cache=cache(fp8=True, k=t(E4M3, 10, 2, 16, 64, ptr=0x400000))), "cache k and v"),
+    ("qs3_kv_append", "append_desc", dict(cache=cache(fp8=True, k=t(E4M3, 10, 2, 16, 64, ptr=0x400000),
+                                                      k_scale=t(F32, 10, 2, 16, ptr=0x500000, stride=(0, 0, 0)))), "slots of the cache"),
+    ("qs3_kv_gather", "gather_desc", dict(), "k_out overlaps v_out"),
+    ("qs3_kv_gather", "gather_desc", dict(v_out=t(BF16, 9, 2, 64, ptr=0x10100)), "k_out overlaps v_out"),
+    ("qs3_paged_attention", "attention_desc", dict(), "workspace overlaps out"),
+    ("qs3_paged_attention", "attention_desc", dict(out=t(BF16, 3, 4, 64, ptr=0x80000000)), "workspace overlaps q"),
+    ("qs3_paged_attention", "attention_desc", dict(workspace=t(U8, 1 << 30, ptr=0x1000000), lse=t(F32, 3, 4)), "lse overlaps q"),
+    ("qs3_paged_attention", "attention_desc", dict(workspace=t(U8, 1 << 30, ptr=0x1000000), lse=t(F32, 3, 4, ptr=0x200020),
+                                                   out=t(BF16, 3, 4, 64, ptr=0x200000)), "lse overlaps out"),
+    ("qs3_paged_attention", "attention_desc", dict(workspace=t(U8, 1 << 30, ptr=0x1000000), lse=t(F32, 3, 4, ptr=0x1000020)), "workspace overlaps lse"),
+    ("qs3_paged_attention", "attention_desc", dict(workspace=t(U8, 1 << 30, ptr=0x1000000), lse=t(F32, 3, 4, ptr=0x200000, stride=(0, 1))),
+     "lse rows must not overlap"),
+])
+def test_outputs_over_other_operands_are_refused(lib, ctx, fn, make, kw, fragment):
+    refused(lib, ctx, fn, globals()[make](**kw), INVALID, fragment)
