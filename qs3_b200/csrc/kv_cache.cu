@@ -499,6 +499,14 @@ template <bool FP8> __global__ void __launch_bounds__(kRowThreads, 6) kv_gather_
 
 bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
 
+// Elements of tables are read one by one, by their own size.
+qsfi_status check_aligned(qsfi_context* ctx, const void* ptr, uint32_t size, const char* op, const char* name)
+{
+    if (reinterpret_cast<uintptr_t>(ptr) % size != 0)
+        return set_invalid_arg(ctx, "%s %s must be aligned to its elements of %u bytes", op, name, size);
+    return QSFI_STATUS_OK;
+}
+
 qsfi_status check_dim(qsfi_context* ctx, int64_t dim, const char* op)
 {
     if (dim % 8 != 0 || dim > static_cast<int64_t>(kMaxHeadDim))
@@ -514,14 +522,14 @@ qsfi_status check_rotary(qsfi_context* ctx, const qsfi_tensor1& inv_freq, float 
         return set_invalid_arg(ctx, "%s inv_freq must have between 1 and head_dim / 2 entries", op);
     if (!std::isfinite(scale))
         return set_invalid_arg(ctx, "%s scale must be finite", op);
-    return QSFI_STATUS_OK;
+    return check_aligned(ctx, inv_freq.data, 8, op, "inv_freq");
 }
 
 qsfi_status check_positions(qsfi_context* ctx, const qsfi_tensor1& t, int64_t rows, const char* op)
 {
     if ((t.dtype != QSFI_DTYPE_I32 && t.dtype != QS3_DTYPE_I64) || t.stride[0] != 1 || t.shape[0] < rows)
         return set_invalid_arg(ctx, "%s positions must be contiguous i32 or i64, one per row", op);
-    return QSFI_STATUS_OK;
+    return check_aligned(ctx, t.data, t.dtype == QS3_DTYPE_I64 ? 8 : 4, op, "positions");
 }
 
 void fill_rows(Rows* r, const qsfi_tensor3& src, const qsfi_tensor3& dst, int64_t size)
@@ -646,7 +654,7 @@ qsfi_status check_index(qsfi_context* ctx, const qsfi_tensor1& t, const char* op
     if (t.stride[0] != 1 || t.shape[0] < length || t.shape[0] > std::numeric_limits<int32_t>::max())
         return set_invalid_arg(ctx, "%s %s must be contiguous and hold at least %lld entries", op, name,
                                static_cast<long long>(length));
-    return QSFI_STATUS_OK;
+    return check_aligned(ctx, t.data, 4, op, name);
 }
 
 RowSet row_set(const qsfi_tensor3& t)

@@ -468,3 +468,21 @@ KV_PARTS = dict(k=t(BF16, 3, 2, 64, ptr=0x200000), v=t(BF16, 3, 2, 64, ptr=0x300
 ])
 def test_outputs_over_other_operands_are_refused(lib, ctx, fn, make, kw, fragment):
     refused(lib, ctx, fn, globals()[make](**kw), INVALID, fragment)
+
+
+@pytest.mark.parametrize("fn,make,kw,name", [
+    ("qs3_rope", "rope_desc", dict(positions=t(I32, 4, ptr=0x10002)), "positions"),
+    ("qs3_rope", "rope_desc", dict(positions=t(I64, 4, ptr=0x10004)), "positions"),
+    ("qs3_rope", "rope_desc", dict(inv_freq=t(F64, 16, ptr=0x10004)), "inv_freq"),
+    ("qs3_kv_append", "append_desc", dict(inv_freq=t(F64, 16, ptr=0x10004)), "inv_freq"),
+    ("qs3_kv_append", "append_desc", dict(inv_freq=t(F64, 16), positions=t(I64, 3, ptr=0x10004)), "positions"),
+    ("qs3_kv_append", "append_desc", dict(q_indptr=t(I32, 4, ptr=0x10001)), "q_indptr"),
+    ("qs3_kv_append", "append_desc", dict(table=table(kv_len=t(I32, 3, ptr=0x10002))), "kv_len"),
+    ("qs3_kv_gather", "gather_desc", dict(table=table(kv_indptr=t(I32, 4, ptr=0x10002))), "kv_indptr"),
+    ("qs3_kv_gather", "gather_desc", dict(out_indptr=t(I32, 4, ptr=0x10002)), "out_indptr"),
+    ("qs3_kv_gather", "gather_desc", dict(kv_start=t(I32, 3, ptr=0x10002)), "kv_start"),
+    ("qs3_paged_attention", "attention_desc", dict(table=table(kv_indices=t(I32, 8, ptr=0x10002))), "kv_indices"),
+    ("qs3_paged_attention", "attention_desc", dict(q_indptr=t(I32, 4, ptr=0x10002)), "q_indptr"),
+])
+def test_misaligned_tables_are_refused(lib, ctx, fn, make, kw, name):
+    refused(lib, ctx, fn, globals()[make](**kw), INVALID, f"{name} must be aligned")
