@@ -51,10 +51,13 @@ template <typename Tensor, uint32_t RANK> void put(char* at_, const at::Tensor& 
 
 PyObject* fill_checked(PyObject* const* args, Py_ssize_t nargs)
 {
-    if (nargs != 3 || !PyBytes_Check(args[1]) || !PyTuple_Check(args[2])) {
-        PyErr_SetString(PyExc_TypeError, "fill(address, layout bytes, tensor tuple)");
+    if (nargs < 3 || nargs > 4 || !PyBytes_Check(args[1]) || !PyTuple_Check(args[2])) {
+        PyErr_SetString(PyExc_TypeError, "fill(address, layout bytes, tensor tuple[, device])");
         return nullptr;
     }
+    const long device = nargs == 4 ? PyLong_AsLong(args[3]) : -1; // negative: any
+    if (device == -1 && PyErr_Occurred())
+        return nullptr;
     char* base = static_cast<char*>(PyLong_AsVoidPtr(args[0]));
     if (base == nullptr) {
         if (!PyErr_Occurred())
@@ -76,6 +79,9 @@ PyObject* fill_checked(PyObject* const* args, Py_ssize_t nargs)
             return nullptr;
         }
         const at::Tensor& t = THPVariable_Unpack(o);
+        // (pinned host memory has the same address on the device)
+        if (device >= 0 && (t.is_cuda() ? t.get_device() != device : !(t.is_cpu() && t.is_pinned())))
+            return PyLong_FromSsize_t(-2 - i);
         char* at_ = base + layout[3 * i];
         const int32_t rank = layout[3 * i + 1];
         const int32_t dtype = layout[3 * i + 2] >= 0 ? layout[3 * i + 2] : dtype_code(t.scalar_type());
@@ -114,7 +120,8 @@ PyObject* fill(PyObject*, PyObject* const* args, Py_ssize_t nargs)
 
 PyMethodDef methods[] = {
     { "fill", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fill)), METH_FASTCALL,
-      "fill(address, layout, tensors) -> -1 or the index of a tensor of the wrong rank" },
+      "fill(address, layout, tensors[, device]) -> -1, the index of a tensor of the wrong rank, or -2 - that of one the device "
+      "cannot address" },
     { nullptr, nullptr, 0, nullptr },
 };
 

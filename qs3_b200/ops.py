@@ -62,6 +62,17 @@ def _fill(d, layout, *tensors):
                        f"expected a rank-{layout[1][bad]} tensor, got {tensors[bad].dim()}")
 
 
+def _fill_on(ctx, d, layout, *tensors):
+    """The same for tensors that have to be on the context's device (a context without one takes any)."""
+    bad = _marshal.fill(C.addressof(d), layout[0], tensors, ctx.device)
+    if bad >= 0:
+        raise Qs3Error(capi.STATUS_INVALID_ARGUMENT,
+                       f"expected a rank-{layout[1][bad]} tensor, got {tensors[bad].dim()}")
+    if bad < -1:
+        raise Qs3Error(capi.STATUS_INVALID_ARGUMENT,
+                       f"expected a tensor on cuda:{ctx.device}, the context's device, got {tensors[-2 - bad].device}")
+
+
 def _desc(t, rank, dtype=None):
     """qsfi_tensorN view of a torch tensor (None -> absent optional tensor)."""
     d = (capi.Tensor1, capi.Tensor2, capi.Tensor3)[rank - 1]()
@@ -721,7 +732,7 @@ def rope(ctx: Context, positions, inv_freq, q, k=None, *, q_out=None, k_out=None
     ``q_out`` / ``k_out`` in place. Pairs are ``(j, j + r/2)``, or ``(2 j, 2 j + 1)`` with ``interleaved``, of the first
     ``r = 2 * len(inv_freq)`` elements; the others are passed through."""
     d = capi.RopeDesc()
-    _fill(d, _ROPE_DESC, q, k, q_out, k_out, positions, inv_freq)
+    _fill_on(ctx, d, _ROPE_DESC, q, k, q_out, k_out, positions, inv_freq)
     d.scale, d.interleaved = scale, 1 if interleaved else 0
     ctx.check(ctx._lib.qs3_rope(ctx.handle, C.byref(d)))
 
@@ -762,12 +773,12 @@ class PageTable:
 _CODES = (torch.float8_e4m3fn, torch.uint8)
 
 
-def _fill_paged(d, layouts, cache: PagedKvCache, table: PageTable, *tensors):
+def _fill_paged(ctx, d, layouts, cache: PagedKvCache, table: PageTable, *tensors):
     if cache.fp8 and not (cache.k.dtype in _CODES and cache.v.dtype in _CODES):
         raise Qs3Error(capi.STATUS_INVALID_ARGUMENT,
                        f"a cache with scales holds e4m3 codes (float8_e4m3fn or u8), not {cache.k.dtype} and {cache.v.dtype}")
-    _fill(d, layouts[1 if cache.fp8 else 0], cache.k, cache.v, cache.k_scale, cache.v_scale, table.kv_indptr,
-          table.kv_indices, table.kv_len, *tensors)
+    _fill_on(ctx, d, layouts[1 if cache.fp8 else 0], cache.k, cache.v, cache.k_scale, cache.v_scale, table.kv_indptr,
+             table.kv_indices, table.kv_len, *tensors)
 
 
 def kv_append(ctx: Context, cache: PagedKvCache, table: PageTable, k, v, *, q_indptr=None, q=None, q_out=None,
@@ -777,7 +788,7 @@ def kv_append(ctx: Context, cache: PagedKvCache, table: PageTable, k, v, *, q_in
     k is rotated on the way, and q as well (in place without ``q_out``), by the tokens' places in the cache or by
     ``positions``."""
     d = capi.KvAppendDesc()
-    _fill_paged(d, _KV_APPEND_DESC, cache, table, q_indptr, k, v, q, q_out, positions, inv_freq)
+    _fill_paged(ctx, d, _KV_APPEND_DESC, cache, table, q_indptr, k, v, q, q_out, positions, inv_freq)
     d.rope_scale, d.interleaved = rope_scale, 1 if interleaved else 0
     ctx.check(ctx._lib.qs3_kv_append(ctx.handle, C.byref(d)))
 
@@ -786,7 +797,7 @@ def kv_gather(ctx: Context, cache: PagedKvCache, table: PageTable, out_indptr, k
     """``qs3_kv_gather``: rows ``out_indptr[b] .. out_indptr[b + 1]`` of k_out and v_out (bf16 [rows, kv_heads, head_dim])
     become the tokens of sequence b from ``kv_start[b]`` (default 0) on; rows without one are left as they are."""
     d = capi.KvGatherDesc()
-    _fill_paged(d, _KV_GATHER_DESC, cache, table, kv_start, out_indptr, k_out, v_out)
+    _fill_paged(ctx, d, _KV_GATHER_DESC, cache, table, kv_start, out_indptr, k_out, v_out)
     ctx.check(ctx._lib.qs3_kv_gather(ctx.handle, C.byref(d)))
 
 
@@ -806,7 +817,7 @@ def paged_attention(ctx: Context, q, cache: PagedKvCache, table: PageTable, out,
     ``q_indptr`` row b is). ``lse`` (f32 [rows, heads]) takes the log-sum-exp of each row. ``max_q_len`` and
     ``max_kv_len``, where the host knows them, choose the kernels; results do not depend on them."""
     d = capi.PagedAttentionDesc()
-    _fill_paged(d, _PAGED_ATTENTION_DESC, cache, table, q, q_indptr, out, lse, workspace)
+    _fill_paged(ctx, d, _PAGED_ATTENTION_DESC, cache, table, q, q_indptr, out, lse, workspace)
     d.sm_scale = 0.0 if sm_scale is None else sm_scale
     d.causal, d.window, d.max_q_len, d.max_kv_len = 1 if causal else 0, window, max_q_len, max_kv_len
     ctx.check(ctx._lib.qs3_paged_attention(ctx.handle, C.byref(d)))

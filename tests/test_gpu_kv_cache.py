@@ -362,3 +362,16 @@ def test_parts_between_each_other(ops, ctx, tokens):
         ops.rope(ctx, positions + 5, f.inv_freq, x, q_out=x.as_strided(x.shape, (1024, 64, 1)))
         torch.cuda.synchronize()
         assert bool(((x.double() - want).abs() <= turn_bound(before[:, 0, :2], want, 64, 1.0, 2.0 ** -8)).all())
+
+
+def test_positions_in_pinned_memory(ops, ctx):
+    """Host memory that the device addresses stands for device memory; other host memory is refused."""
+    q = torch.randn((5, 2, 64), device="cuda").to(torch.bfloat16)
+    f, positions = ops.rope_frequencies(64), torch.arange(5)
+    got, want = torch.empty_like(q), torch.empty_like(q)
+    ops.rope(ctx, positions.pin_memory(), f.inv_freq, q, q_out=got)
+    ops.rope(ctx, positions.cuda(), f.inv_freq, q, q_out=want)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    with pytest.raises(ops.Qs3Error, match="on cuda:0"):
+        ops.rope(ctx, positions, f.inv_freq, q, q_out=got)

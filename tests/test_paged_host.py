@@ -486,3 +486,25 @@ def test_outputs_over_other_operands_are_refused(lib, ctx, fn, make, kw, fragmen
 ])
 def test_misaligned_tables_are_refused(lib, ctx, fn, make, kw, name):
     refused(lib, ctx, fn, globals()[make](**kw), INVALID, f"{name} must be aligned")
+
+
+@pytest.mark.parametrize("name", ["rope", "kv_append", "kv_gather", "paged_attention"])
+def test_tensors_off_the_device_are_refused(name, monkeypatch):
+    """CPU tensors in a call by a context of a device (no call is made)."""
+    import torch
+
+    from qs3_b200 import ops
+    real = ops.Context
+
+    class OfDevice(real):
+        def __init__(self, device):
+            super().__init__(device=-1)
+            self.device = 0
+    monkeypatch.setattr(ops, "Context", OfDevice)
+    with pytest.raises(ops.Qs3Error, match="on cuda:0") as e:
+        if name == "rope":
+            ops.rope(OfDevice(0), torch.zeros(4, dtype=torch.int32), ops.rope_frequencies(16, device="cpu").inv_freq,
+                     torch.zeros((4, 2, 64), dtype=torch.bfloat16))
+        else:
+            paged_call(name, torch.bfloat16, scales=False)
+    assert e.value.status == INVALID
