@@ -726,6 +726,13 @@ def rope_frequencies(rotary_dim: int, theta: float = 10000.0, *, scaling: str = 
     return RotaryFrequencies(freq.to(device), factor_on_both if scale is None else scale)
 
 
+def _nonzero_scale(name, scale):
+    """0 stands for the default in the descriptors."""
+    if scale == 0:
+        raise Qs3Error(capi.STATUS_INVALID_ARGUMENT, f"{name} must not be 0")
+    return scale
+
+
 def rope(ctx: Context, positions, inv_freq, q, k=None, *, q_out=None, k_out=None, scale: float = 1.0,
          interleaved: bool = False):
     """``qs3_rope``: rotary positions (i32 or i64 [tokens]) on q and k (bf16 or f32 [tokens, heads, head_dim]); without
@@ -733,7 +740,7 @@ def rope(ctx: Context, positions, inv_freq, q, k=None, *, q_out=None, k_out=None
     ``r = 2 * len(inv_freq)`` elements; the others are passed through."""
     d = capi.RopeDesc()
     _fill_on(ctx, d, _ROPE_DESC, q, k, q_out, k_out, positions, inv_freq)
-    d.scale, d.interleaved = scale, 1 if interleaved else 0
+    d.scale, d.interleaved = _nonzero_scale("scale", scale), 1 if interleaved else 0
     ctx.check(ctx._lib.qs3_rope(ctx.handle, C.byref(d)))
 
 
@@ -789,7 +796,7 @@ def kv_append(ctx: Context, cache: PagedKvCache, table: PageTable, k, v, *, q_in
     ``positions``."""
     d = capi.KvAppendDesc()
     _fill_paged(ctx, d, _KV_APPEND_DESC, cache, table, q_indptr, k, v, q, q_out, positions, inv_freq)
-    d.rope_scale, d.interleaved = rope_scale, 1 if interleaved else 0
+    d.rope_scale, d.interleaved = _nonzero_scale("rope_scale", rope_scale), 1 if interleaved else 0
     ctx.check(ctx._lib.qs3_kv_append(ctx.handle, C.byref(d)))
 
 
@@ -818,6 +825,6 @@ def paged_attention(ctx: Context, q, cache: PagedKvCache, table: PageTable, out,
     ``max_kv_len``, where the host knows them, choose the kernels; results do not depend on them."""
     d = capi.PagedAttentionDesc()
     _fill_paged(ctx, d, _PAGED_ATTENTION_DESC, cache, table, q, q_indptr, out, lse, workspace)
-    d.sm_scale = 0.0 if sm_scale is None else sm_scale
+    d.sm_scale = 0.0 if sm_scale is None else _nonzero_scale("sm_scale", sm_scale)
     d.causal, d.window, d.max_q_len, d.max_kv_len = 1 if causal else 0, window, max_q_len, max_kv_len
     ctx.check(ctx._lib.qs3_paged_attention(ctx.handle, C.byref(d)))
