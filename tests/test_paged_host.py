@@ -510,8 +510,9 @@ def test_tensors_off_the_device_are_refused(name, monkeypatch):
     assert e.value.status == INVALID
 
 
+@pytest.mark.parametrize("zero", [0.0, -0.0, 1e-60])
 @pytest.mark.parametrize("name", ["rope", "kv_append", "paged_attention"])
-def test_a_scale_of_zero_is_not_the_default(name):
+def test_a_scale_of_zero_is_not_the_default(name, zero):
     """0 stands for the default in the C interface, which takes no other zero; the Python one has None and 1."""
     import torch
 
@@ -522,9 +523,9 @@ def test_a_scale_of_zero_is_not_the_default(name):
     c, p = ops.PagedKvCache(new(4, 2, 16, 64), new(4, 2, 16, 64)), ops.PageTable(i32(4), i32(8), i32(3))
     with pytest.raises(ops.Qs3Error, match="scale must not be 0") as e:
         if name == "rope":
-            ops.rope(ctx, i32(4), freq, new(4, 2, 64), scale=0.0)
+            ops.rope(ctx, i32(4), freq, new(4, 2, 64), scale=zero)
         elif name == "kv_append":
-            ops.kv_append(ctx, c, p, new(3, 2, 64), new(3, 2, 64), inv_freq=freq, rope_scale=0.0)
+            ops.kv_append(ctx, c, p, new(3, 2, 64), new(3, 2, 64), inv_freq=freq, rope_scale=zero)
         else:
-            ops.paged_attention(ctx, new(3, 4, 64), c, p, new(3, 4, 64), new(1 << 26, dtype=torch.uint8), sm_scale=0.0)
+            ops.paged_attention(ctx, new(3, 4, 64), c, p, new(3, 4, 64), new(1 << 26, dtype=torch.uint8), sm_scale=zero)
     assert e.value.status == INVALID
