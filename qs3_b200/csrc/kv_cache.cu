@@ -587,9 +587,11 @@ template <typename T, int TARGET, int PARTS> cudaError_t launch_turn_parts(TurnP
 
 template <typename T, int TARGET> cudaError_t launch_turn(TurnParams* p, bool interleaved, cudaStream_t stream)
 {
-    const bool own = p->half == 0 || interleaved || 2 * p->half == p->dim;
-    if (sizeof(T) == 2 && p->dim % 16 == 0 && own)
-        return launch_turn_parts<T, TARGET, 2>(p, interleaved, stream);
+    if constexpr (sizeof(T) == 2) {
+        const bool own = p->half == 0 || interleaved || 2 * p->half == p->dim;
+        if (p->dim % 16 == 0 && own)
+            return launch_turn_parts<T, TARGET, 2>(p, interleaved, stream);
+    }
     return launch_turn_parts<T, TARGET, 1>(p, interleaved, stream);
 }
 
