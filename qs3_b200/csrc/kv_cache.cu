@@ -427,9 +427,7 @@ __device__ __forceinline__ void put_cached(uint8_t* dst, const uint4& w, float s
         uint32_t out[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const uint32_t two = in[j / 2] >> (16 * (j & 1));
-            uint32_t h;
-            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two)));
+            const uint32_t h = e4m3x2_to_f16x2(in[j / 2] >> (16 * (j & 1)));
             const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
             const __nv_bfloat162 r = __floats2bfloat162_rn(v.x * scale, v.y * scale);
             out[j] = *reinterpret_cast<const uint32_t*>(&r);

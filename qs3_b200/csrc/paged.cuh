@@ -37,6 +37,34 @@ struct PagedView {
 
 #ifdef __CUDACC__
 
+// 16 bytes to shared memory, zeros where `there` is false.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
+}
+
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+
+// Two codes in the low half of x.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t x)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(x)));
+    return r;
+}
+
 // Tokens of a sequence, and where its page ids begin. Positions, masks and angles go by `length`, as the table says it; what may be
 // read or written by `room`, the tokens that its pages hold of them: whatever the tables hold, the ids of positions below it lie
 // inside `indices`.

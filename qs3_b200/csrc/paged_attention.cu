@@ -65,11 +65,6 @@ template <bool F16> __device__ __forceinline__ void mma16816(float* c, const uin
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// 16 bytes to shared memory, zeros where `there` is 0.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t there)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
-}
 __device__ __forceinline__ void cp_async4z(uint32_t dst, const void* src, uint32_t there)
 {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4u : 0u) : "memory");
@@ -78,27 +73,6 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N> __device__ __forceinline__ void cp_async_wait_group()
 {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ float exp2_fast(float x)
-{
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
-// Two codes in the low half of x.
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t x)
-{
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(x)));
-    return r;
-}
-__device__ __forceinline__ uint32_t pack_f16x2(float a, float b)
-{
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    return r;
 }
 
 // e4m3: where the largest weight lies, in powers of two (f16 ends at 2^16 and loses bits below 2^-14), and a factor on 1 / scale

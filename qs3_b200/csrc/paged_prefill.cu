@@ -111,11 +111,6 @@ template <uint32_t D, bool FP8> struct PrefillShape {
     static_assert(kThreads <= 512, "128 registers for each");
 };
 
-__device__ __forceinline__ void cp_async16z(uint32_t dst, const void* src, bool there)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
-}
-
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -160,20 +155,6 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r)
 }
 
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ uint32_t pack_f16x2(float a, float b)
-{
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    return r;
-}
-// Two codes in the low half of x.
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t x)
-{
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(x)));
-    return r;
-}
 
 // Two codes in the low half, that of a in the low byte.
 __device__ __forceinline__ uint32_t pack_e4m3x2(float a, float b)
@@ -231,13 +212,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
 {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
-__device__ __forceinline__ float exp2_approx(float x)
-{
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
@@ -389,7 +363,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                         const uint32_t dst = tile_at + in_tile * 128 + (((lane & 7) ^ (r & 7)) * 16);
 #pragma unroll
                         for (uint32_t panel = 0; panel < D / 64; ++panel)
-                            cp_async16z(smem_u32(smem) + dst + panel * (kRowTile * 128), src + panel * 128, there);
+                            cp_async16(smem_u32(smem) + dst + panel * (kRowTile * 128), src + panel * 128, there);
                     } else {
                         uint4 v[D / 64];
                         uint32_t most = 0; // of the magnitudes, which are in the order of their bits
@@ -501,7 +475,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
 #pragma unroll
                     for (uint32_t j = 0; j < LOADS; ++j) {
                         const uint32_t r = __shfl_sync(0xffffffffu, row[j * AT_ONCE / 32], (j * AT_ONCE + lane / UNITS) & 31);
-                        cp_async16z(stage_at + (j * 32 + lane) * 16, from + row_bytes(p.view.v, r), r != kNoRow);
+                        cp_async16(stage_at + (j * 32 + lane) * 16, from + row_bytes(p.view.v, r), r != kNoRow);
                     }
                 };
                 Places ahead;
@@ -692,7 +666,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 for (uint32_t j = 0; j < KEYS / AT_ONCE; ++j) {
                     const uint32_t key = j * AT_ONCE + lane / UNITS;
                     const uint32_t r = __shfl_sync(0xffffffffu, row[j * AT_ONCE / 32], key & 31);
-                    cp_async16z(to + key * WIDTH + ((lane % (WIDTH / 16) ^ swizzle_of<WIDTH>(key)) * 16),
+                    cp_async16(to + key * WIDTH + ((lane % (WIDTH / 16) ^ swizzle_of<WIDTH>(key)) * 16),
                                 from + row_bytes(pool, r), r != kNoRow);
                 }
                 copies.push(&full_bar[s]);
@@ -937,7 +911,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                             }
                             const bool grow = top > m + kGrowth<FP8>;
                             const float next = grow ? top : m;
-                            const float keep = grow ? exp2_approx(m - next) : 1.0f;
+                            const float keep = grow ? exp2_fast(m - next) : 1.0f;
                             m = next;
                             l *= keep;
                             if (u > 0) { // O holds the sums up to step u - 1 once they are through
@@ -969,7 +943,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                                 const uint32_t i = c * 32 + 2 * j;
                                 const uint64_t x2 = pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
                                 const uint64_t e = FP8 ? add2(x2, base2) : fma2(x2, scale2, base2);
-                                const float a = exp2_approx(low2(e)), b = exp2_approx(high2(e));
+                                const float a = exp2_fast(low2(e)), b = exp2_fast(high2(e));
                                 if constexpr (FP8) {
                                     const float2 inv = *reinterpret_cast<const float2*>(scale + kKeyTile * 2 + in_tile + i);
                                     sum2 = fma2(pack2(a, b), pack2(inv.x, inv.y), sum2);
