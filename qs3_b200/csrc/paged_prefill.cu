@@ -341,7 +341,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
             copies.drain();
             return __all_sync(0xffffffffu, mbar_wait(b, parity, &bar.abort, p.err, code)) != 0;
         };
-        while (ok && this_segment(p, at, left, &seg)) {
+        while (ok && this_segment<false>(p, at, left, &seg)) {
             uint32_t seen_lo, seen_hi, unused;
             visible_keys(p.tiling, seg.rows.fresh, seg.pages.length, p.tiling.group.div(seg.row0), &seen_lo, &unused);
             visible_keys(p.tiling, seg.rows.fresh, seg.pages.length, p.tiling.group.div(seg.row0 + seg.nrows - 1), &unused, &seen_hi);
@@ -792,7 +792,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
             ++done[q];
             return true;
         };
-        while (ok && this_segment(p, at, left, &seg)) {
+        while (ok && this_segment<false>(p, at, left, &seg)) {
             const uint32_t n = uniform(seg.count);
             const bool second = TILES == 2 && uniform(seg.nrows) > kRowTile, score = warp == Shape::kScoreWarp;
             if (score)
@@ -835,7 +835,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 return __any_sync(0xffffffffu, v) != 0;
             return !group_all(1 + (warp & 3), 64, !v);
         };
-        while (ok && this_segment(p, at, left, &seg)) {
+        while (ok && this_segment<false>(p, at, left, &seg)) {
             const uint32_t steps = seg.count * STEPS;
             if (q * kRowTile < seg.nrows) {
                 const uint32_t r = q * kRowTile + tile_row;
@@ -973,16 +973,16 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                 if (!ok)
                     break;
                 const bool whole = seg.whole;
-                const bool scored = m != -INFINITY;
-                const float none = lo < hi ? __int_as_float(0x7fffffff) : 0.0f; // without a score: as in without_scores
+                if (whole && m == -INFINITY) // as in without_scores
+                    l = lo < hi ? __int_as_float(0x7fffffff) : 0.0f;
                 // in units of the sums: O counts 2^kSumUnit times too much
-                if (scored)
+                if (m != -INFINITY)
                     m += kSumUnit<FP8> - kTop<FP8>;
                 const uint32_t h = at.head * p.tiling.group.d + flat - token * p.tiling.group.d;
                 const size_t part_row = static_cast<size_t>(blockIdx.x * 2 + (seg.starts ? 1 : 0)) * Shape::kRows + r;
                 uint8_t* const out = p.out + (seg.rows.row0 + token) * p.out_token + h * p.out_head;
                 float* const part_o = p.part_o + part_row * D;
-                const float inv = whole ? (scored ? kSumFactor<FP8> / l : none) : kSumFactor<FP8>;
+                const float inv = whole ? (m == -INFINITY ? l : kSumFactor<FP8> / l) : kSumFactor<FP8>;
                 uint32_t x[32];
 #pragma unroll 1
                 for (uint32_t i = 0; i < D / 32 / (TILES == 1 ? 2 : 1); ++i) {
@@ -1014,7 +1014,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
                     mbar_arrive(&bar.o_free[q]);
                 if (live && whole && half == 0 && p.lse != nullptr)
                     p.lse[(seg.rows.row0 + token) * p.lse_token + h * p.lse_head]
-                        = scored ? (m + log2f(l)) * 0.693147180559945f : none == 0.0f ? -INFINITY : none;
+                        = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
                 if (live && !whole && half == 0)
                     p.part_ml[part_row] = make_float2(m, l);
             }
