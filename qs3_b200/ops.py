@@ -728,7 +728,7 @@ def rope_frequencies(rotary_dim: int, theta: float = 10000.0, *, scaling: str = 
 
 def _nonzero_scale(name, scale):
     """0 stands for the default in the descriptors, whose scales are f32."""
-    if C.c_float(scale).value == 0:
+    if -1e-30 < scale < 1e-30 and C.c_float(scale).value == 0:
         raise Qs3Error(capi.STATUS_INVALID_ARGUMENT, f"{name} must not be 0 in 32 bits")
     return scale
 
