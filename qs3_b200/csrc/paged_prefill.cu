@@ -313,6 +313,7 @@ attn_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant_
     chain_begin();
 
     const BlockRange range = find_range<Shape::kThreads>(p, reinterpret_cast<uint64_t*>(ring), blockIdx.x);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // boxes overwrite what the search wrote and read there
     __syncthreads();
     uint64_t left = range.end - range.begin;
     AttnPlace at = range.place;
