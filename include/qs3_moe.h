@@ -962,7 +962,8 @@ qsfi_status qs3_rope(qsfi_context* ctx, const qs3_rope_desc* desc);
 
 /* A pool of pages. bf16, or e4m3 codes with one f32 scale per token and KV head:
  *   scale = max(amax / 448, 1e-30),  code = e4m3_rn_sat(x * (1 / scale)).
- * A row with an infinity or a NaN reads back as NaNs. Scales are positive; V's below 1e-30 count as 1e-30 in attention. */
+ * A row with an infinity or a NaN reads back as NaNs. Scales are positive; V's below 1e-30 count as 1e-30 in attention.
+ * Where those of one sequence are 2^100 apart, weights below 2^-34 of the largest may be lost from a row's sum there. */
 typedef struct {
     qsfi_tensor4 k, v;             /* bf16 or e4m3 [pages, kv_heads, page_size, head_dim] */
     qsfi_tensor3 k_scale, v_scale; /* e4m3: f32 [pages, kv_heads, page_size] */
@@ -1023,14 +1024,16 @@ typedef struct {
                                are left as they are */
     qsfi_tensor2 lse;       /* optional f32 [rows, heads] */
     qsfi_tensor1 workspace; /* u8, qs3_paged_attention_workspace_size bytes, 256-byte aligned; calls that may overlap on
-                               the device need one each */
+                               the device need one each, layers that follow each other on a stream one for all */
     float sm_scale;         /* 0 means 1 / sqrt(head_dim) */
     uint32_t causal;
     uint32_t window;        /* 0: none; needs causal */
-    uint32_t max_q_len;     /* most new tokens of one sequence; 0: unknown. A larger number costs time, a smaller one too:
-                               results do not depend on it */
+    uint32_t max_q_len;     /* most new tokens of one sequence; 0: unknown. A larger number costs time, a smaller one too. It helps
+                               to choose the kernel and where work is cut, and with them the order of sums: results depend on
+                               it, as on the batch around a sequence, up to rounding */
     uint32_t max_kv_len;    /* likewise for kv_len */
 } qs3_paged_attention_desc;
+/* Enough for any call with that head_dim, whatever its tables say. */
 qsfi_status qs3_paged_attention_workspace_size(
     qsfi_context* ctx, uint32_t rows, uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, size_t* bytes
 );

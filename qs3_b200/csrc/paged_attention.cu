@@ -784,6 +784,8 @@ qsfi_status qs3_paged_attention(qsfi_context* ctx, const qs3_paged_attention_des
     // A tile of the streaming kernel has 16 rows. Up to there it is the faster one, or not far behind where the cache's stream
     // bounds both: 8 sequences of 700 tokens 21.5 us (chunk kernel 31.7), 64 of 4096 tokens with 4 new ones, 32 heads over 8,
     // 212 (236), over an e4m3 cache 191 (472), 128 of 4096 with 16 heads over 2 of 256 208 (200), L2 flushed before each call.
+    // The border is a bf16 cache's: just beyond it, with 5 new tokens, the 64 sequences take 246 us, and over an e4m3 cache, where
+    // the chunk kernel converts V anew for every row tile, 465 (with 4: 202 and 224, calls one after another). There it lies too low.
     const bool chunks = fresh * group > 16;
     uint32_t item_rows;
     if (chunks) {

@@ -10,7 +10,7 @@
 // Beside O (256 columns of 512) there is room for one score tile of each query tile and two of its weights. Scores are read into
 // registers at once, so that the next ones are on their way while their exponentials are taken: where weights took the place of
 // the scores that they came from, with two such tiles in turn, the scores waited for the sums of the step before the last
-// (8192 tokens of 16 heads of 256: 559 us). Eight warps take the exponentials, because one alone waits longer for each of its
+// (8192 tokens of 16 heads of 256: 559 us, 541; with heads of 128 the mixed batch of 12 sequences lost by it, 118 us, 124). Eight warps take the exponentials, because one alone waits longer for each of its
 // instructions than they take. One warp issues the scores and another the sums: every wait, product and commit costs its thread
 // 50 to 100 cycles, together twice as much as the products take.
 // m follows the row's maximum only when that has grown by 2^8 (the weights stay below 256, the sums take the difference):
@@ -29,9 +29,9 @@
 // small weights together need. So the weights are f16 and V is converted, by the four warps that fetch it: boxes to a staging
 // area, from there to registers, which makes room for the next ones, and to the ring. A fifth warp fetches K and a sixth the
 // scales. The row's sum takes V's scale out again.
-// 1021 tokens behind 31 111 cached ones take 670 us; with V's loads straight to registers, which fill what the first-level cache
-// has left beside so much shared memory, 765; with everything converted to f16, K too, 965. Shared memory is the bound: codes in
-// and out, V in f16, the products' operands and the scales.
+// 1021 tokens behind 31 111 cached ones take 676 us; with V's loads straight to registers, which fill what the first-level cache
+// has left beside so much shared memory, it was 765; with everything converted to f16, K too, 965. Shared memory is the bound: codes
+// in and out, V in f16, the products' operands and the scales.
 #include "paged_attention.cuh"
 #include "tcgen05.cuh"
 

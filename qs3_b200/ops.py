@@ -809,7 +809,8 @@ def kv_gather(ctx: Context, cache: PagedKvCache, table: PageTable, out_indptr, k
 
 
 def paged_attention_workspace_size(ctx: Context, q, cache: PagedKvCache, *, batch: int) -> int:
-    """Bytes of workspace that :func:`paged_attention` needs for q (or any with fewer rows) and a batch."""
+    """Bytes of workspace that :func:`paged_attention` needs for q (or any with fewer rows) and a batch. One serves all layers
+    that follow each other on a stream."""
     n = C.c_size_t(0)
     ctx.check(ctx._lib.qs3_paged_attention_workspace_size(ctx.handle, q.shape[0], batch, q.shape[1], cache.k.shape[1],
                                                           q.shape[2], C.byref(n)))
@@ -822,7 +823,7 @@ def paged_attention(ctx: Context, q, cache: PagedKvCache, table: PageTable, out,
     """``qs3_paged_attention``: attention of new tokens over the cache, which holds them already. q and out are bf16
     [rows, heads, head_dim]; rows ``q_indptr[b] .. q_indptr[b + 1]`` are the last tokens of sequence b (without
     ``q_indptr`` row b is). ``lse`` (f32 [rows, heads]) takes the log-sum-exp of each row. ``max_q_len`` and
-    ``max_kv_len``, where the host knows them, choose the kernels; results do not depend on them."""
+    ``max_kv_len``, where the host knows them, help to choose the kernels; results depend on them up to rounding."""
     d = capi.PagedAttentionDesc()
     _fill_paged(ctx, d, _PAGED_ATTENTION_DESC, cache, table, q, q_indptr, out, lse, workspace)
     d.sm_scale = 0.0 if sm_scale is None else _nonzero_scale("sm_scale", sm_scale)
