@@ -938,10 +938,10 @@ qsfi_status qs3_checkpoint_load_moe_layer(
 /* ---- gated attention between its projections and its output: rotary positions, the paged KV cache as it is written
  * and read back, attention of new tokens over it (upstream: FlashInfer calls, qsfi_attn.cu and qsfi_norm_rope.cu; the
  * page table is upstream's CSR one, src/runtime.rs:99-181). Tensors have a contiguous innermost dimension, 16-byte
- * aligned rows and any other strides. head_dim is a multiple of 8 up to 256. What a call writes may not lie over its other
- * operands, but for the outputs that may be their inputs; rows, log-sum-exps and workspaces that do are refused, parts of one buffer that
- * lie between each other are not. A pool is compared with its own parts alone: a page table may name other pages of it than
- * those that rows are taken from or put to. ---- */
+ * aligned rows and any other strides. head_dim is a multiple of 8 up to 256. A step without rows makes no call: every extent
+ * is positive. What a call writes may not lie over its other operands, but for the outputs that may be their inputs: rows,
+ * log-sum-exps and workspaces that do are refused, parts of one buffer that lie between each other are not. A pool is compared
+ * with its own parts alone, as a page table may name other pages of it than those that rows are taken from or put to. ---- */
 
 /* Rotary positions. Element pairs of the first r = 2 * inv_freq.shape[0] elements of every head are turned by the angle
  * positions[t] * inv_freq[j]:
